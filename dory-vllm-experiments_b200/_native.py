@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -24,6 +25,8 @@ FLAG_RAW_QKV, FLAG_MULTI_TOKEN, FLAG_SHARED_CACHE, FLAG_OVERLAP_LAUNCH = 1, 2, 4
 FLAG_FMA_CONSUMER = 16
 # DORY_QKNORM_*
 QKNORM_WRITE_CACHE = 1
+# DORY_ROTARY_*
+ROTARY_INTERLEAVED, ROTARY_INVERSE, ROTARY_NORM = 1, 2, 4
 # DORY_DEVERR_*
 DEVERR_BLOCK_OOB, DEVERR_SLOT_OOB, DEVERR_OFFSET_ALIGN, DEVERR_WAIT_TIMEOUT = 1, 2, 4, 8
 DEVERR_POSITION_OOB = 16
@@ -38,7 +41,8 @@ EXPORTS = ("dory_decode_abi_version", "dory_decode_params_bytes", "dory_decode_s
            "dory_decode_last_error", "dory_decode_attention_static_scratch",
            "dory_decode_static_scratch_fetch_errors",
            "dory_qk_norm_params_bytes", "dory_qk_norm_cache", "dory_qkvg_params_bytes",
-           "dory_qkvg_epilogue", "dory_residual_params_bytes", "dory_residual_update")
+           "dory_qkvg_epilogue", "dory_residual_params_bytes", "dory_residual_update",
+           "dory_rotary_params_bytes", "dory_rotary_embed", "dory_rotary_append")
 
 # Size of the library's static scratch array (DORY_DECODE_STATIC_SCRATCH_BYTES).
 STATIC_SCRATCH_BYTES = 4 << 20
@@ -98,6 +102,35 @@ class DoryResidualParams(ctypes.Structure):
     ]
 
 
+class DoryRotaryParams(ctypes.Structure):
+    """Mirror of DoryRotaryParams (include/dory_decode.h); field order is the ABI."""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("positions", _vp), ("cos_sin", _vp), ("sqk", _vp),
+        ("slot_mapping", _vp), ("q_out", _vp), ("k_out", _vp), ("key_cache", _vp),
+        ("value_cache", _vp), ("error_word", _vp),
+        ("q_stride_token", _i64), ("q_stride_head", _i64), ("k_stride_token", _i64),
+        ("k_stride_head", _i64), ("v_stride_token", _i64), ("v_stride_head", _i64),
+        ("q_out_stride_token", _i64), ("q_out_stride_head", _i64), ("k_out_stride_token", _i64),
+        ("k_out_stride_head", _i64), ("stride_block", _i64), ("stride_offset", _i64),
+        ("stride_head", _i64), ("num_cache_blocks", _i64), ("max_position", _i64),
+        ("sqk_factor", _f32), ("eps", _f32), ("k_scale", _f32), ("v_scale", _f32),
+        ("num_tokens", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("block_size", _i32), ("io_dtype", _i32), ("cos_sin_dtype", _i32),
+        ("positions_dtype", _i32), ("sqk_dtype", _i32), ("kv_dtype", _i32), ("flags", _u32),
+    ]
+
+
+_FORMAT = {_vp: "P", _i64: "q", _f32: "f", _i32: "i", _u32: "I"}
+
+
+def packer(cls):
+    """`pack(*values)` of a parameter struct's fields, in order, as the bytes the library
+    reads (a null pointer is 0): one call per launch instead of an attribute set per field."""
+    fmt = struct.Struct("@" + "".join(_FORMAT[kind] for _, kind in cls._fields_))
+    assert fmt.size == ctypes.sizeof(cls)
+    return fmt.pack
+
+
 _lib = None
 
 
@@ -142,6 +175,11 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib.dory_residual_params_bytes.argtypes = []
     lib.dory_residual_update.restype = _i32
     lib.dory_residual_update.argtypes = [ctypes.POINTER(DoryResidualParams), _vp]
+    lib.dory_rotary_params_bytes.restype = _i64
+    lib.dory_rotary_params_bytes.argtypes = []
+    for name in ("dory_rotary_embed", "dory_rotary_append"):
+        getattr(lib, name).restype = _i32
+        getattr(lib, name).argtypes = [_vp, _vp]
     if lib.dory_decode_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {lib.dory_decode_abi_version()} != {ABI_VERSION}")
     if lib.dory_decode_params_bytes() != ctypes.sizeof(DoryDecodeParams):
@@ -156,6 +194,9 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     if lib.dory_residual_params_bytes() != ctypes.sizeof(DoryResidualParams):
         raise RuntimeError(f"{path}: DoryResidualParams is {lib.dory_residual_params_bytes()} "
                            f"bytes, the binding's is {ctypes.sizeof(DoryResidualParams)}")
+    if lib.dory_rotary_params_bytes() != ctypes.sizeof(DoryRotaryParams):
+        raise RuntimeError(f"{path}: DoryRotaryParams is {lib.dory_rotary_params_bytes()} "
+                           f"bytes, the binding's is {ctypes.sizeof(DoryRotaryParams)}")
     _lib = lib
     return lib
 

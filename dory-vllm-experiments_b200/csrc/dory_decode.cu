@@ -56,6 +56,7 @@
 #include <mutex>
 
 #include "../../include/dory_decode.h"
+#include "dory_common.h"
 
 namespace {
 
@@ -2421,6 +2422,14 @@ int32_t fail(int32_t status, const char* fmt, ...) {
   va_end(ap);
   return status;
 }
+
+}  // namespace
+
+int32_t dory::set_error(int32_t status, const char* message) {
+  return ::fail(status, "%s", message);  // the one above, which records the message
+}
+
+namespace {
 
 template <int HD, int NT, int NS, bool SS, bool DM, bool FMA = false, bool KV8 = false,
           bool WIDE = false, bool SHK = false>

@@ -81,8 +81,8 @@ enum {
   DORY_DEVERR_SLOT_OOB = 2u,      /* an append slot outside the cache                     */
   DORY_DEVERR_OFFSET_ALIGN = 4u,  /* a cache offset not a multiple of 8 elements          */
   DORY_DEVERR_WAIT_TIMEOUT = 8u,  /* a pipeline wait gave up after its iteration limit    */
-  DORY_DEVERR_POSITION_OOB = 16u  /* dory_qkvg_epilogue: a rotary position outside
-                                   * [0, max_position); that token's q and k are zero      */
+  DORY_DEVERR_POSITION_OOB = 16u  /* a rotary position outside [0, max_position); that token's
+                                   * q and k are zero                                       */
 };
 
 /*
@@ -345,6 +345,85 @@ int64_t dory_residual_params_bytes(void);
 
 /* One launch of the residual update on `stream` (one CTA per token). */
 int32_t dory_residual_update(const DoryResidualParams* params, void* stream);
+
+/*
+ * Rotary positions, and the append of a chunk of new tokens to the paged cache with the
+ * rotation applied on the way: the input side of chunk attention (prompts and parts of
+ * them, ragged batches, single tokens).  No counterpart in the reference, whose prompts run
+ * on vLLM's own rotary embedding and cache write.
+ *
+ * The first rotary_dim dims of a head are pairs: dims (i, i + rotary_dim / 2), or (2i, 2i + 1)
+ * with DORY_ROTARY_INTERLEAVED.  Pair i of a token at position p becomes
+ *   (a c - b s, b c + a s),  c = cos_sin[p][i],  s = cos_sin[p][rotary_dim / 2 + i]
+ * in FP32 (s negated with DORY_ROTARY_INVERSE: the inverse rotation, which is also the
+ * rotation's gradient); the other dims are copied.  A scaled context is the caller's table.
+ * A position outside [0, max_position) gives zero q and k and is reported
+ * (DORY_DEVERR_POSITION_OOB in error_word; not for a padding token of the append).
+ *
+ * dory_rotary_embed writes q_out and, where k is given, k_out, in the inputs' type; an output
+ * may be its input itself (same pointer and strides).
+ *
+ * dory_rotary_append writes q_out (BF16; q and q_out may be NULL) and the cache rows of k and
+ * v at slot_mapping[t] (negative: a padding token, no row is written; outside the cache:
+ * reported as DORY_DEVERR_SLOT_OOB and skipped).  With DORY_ROTARY_NORM the rotated q and k
+ * are brought to unit length first, as the raw decode calls do:
+ *   q_out = bf16((float(sqk[h]) * sqk_factor)^2 * q * rsqrt(sum q^2 + eps)),
+ *   k     = bf16(k * rsqrt(sum k^2 + eps)).
+ * BF16 caches take bf16(k), bf16(v); FP8 caches e4m3(bf16(k) / k_scale), e4m3(bf16(v) /
+ * v_scale), rounded to nearest even and saturated at +-448, as the raw decode calls quantise
+ * theirs.  Two tokens of one call must not name the same slot.
+ */
+#define DORY_ROTARY_INTERLEAVED 1u
+#define DORY_ROTARY_INVERSE 2u
+#define DORY_ROTARY_NORM 4u
+typedef struct DoryRotaryParams {
+  const void* q;                  /* [T, NH, HD] of io_dtype, unit last stride                */
+  const void* k;                  /* [T, NKV, HD] of io_dtype (embed: optional)               */
+  const void* v;                  /* append: [T, NKV, HD] of io_dtype                         */
+  const void* positions;          /* [T], int64 or int32 (positions_dtype)                    */
+  const void* cos_sin;            /* [max_position, rotary_dim] of cos_sin_dtype; append: NULL
+                                   * with rotary_dim 0 leaves q and k unrotated               */
+  const void* sqk;                /* NORM: [NH * HD] of sqk_dtype                             */
+  const int64_t* slot_mapping;    /* append: int64 [T]                                        */
+  void* q_out;                    /* embed: io_dtype, append: BF16; [T, NH, HD]               */
+  void* k_out;                    /* embed: io_dtype [T, NKV, HD]                             */
+  void* key_cache;                /* append: [num_cache_blocks, block_size, NKV, HD] view     */
+  void* value_cache;              /* append: same strides as key_cache, unit last stride      */
+  uint32_t* error_word;           /* optional: DORY_DEVERR_* bits are or-ed in                */
+  int64_t q_stride_token, q_stride_head;
+  int64_t k_stride_token, k_stride_head;
+  int64_t v_stride_token, v_stride_head;
+  int64_t q_out_stride_token, q_out_stride_head;
+  int64_t k_out_stride_token, k_out_stride_head;
+  int64_t stride_block;           /* key_cache.stride(0) */
+  int64_t stride_offset;          /* key_cache.stride(1) */
+  int64_t stride_head;            /* key_cache.stride(2) */
+  int64_t num_cache_blocks;       /* key_cache.shape[0] */
+  int64_t max_position;
+  float sqk_factor;
+  float eps;
+  float k_scale;                  /* FP8 caches: positive, finite */
+  float v_scale;
+  int32_t num_tokens;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;               /* embed: up to 1024; append: 64, 128 or 256 */
+  int32_t rotary_dim;             /* even, at most head_dim */
+  int32_t block_size;
+  int32_t io_dtype;               /* DoryDType of q, k, v (F32, BF16, F16) */
+  int32_t cos_sin_dtype;          /* DoryDType */
+  int32_t positions_dtype;        /* 0: int64, 1: int32 */
+  int32_t sqk_dtype;              /* DoryDType */
+  int32_t kv_dtype;               /* 0 or DORY_DTYPE_BF16, or DORY_DTYPE_FP8_E4M3 */
+  uint32_t flags;                 /* DORY_ROTARY_* */
+} DoryRotaryParams;
+
+/* sizeof(DoryRotaryParams) as compiled into the library. */
+int64_t dory_rotary_params_bytes(void);
+
+/* One launch each on `stream`. */
+int32_t dory_rotary_embed(const DoryRotaryParams* params, void* stream);
+int32_t dory_rotary_append(const DoryRotaryParams* params, void* stream);
 
 /* Copies the device error word (DORY_DEVERR_* bits) to *flags_out, synchronising `stream`;
  * clears it when `clear` is non-zero.  The only entry point that waits on the device. */
