@@ -42,7 +42,8 @@ EXPORTS = ("dory_decode_abi_version", "dory_decode_params_bytes", "dory_decode_s
            "dory_decode_static_scratch_fetch_errors",
            "dory_qk_norm_params_bytes", "dory_qk_norm_cache", "dory_qkvg_params_bytes",
            "dory_qkvg_epilogue", "dory_residual_params_bytes", "dory_residual_update",
-           "dory_rotary_params_bytes", "dory_rotary_embed", "dory_rotary_append")
+           "dory_rotary_params_bytes", "dory_rotary_embed", "dory_rotary_append",
+           "dory_chunk_params_bytes", "dory_chunk_scratch_bytes", "dory_chunk_attention")
 
 # Size of the library's static scratch array (DORY_DECODE_STATIC_SCRATCH_BYTES).
 STATIC_SCRATCH_BYTES = 4 << 20
@@ -120,6 +121,21 @@ class DoryRotaryParams(ctypes.Structure):
     ]
 
 
+class DoryChunkParams(ctypes.Structure):
+    """Mirror of DoryChunkParams (include/dory_decode.h); field order is the ABI."""
+    _fields_ = [
+        ("q", _vp), ("key_cache", _vp), ("value_cache", _vp), ("block_tables", _vp),
+        ("query_start", _vp), ("seq_lens", _vp), ("gate", _vp), ("out", _vp), ("scratch", _vp),
+        ("scratch_bytes", _i64), ("q_stride_token", _i64), ("q_stride_head", _i64),
+        ("out_stride_token", _i64), ("gate_stride_token", _i64), ("table_stride", _i64),
+        ("stride_block", _i64), ("stride_offset", _i64), ("stride_head", _i64),
+        ("num_cache_blocks", _i64), ("softmax_scale", _f32), ("k_scale", _f32),
+        ("v_scale", _f32), ("num_tokens", _i32), ("num_seqs", _i32), ("max_blocks", _i32),
+        ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32),
+        ("window", _i32), ("gate_dtype", _i32), ("kv_dtype", _i32),
+    ]
+
+
 _FORMAT = {_vp: "P", _i64: "q", _f32: "f", _i32: "i", _u32: "I"}
 
 
@@ -127,7 +143,7 @@ def packer(cls):
     """`pack(*values)` of a parameter struct's fields, in order, as the bytes the library
     reads (a null pointer is 0): one call per launch instead of an attribute set per field."""
     fmt = struct.Struct("@" + "".join(_FORMAT[kind] for _, kind in cls._fields_))
-    assert fmt.size == ctypes.sizeof(cls)
+    assert fmt.size <= ctypes.sizeof(cls) < fmt.size + 8  # but for padding at the end
     return fmt.pack
 
 
@@ -180,6 +196,12 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     for name in ("dory_rotary_embed", "dory_rotary_append"):
         getattr(lib, name).restype = _i32
         getattr(lib, name).argtypes = [_vp, _vp]
+    lib.dory_chunk_params_bytes.restype = _i64
+    lib.dory_chunk_params_bytes.argtypes = []
+    lib.dory_chunk_scratch_bytes.restype = _i64
+    lib.dory_chunk_scratch_bytes.argtypes = [_i32, _i32, _i32]
+    lib.dory_chunk_attention.restype = _i32
+    lib.dory_chunk_attention.argtypes = [_vp, _vp]
     if lib.dory_decode_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {lib.dory_decode_abi_version()} != {ABI_VERSION}")
     if lib.dory_decode_params_bytes() != ctypes.sizeof(DoryDecodeParams):
@@ -197,6 +219,9 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     if lib.dory_rotary_params_bytes() != ctypes.sizeof(DoryRotaryParams):
         raise RuntimeError(f"{path}: DoryRotaryParams is {lib.dory_rotary_params_bytes()} "
                            f"bytes, the binding's is {ctypes.sizeof(DoryRotaryParams)}")
+    if lib.dory_chunk_params_bytes() != ctypes.sizeof(DoryChunkParams):
+        raise RuntimeError(f"{path}: DoryChunkParams is {lib.dory_chunk_params_bytes()} "
+                           f"bytes, the binding's is {ctypes.sizeof(DoryChunkParams)}")
     _lib = lib
     return lib
 

@@ -18,7 +18,8 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
-SOURCES = [HERE / "csrc" / "dory_decode.cu", HERE / "csrc" / "dory_rotary.cu"]
+SOURCES = [HERE / "csrc" / name
+           for name in ("dory_decode.cu", "dory_rotary.cu", "dory_chunk.cu")]
 HEADERS = [ROOT / "include" / "dory_decode.h", HERE / "csrc" / "dory_common.h"]
 LIBRARY = HERE / "libdory_decode.so"
 OBJECTS = HERE / "_build"

@@ -425,6 +425,72 @@ int64_t dory_rotary_params_bytes(void);
 int32_t dory_rotary_embed(const DoryRotaryParams* params, void* stream);
 int32_t dory_rotary_append(const DoryRotaryParams* params, void* stream);
 
+/*
+ * Attention of a chunk of new tokens over the paged cache: prompts, parts of prompts whose
+ * earlier part is cached, drafted tokens, and single tokens among them, as one ragged batch.
+ * No counterpart in the reference, whose prompts run on vLLM's attention.
+ *
+ * Sequence i owns the query rows t in [query_start[i], query_start[i + 1]), its last n =
+ * query_start[i + 1] - query_start[i] positions: row query_start[i] + j is at position
+ * p = seq_lens[i] - n + j and attends the cached positions c <= p, with a window c > p - window:
+ *   out[t][h] = gate[t][h] * sum_c softmax_c(softmax_scale * q[t][h] . K[c]) V[c],
+ * K and V of the head's KV head at block_tables[i][c / block_size], row c % block_size (the
+ * chunk's own rows already appended, dory_rotary_append).  Scores, softmax statistics and sums
+ * are FP32; the weights enter the V product rounded to 11 bits or more relative to the row's
+ * largest (BF16 caches: 8 bits).
+ *
+ * A row that sees no position gives zeros; rows outside every sequence keep their contents;
+ * seq_lens 0 (a padded request) gives zero rows.  Positions whose block id lies outside the
+ * cache, or beyond the table's width, are left out and reported (DORY_DEVERR_BLOCK_OOB).
+ * Nothing else of the cache is read into a result: unused rows of a page may hold anything.
+ */
+typedef struct DoryChunkParams {
+  const void* q;                  /* BF16 [T, NH, HD], unit last stride, 16-byte aligned rows */
+  const void* key_cache;          /* [num_cache_blocks, block_size, NKV, HD] view            */
+  const void* value_cache;        /* same strides as key_cache, unit last stride             */
+  const int32_t* block_tables;    /* int32 [S, max_blocks], rows table_stride apart          */
+  const int32_t* query_start;     /* int32 [S + 1], not decreasing, within [0, T]            */
+  const int32_t* seq_lens;        /* int32 [S]: positions including the chunk's own          */
+  const void* gate;               /* optional [T, NH * HD] of gate_dtype                     */
+  void* out;                      /* BF16 [T, NH * HD], 16-byte aligned rows                 */
+  void* scratch;                  /* dory_chunk_scratch_bytes(), zeroed once by
+                                   * dory_decode_scratch_init(); word 0 is the error word
+                                   * (dory_decode_fetch_errors); calls that can overlap on the
+                                   * GPU need a scratch each                                  */
+  int64_t scratch_bytes;
+  int64_t q_stride_token, q_stride_head;
+  int64_t out_stride_token;
+  int64_t gate_stride_token;
+  int64_t table_stride;
+  int64_t stride_block;           /* key_cache.stride(0) */
+  int64_t stride_offset;          /* key_cache.stride(1) */
+  int64_t stride_head;            /* key_cache.stride(2) */
+  int64_t num_cache_blocks;       /* key_cache.shape[0] */
+  float softmax_scale;            /* positive, finite */
+  float k_scale;                  /* FP8 caches: positive, finite */
+  float v_scale;
+  int32_t num_tokens;             /* T */
+  int32_t num_seqs;               /* S */
+  int32_t max_blocks;             /* block_tables.shape[1] */
+  int32_t num_heads;              /* a multiple of num_kv_heads, at most 64 times it */
+  int32_t num_kv_heads;
+  int32_t head_dim;               /* 64, 128 or 256 (FP8 caches: 128 or 256) */
+  int32_t block_size;             /* a multiple of 16 */
+  int32_t window;                 /* 0: all earlier positions */
+  int32_t gate_dtype;             /* DoryDType */
+  int32_t kv_dtype;               /* 0 or DORY_DTYPE_BF16, or DORY_DTYPE_FP8_E4M3 */
+} DoryChunkParams;
+
+/* sizeof(DoryChunkParams) as compiled into the library. */
+int64_t dory_chunk_params_bytes(void);
+
+/* Bytes of scratch a chunk call needs on the current device, whatever its tokens (partial
+ * results of the pieces of work that were cut between SMs); 0 for an unsupported shape. */
+int64_t dory_chunk_scratch_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/* Chunk attention on `stream`. */
+int32_t dory_chunk_attention(const DoryChunkParams* params, void* stream);
+
 /* Copies the device error word (DORY_DEVERR_* bits) to *flags_out, synchronising `stream`;
  * clears it when `clear` is non-zero.  The only entry point that waits on the device. */
 int32_t dory_decode_fetch_errors(void* scratch, uint32_t* flags_out, int32_t clear, void* stream);

@@ -52,34 +52,47 @@ def normalised(y: torch.Tensor, eps: float, weight: torch.Tensor | None = None,
 
 def chunk_attention(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, tables: torch.Tensor,
                     query_start, seq_lens, window: int, scale: float, gate=None):
-    """q [T, NH, D]; key / value [blocks, B, NKV, D] (already dequantised); tables [S, width].
-    -> (out FP64 [T, NH * D], softmax-weighted mean of |v|, FP64, same shape).  Rows no
-    sequence owns are NaN; a token that sees nothing gives zero; positions whose block id is
-    outside the cache (or beyond the table) are left out."""
+    """q [T, NH, D]; key / value [blocks, B, NKV, D] (already dequantised); tables [S, width];
+    any device.  -> (out FP64 [T, NH * D], softmax-weighted mean of |v|, FP64, same shape).
+    Rows no sequence owns are NaN; a token that sees nothing gives zero; positions whose block
+    id is outside the cache (or beyond the table) are left out.  Hidden positions take no part
+    at all, whatever they hold."""
     T, NH, D = q.shape
     blocks, B, NKV, _ = key.shape
-    G = NH // NKV
-    out = torch.full((T, NH, D), float("nan"), dtype=torch.float64)
+    G, dev = NH // NKV, q.device
+    out = torch.full((T, NH, D), float("nan"), dtype=torch.float64, device=dev)
     size = torch.zeros_like(out)
-    q, key, value = q.double(), key.double(), value.double()
     for i, length in enumerate(int(n) for n in seq_lens):
         t0, t1 = int(query_start[i]), int(query_start[i + 1])
-        for t in range(t0, t1):
-            p = length - (t1 - t0) + (t - t0)
-            low = max(0, p + 1 - window) if window else 0
-            pos = torch.arange(low, min(p, length - 1) + 1)
-            pos = pos[pos // B < tables.shape[1]]
-            ids = tables[i, pos // B].long()
-            ok = (ids >= 0) & (ids < blocks)
-            pos, ids = pos[ok], ids[ok]
-            out[t], size[t] = 0.0, 0.0
-            if not len(pos):
-                continue
-            k, v = key[ids, pos % B], value[ids, pos % B]  # [n, NKV, D]
-            for g in range(NKV):
-                rows = slice(g * G, (g + 1) * G)
-                w = torch.softmax(q[t, rows] @ k[:, g].T * scale, dim=-1)
-                out[t, rows], size[t, rows] = w @ v[:, g], w @ v[:, g].abs()
+        if t1 <= t0:
+            continue
+        out[t0:t1], size[t0:t1] = 0.0, 0.0
+        p = length - (t1 - t0) + torch.arange(t1 - t0, device=dev)[:, None]
+        pos = torch.arange(max(0, min(length, tables.shape[1] * B)), device=dev)
+        ids = tables[i].to(dev)[pos // B].long()
+        ok = (ids >= 0) & (ids < blocks)
+        pos, ids = pos[ok], ids[ok]
+        seen = pos[None] <= p
+        if window:
+            seen &= pos[None] > p - window
+        some = seen.any(0)
+        pos, ids, seen = pos[some], ids[some], seen[:, some]
+        if not len(pos):
+            continue
+        rows = seen.any(1)
+        for g in range(NKV):
+            k, v = key[ids, pos % B, g].double(), value[ids, pos % B, g].double()
+            finite = torch.isfinite(v).all()
+            for h in range(g * G, (g + 1) * G):
+                s = (q[t0:t1, h].double() @ k.T * scale).masked_fill(~seen, -torch.inf)
+                w = torch.where(rows[:, None], torch.softmax(s, dim=-1), 0.0)
+                if finite:
+                    out[t0:t1, h], size[t0:t1, h] = w @ v, w @ v.abs()
+                else:  # a hidden Inf or NaN must not reach a row
+                    for j in range(t1 - t0):
+                        see = seen[j]
+                        out[t0 + j, h] = w[j, see] @ v[see]
+                        size[t0 + j, h] = w[j, see] @ v[see].abs()
     out, size = out.reshape(T, NH * D), size.reshape(T, NH * D)
     if gate is not None:
         out, size = out * gate.double(), size * gate.double().abs()
