@@ -20,7 +20,8 @@ HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
 SOURCES = [HERE / "csrc" / name
            for name in ("dory_decode.cu", "dory_rotary.cu", "dory_chunk.cu")]
-HEADERS = [ROOT / "include" / "dory_decode.h", HERE / "csrc" / "dory_common.h"]
+HEADERS = [ROOT / "include" / "dory_decode.h", HERE / "csrc" / "dory_common.h",
+           HERE / "csrc" / "dory_sm100.cuh"]
 LIBRARY = HERE / "libdory_decode.so"
 OBJECTS = HERE / "_build"
 

@@ -1,9 +1,38 @@
 // dory_chunk.cu — attention of a chunk of new tokens over the paged cache
 // (dory_chunk_attention; the C ABI is in include/dory_decode.h).
 //
-// chunk_rows: one warp per (token, head) row.  Lanes take 32 positions at a time for the scores
-// (q from shared memory), then HD / 32 dims each for the weighted sum, with a running maximum
-// and sum.
+// out[t][h] = gate * sum_c softmax_c(scale q.k_c) v_c over the positions c a token sees.
+//
+// Shape of the work.  The G query heads of a KV head see the same keys, so G x (128 / G) rows
+// (token, head) fill the 128 rows of a tensor-core tile; an item of work is one or two such
+// tiles (kTiles) of one sequence and KV head, with the 128-position cache tiles they see.  A
+// unit is one cache tile of one item.  All units of the batch, in (sequence, KV head, item)
+// order, are cut into equal consecutive pieces, one per SM: causal triangles, ragged lengths
+// and a few rows over a long cache all balance by themselves.  An item cut between SMs leaves
+// FP32 partial results (unnormalised sum, maximum, sum of weights) which a second small launch
+// joins, so results do not depend on arrival order.
+//
+// chunk_kernel, one CTA per SM, warp roles:
+//   scheduler  derives the SM's piece from query_start / seq_lens on the device (no host read,
+//              so a captured graph follows new lengths) and hands items to the others;
+//   loader     tensor copies: the queries, and K and V tiles page by page through the block
+//              table into a ring; pages outside the item's positions, and bad block ids, load
+//              as zeros without touching memory;
+//   products   tcgen05: S = Q K^T into tensor memory, O += P V with P read from there;
+//   softmax    two warpgroups, a row (or half a row) per thread: scores to registers, running
+//              maximum, exponentials, P back to tensor memory as 16-bit floats, and at the
+//              end of an item O / sum, gate and store.
+// With 64/128-dim heads an item has two tiles and the products of one overlap the softmax of
+// the other.  With 256-dim heads tensor memory holds one tile's O and two score buffers, and
+// the two warpgroups share each tile's columns.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8: the weights stay below
+// 2^8, far from the range's end, and most tiles touch O not at all.
+//
+// Positions no row of the item sees (behind the sequence, before the window) may hold anything,
+// so their V rows are zeroed in shared memory (0 x NaN would reach the sum).  A position that
+// some rows see and others do not can still hold Inf or NaN: a row whose O comes out
+// non-finite from finite weights is recomputed from its own positions alone (redo_row).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -11,14 +40,29 @@
 #include <math.h>
 #include <string.h>
 
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "dory_common.h"
+#include "dory_sm100.cuh"
 
 namespace {
 
+using namespace sm100;
 using dory::aligned16;
 using dory::fail;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kM = 128;              // rows of a tensor-core tile
+constexpr int kN = 128;              // positions of a cache tile
+constexpr int kChunkBytes = kN * 128;  // 64 columns of a tile: 128 rows of 128 bytes
+constexpr int kQueue = 4;            // items handed out ahead
+constexpr int kBadRing = 16;         // tiles whose bad-page masks are kept
+constexpr int kMaxPosition = 1 << 30;
+constexpr float kSlack = 8.0f;       // log2 a row's maximum may grow before O is rescaled
+// ~4 s, then give up: above a whole item of redo_row, which the other roles wait for.
+constexpr long long kWaitLimitCycles = 8000000000LL;
 
 struct ChunkArgs {
   const __nv_bfloat16* q;
@@ -33,6 +77,17 @@ struct ChunkArgs {
   int64_t q_t, q_h, out_t, gate_t, table_stride, sb, so, sh, blocks;
   float scale_log2, k_scale, v_scale;
   int T, S, max_blocks, NH, NKV, G, B, window, gate_dtype;
+  int TB;             // tokens of a tile: 128 / G
+  int copy_rows;      // rows of a tensor copy: the largest power of two dividing B, up to 128
+  int copy_shift;     // its logarithm
+  int table_span;     // positions the table names, at most kMaxPosition
+  int min_units;      // cache tiles an SM takes at least
+  int32_t* joins;     // [CTAs][8]: the item cut at the end of each CTA's piece
+  float2* part_ml;    // [2 CTAs][rows]: (maximum in log2 units, sum of weights)
+  float* part_o;      // [2 CTAs][rows][HD]
+};
+struct Maps {
+  CUtensorMap q, k, v;
 };
 
 __device__ __forceinline__ float load_gate(const ChunkArgs& a, int64_t i) {
@@ -140,6 +195,1074 @@ __global__ void __launch_bounds__(128) chunk_rows(const ChunkArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------------------
+// The tensor-core kernel
+// ------------------------------------------------------------------------------------
+template <int HD>
+struct Shape {
+  static constexpr int kTiles = HD == 256 ? 1 : 2;           // tensor-core tiles of an item
+  static constexpr int kCols = HD < 128 ? HD : 128;          // columns of a ring stage
+  static constexpr int kHalves = HD / kCols;                 // stages of a K (or V) tile
+  static constexpr int kStageBytes = kCols / 64 * kChunkBytes;
+  static constexpr int kStages = HD == 64 ? 8 : 5;
+  static constexpr int kQBytes = kTiles * HD / 64 * kChunkBytes;
+  static constexpr int kScoreCols = kTiles == 2 ? kN : kN / 2;  // of a row, per softmax thread
+  static constexpr int kOutCols = kTiles == 2 ? HD : HD / 2;
+  static constexpr int kItemRows = kTiles * kM;
+  // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
+  static constexpr int kO = 2 * kN;
+  static constexpr int kOStride = HD <= 128 ? 128 : 0;       // between the tiles' O
+};
+
+constexpr int kSoftmaxWarps = 8;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kPlanWarp = 10;
+constexpr int kThreads = 12 * 32;  // three whole warpgroups: registers are handed over by group
+// Registers a thread: 168 at launch (384 threads, 64,512 in all); the softmax groups, which hold
+// a row's 128 scores, take what the third group gives up: 2 x 128 x 200 + 128 x 104 = 64,512.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+
+enum : int { kItemEnd = 1 };
+struct Item {
+  int flags;
+  int kv0, kvn;      // cache tiles of this piece: [kv0, kv0 + kvn)
+  int tok0, ntok;    // query rows of the batch
+  int pos0;          // position of the first (negative: before the sequence)
+  int kvh, seq;
+  int cap;           // positions of the sequence that the table names
+  int slot;          // partial-result slot, -1: the whole item is here
+  int pad[6];
+};
+
+template <int HD>
+struct Control {  // shared memory behind the tiles
+  alignas(8) uint64_t kv_full[Shape<HD>::kStages], kv_empty[Shape<HD>::kStages];
+  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], item_full[kQueue],
+      item_empty[kQueue], drained;
+  Item items[kQueue];
+  uint32_t bad[kBadRing];
+  uint32_t tmem;
+  int abort;
+  float swap[2][2][kM];  // the warpgroups' halves of a row's maximum and sum (256-dim heads)
+};
+
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
+                                       uint32_t* err) {
+  const long long start = clock64();
+  while (!mbar_try(bar, parity)) {
+    if (*abort) return false;
+    if (clock64() - start > kWaitLimitCycles) {
+      *abort = 1;
+      atomicOr(err, DORY_DEVERR_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+// One thread's wait; false once any role of the CTA has given up.
+__device__ __forceinline__ bool wait_one(const uint64_t& bar, uint32_t parity, int* abort,
+                                         uint32_t* err) {
+  const uint32_t b = smem_u32(&bar);
+  return mbar_try(b, parity) || wait_slow(b, parity, abort, err);
+}
+// A whole warp's wait, the same answer in every lane.
+__device__ __forceinline__ bool wait_warp(const uint64_t& bar, uint32_t parity, int* abort,
+                                          uint32_t* err) {
+  const uint32_t b = smem_u32(&bar);
+  bool ok = mbar_try(b, parity);
+  if (!__all_sync(0xffffffffu, ok)) {
+    if (!ok) ok = wait_slow(b, parity, abort, err);
+    return __all_sync(0xffffffffu, ok);
+  }
+  return true;
+}
+
+// The cache tiles that rows at positions [p0, p0 + n) see: their number and the first.
+__device__ __forceinline__ int tiles_seen(int p0, int n, int cap, int window, int& first) {
+  const int hi = min(p0 + n, cap), lo = window ? max(0, p0 - window + 1) : 0;
+  first = 0;
+  if (n <= 0 || hi <= lo) return 0;
+  first = lo / kN;
+  return (hi + kN - 1) / kN - first;
+}
+// Those of tile t of an item within this CTA's piece: [b, e).
+template <int HD>
+__device__ __forceinline__ void tile_range(const ChunkArgs& a, const Item& it, int t, int& b, int& e) {
+  const int skip = t * a.TB;
+  const int n = tiles_seen(it.pos0 + skip, min(it.ntok - skip, a.TB), it.cap, a.window, b);
+  e = b + n;
+  b = max(b, it.kv0);
+  e = min(e, it.kv0 + it.kvn);
+  if (e < b) e = b;
+}
+
+// ---- scheduler ----
+struct Seq {
+  int t0, n, pos, cap;  // first row, rows, position of the first, positions to see
+};
+__device__ __forceinline__ Seq sequence(const ChunkArgs& a, int i) {
+  Seq s{0, 0, 0, 0};
+  if (i < a.S) {
+    int t1;
+    rows_of(a, i, s.t0, t1);
+    s.n = t1 - s.t0;
+    const int len = min(max(a.seq_lens[i], 0), kMaxPosition);
+    s.pos = len - s.n;
+    s.cap = min(len, a.table_span);
+  }
+  return s;
+}
+__device__ __forceinline__ int item_units(const ChunkArgs& a, const Seq& s, int m, int tokens,
+                                          int& first, int& tiles) {
+  tiles = tiles_seen(s.pos + m * tokens, min(tokens, s.n - m * tokens), s.cap, a.window, first);
+  return max(tiles, 1);  // an item that sees nothing still writes its zeros
+}
+// Units of one KV head of every lane's sequence.
+__device__ __forceinline__ long long head_units(const ChunkArgs& a, const Seq& s, int tokens,
+                                                int lane) {
+  const int items = (s.n + tokens - 1) / tokens;
+  long long u = 0;
+  int first, tiles;
+  if (items <= 4)
+    for (int m = 0; m < items; ++m) u += item_units(a, s, m, tokens, first, tiles);
+  uint32_t big = __ballot_sync(0xffffffffu, items > 4);
+  while (big) {  // long sequences: the warp shares the items
+    const int src = __ffs(big) - 1;
+    big &= big - 1;
+    Seq o;
+    o.t0 = 0;
+    o.n = __shfl_sync(0xffffffffu, s.n, src);
+    o.pos = __shfl_sync(0xffffffffu, s.pos, src);
+    o.cap = __shfl_sync(0xffffffffu, s.cap, src);
+    long long sum = 0;
+    for (int m = lane; m * tokens < o.n; m += 32) sum += item_units(a, o, m, tokens, first, tiles);
+    for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (lane == src) u = sum;
+  }
+  return u;
+}
+__device__ __forceinline__ long long scan_add(long long x, int lane) {  // inclusive
+  for (int k = 1; k < 32; k <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, k);
+    if (lane >= k) x += y;
+  }
+  return x;
+}
+
+template <int HD>
+__device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
+  const int tokens = Shape<HD>::kTiles * a.TB, cta = blockIdx.x;
+  int32_t* join = a.joins + cta * 8;
+  int queued = 0;
+  auto push = [&](const Item& it) {
+    const int at = queued % kQueue;
+    if (queued >= kQueue &&
+        !wait_warp(c.item_empty[at], (queued / kQueue - 1) & 1, &c.abort, a.err))
+      return false;
+    if (lane == 0) {
+      c.items[at] = it;
+      mbar_arrive(smem_u32(&c.item_full[at]));
+    }
+    __syncwarp();
+    ++queued;
+    return true;
+  };
+  Item end;
+  memset(&end, 0, sizeof(end));
+  end.flags = kItemEnd;
+
+  long long total = 0, mine = 0;
+  for (int base = 0; base < a.S; base += 32) {
+    mine = head_units(a, sequence(a, base + lane), tokens, lane) * a.NKV;
+    total += __shfl_sync(0xffffffffu, scan_add(mine, lane), 31);
+  }
+  const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_units);
+  const long long u0 = cta * per, u1 = min(u0 + per, total);
+  int cut = 0;  // whether this CTA holds the first part of a cut item
+  if (u0 < u1) {
+    // the sequence, KV head and item that hold unit u0
+    long long before = 0;
+    int seq = 0;
+    for (int base = 0; base < a.S; base += 32) {
+      if (a.S > 32) mine = head_units(a, sequence(a, base + lane), tokens, lane) * a.NKV;
+      const long long upto = before + scan_add(mine, lane);
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > u0);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        before = __shfl_sync(0xffffffffu, upto - mine, src);
+        seq = base + src;
+        break;
+      }
+      before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    Seq s = sequence(a, seq);
+    const long long per_head =
+        __shfl_sync(0xffffffffu, head_units(a, lane ? Seq{0, 0, 0, 0} : s, tokens, lane), 0);
+    long long rest = u0 - before;
+    int kvh = int(rest / per_head), m = 0;
+    rest -= kvh * per_head;
+    int first, tiles;
+    for (int base = 0;; base += 32) {
+      const bool real = (base + lane) * tokens < s.n;
+      const long long u = real ? item_units(a, s, base + lane, tokens, first, tiles) : 0;
+      const long long upto = scan_add(u, lane);
+      const uint32_t past = __ballot_sync(0xffffffffu, upto > rest);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        rest -= __shfl_sync(0xffffffffu, upto - u, src);
+        m = base + src;
+        break;
+      }
+      rest -= __shfl_sync(0xffffffffu, upto, 31);
+      if ((base + 32) * tokens >= s.n) break;  // not reached: rest lies within the head
+    }
+    int off = int(rest);
+    for (long long at = u0; at < u1;) {
+      const int units = item_units(a, s, m, tokens, first, tiles);
+      const int take = int(min((long long)(units - off), u1 - at));
+      const bool whole = off == 0 && take == units;
+      Item it;
+      it.flags = 0;
+      it.kv0 = first + off;
+      it.kvn = tiles ? take : 0;
+      it.tok0 = s.t0 + m * tokens;
+      it.ntok = min(tokens, s.n - m * tokens);
+      it.pos0 = s.pos + m * tokens;
+      it.kvh = kvh;
+      it.seq = seq;
+      it.cap = s.cap;
+      it.slot = whole ? -1 : (off == 0 ? 2 * cta + 1 : 2 * cta);
+      if (!whole && off == 0) {
+        cut = 1;
+        if (lane == 0) {
+          join[0] = int((at + units - 1) / per) - cta + 1;  // CTAs that hold a part
+          join[1] = it.tok0;
+          join[2] = it.ntok;
+          join[3] = kvh;
+        }
+      }
+      if (!push(it)) return;
+      at += take;
+      off = 0;
+      if (++m * tokens >= s.n) {
+        m = 0;
+        if (++kvh == a.NKV) {
+          kvh = 0;
+          if (at < u1) do s = sequence(a, ++seq); while (s.n == 0 && seq < a.S);
+        }
+      }
+    }
+  }
+  if (!cut && lane == 0) join[0] = 0;
+  if (cta == 0)  // lengths beyond the block table
+    for (int i = lane; i < a.S; i += 32)
+      if (a.seq_lens[i] > a.table_span && sequence(a, i).n) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
+  push(end);
+}
+
+// ---- loader ----
+template <int HD>
+__device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, uint32_t tiles,
+                          int lane) {
+  using Sh = Shape<HD>;
+  const uint32_t stages = tiles + Sh::kQBytes;
+  const int copies = kN / a.copy_rows;
+  int stage = 0, queued = 0, q_uses = 0;
+  uint32_t phase = 1, tile_no = 0;  // of the stage's empty barrier: free at first
+  uint32_t issued = 0;
+  bool ok = true;
+  // One ring stage: columns [64 col, 64 col + kCols) of a cache tile whose copy `lane` has
+  // block `id` (-1: zeros) and first row `off`.
+  auto fill = [&](const CUtensorMap* map, int col, int kvh, int id, int off) {
+    if (!wait_warp(c.kv_empty[stage], phase, &c.abort, a.err)) return false;
+    const uint32_t bar = smem_u32(&c.kv_full[stage]);
+    const uint32_t dst = stages + stage * Sh::kStageBytes;
+    if (lane == 0) mbar_expect(bar, Sh::kStageBytes);
+    __syncwarp();
+    if (lane < copies) {
+#pragma unroll
+      for (int k = 0; k < Sh::kCols / 64; ++k)
+        tma_load_4d(dst + k * kChunkBytes + lane * a.copy_rows * 128, map, col + 64 * k, off, kvh,
+                    id < 0 ? int(a.blocks) : id, bar);
+    }
+    ++issued;
+    if (++stage == Sh::kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    return true;
+  };
+  for (;;) {
+    const int at = queued % kQueue;
+    if (!(ok = wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err))) break;
+    const Item it = c.items[at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
+    ++queued;
+    if (it.flags & kItemEnd) break;
+    if (!it.kvn) continue;
+    // the queries
+    if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
+    ++q_uses;
+    if (lane == 0) {
+      const int filled = min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB);
+      const uint32_t bar = smem_u32(&c.q_full);
+      mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
+      for (int t = 0; t < filled; ++t)
+        for (int k = 0; k < HD / 64; ++k)
+          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, it.kvh * a.G,
+                      it.tok0 + t * a.TB, bar);
+    }
+    __syncwarp();
+    // the cache tiles: K of tile j + 1 goes in before V of tile j (256-dim heads need it first)
+    const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
+    const int hi = min(it.pos0 + it.ntok, it.cap);
+    const int32_t* table = a.tables + int64_t(it.seq) * a.table_stride;
+    auto look_up = [&](int j, int& id, int& off) {
+      const int pos = j * kN + lane * a.copy_rows;
+      const int block = pos / a.B;
+      off = pos - block * a.B;
+      id = -1;
+      bool bad = false;
+      if (lane < copies && pos < hi && pos + a.copy_rows > lo) {
+        id = table[block];
+        bad = id < 0 || id >= a.blocks;
+        if (bad) id = -1;
+      }
+      return __ballot_sync(0xffffffffu, bad);
+    };
+    int id = -1, off = 0, next_id = -1, next_off = 0;
+    uint32_t bad = look_up(it.kv0, id, off), next_bad = 0;
+    auto fill_k = [&](uint32_t mask, int i, int o) {
+      if (lane == 0) {
+        c.bad[tile_no % kBadRing] = mask;
+        if (mask) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
+      }
+      ++tile_no;
+      for (int h = 0; h < Sh::kHalves; ++h)
+        if (!fill(&maps.k, h * Sh::kCols, it.kvh, i, o)) return false;
+      return true;
+    };
+    if (!(ok = fill_k(bad, id, off))) break;
+    for (int j = 0; j < it.kvn; ++j) {
+      const bool more = j + 1 < it.kvn;
+      if (more) next_bad = look_up(it.kv0 + j + 1, next_id, next_off);
+      if (Sh::kTiles == 1 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
+      for (int h = 0; h < Sh::kHalves && ok; ++h)
+        ok = fill(&maps.v, h * Sh::kCols, it.kvh, id, off);
+      if (!ok) break;
+      if (Sh::kTiles == 2 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
+      id = next_id;
+      off = next_off;
+    }
+    if (!ok) break;
+  }
+  if (!ok) {  // given up: no copy may land after the CTA has gone
+    for (uint32_t i = issued > Sh::kStages ? issued - Sh::kStages : 0; i < issued; ++i) {
+      const long long start = clock64();
+      while (!mbar_try(smem_u32(&c.kv_full[i % Sh::kStages]), (i / Sh::kStages) & 1) &&
+             clock64() - start < 100000000LL) {
+      }
+    }
+    const long long start = clock64();
+    while (q_uses && !mbar_try(smem_u32(&c.q_full), (q_uses - 1) & 1) &&
+           clock64() - start < 100000000LL) {
+    }
+  }
+}
+
+// ---- products: one thread ----
+template <int HD>
+__device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
+  using Sh = Shape<HD>;
+  const uint32_t tmem = c.tmem, stages = tiles + Sh::kQBytes;
+  constexpr uint32_t kScores = instruction(true, false, kM, kN);
+  constexpr uint32_t kSum = instruction(true, true, kM, Sh::kCols);
+  int stage = 0, queued = 0;
+  uint32_t phase = 0, q_phase = 0, p_count[2] = {0, 0}, buffers = 0;
+#define WAIT(bar, parity) \
+  if (!wait_one(bar, parity, &c.abort, a.err)) return false
+  auto wait_stage = [&]() { return wait_one(c.kv_full[stage], phase, &c.abort, a.err); };
+  auto take = [&]() {
+    const int was = stage;
+    if (++stage == Sh::kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    return was;
+  };
+  auto scores = [&](int t, int buffer, int st, int half, bool add) {
+    const uint32_t q = tiles + (t * (HD / 64) + half * (Sh::kCols / 64)) * kChunkBytes;
+    const uint32_t k = stages + st * Sh::kStageBytes;
+#pragma unroll
+    for (int x = 0; x < Sh::kCols / 64; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        mma_ss(tmem + buffer * kN, desc_k_major(q + x * kChunkBytes + 32 * y),
+               desc_k_major(k + x * kChunkBytes + 32 * y), kScores, add || x + y > 0);
+  };
+  auto sum = [&](int o_col, int buffer, int st, bool add) {
+    const uint32_t v = stages + st * Sh::kStageBytes;
+#pragma unroll
+    for (int x = 0; x < kN / 16; ++x)
+      mma_ts(tmem + o_col, tmem + buffer * kN + 8 * x,
+             desc_mn_major(v + x * 16 * 128, kChunkBytes), kSum, add || x > 0);
+  };
+  auto commit = [&](const uint64_t& bar) { mma_commit(smem_u32(&bar)); };
+  for (;;) {
+    const int at = queued % kQueue;
+    WAIT(c.item_full[at], (queued / kQueue) & 1);
+    const Item it = c.items[at];
+    mbar_arrive(smem_u32(&c.item_empty[at]));
+    ++queued;
+    if (it.flags & kItemEnd) return true;
+    if (!it.kvn) continue;
+    const int j0 = it.kv0, j1 = it.kv0 + it.kvn;
+    WAIT(c.q_full, q_phase);
+    q_phase ^= 1;
+    if constexpr (Sh::kTiles == 2) {
+      int b[2], e[2];
+      tile_range<HD>(a, it, 0, b[0], e[0]);
+      tile_range<HD>(a, it, 1, b[1], e[1]);
+      if (!wait_stage()) return false;
+      tc_fence_after();
+      int k_st = take();
+      for (int t = 0; t < 2; ++t)
+        if (b[t] <= j0 && j0 < e[t]) {
+          scores(t, t, k_st, 0, false);
+          commit(c.s_full[t]);
+        }
+      commit(c.kv_empty[k_st]);
+      if (j0 + 1 == j1) commit(c.q_empty);
+      for (int j = j0; j < j1; ++j) {
+        if (!wait_stage()) return false;
+        const int v_st = take();
+        const bool more = j + 1 < j1;
+        k_st = -1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (b[t] <= j && j < e[t]) {
+            WAIT(c.p_full[t], p_count[t] & 1);
+            ++p_count[t];
+            tc_fence_after();
+            sum(Sh::kO + t * Sh::kOStride, t, v_st, j > b[t]);
+            if (j + 1 == e[t]) commit(c.o_full[t]);
+          }
+          if (more && b[t] <= j + 1 && j + 1 < e[t]) {
+            if (k_st < 0) {
+              if (!wait_stage()) return false;
+              tc_fence_after();
+              k_st = take();
+            }
+            scores(t, t, k_st, 0, false);
+            commit(c.s_full[t]);
+          }
+        }
+        commit(c.kv_empty[v_st]);
+        if (more) {
+          if (k_st < 0) {  // a tile of positions between the two tiles' windows
+            if (!wait_stage()) return false;
+            k_st = take();
+          }
+          commit(c.kv_empty[k_st]);
+          if (j + 2 == j1) commit(c.q_empty);
+        }
+      }
+    } else {
+      auto next_scores = [&]() {
+        for (int h = 0; h < Sh::kHalves; ++h) {
+          if (!wait_stage()) return false;
+          tc_fence_after();
+          const int st = take();
+          scores(0, buffers & 1, st, h, h > 0);
+          commit(c.kv_empty[st]);
+        }
+        commit(c.s_full[buffers & 1]);
+        ++buffers;
+        return true;
+      };
+      if (!next_scores()) return false;
+      for (int j = j0; j < j1; ++j) {
+        if (j + 1 < j1 && !next_scores()) return false;
+        if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1)) commit(c.q_empty);
+        WAIT(c.p_full[0], p_count[0] & 1);
+        const int buffer = p_count[0] & 1;
+        ++p_count[0];
+        for (int h = 0; h < Sh::kHalves; ++h) {
+          if (!wait_stage()) return false;
+          tc_fence_after();
+          const int st = take();
+          sum(Sh::kO + h * Sh::kCols, buffer, st, j > j0);
+          commit(c.kv_empty[st]);
+        }
+        commit(c.o_full[0]);
+      }
+    }
+  }
+#undef WAIT
+}
+
+// ---- softmax ----
+// One row from its own positions [lo, hi) alone, by the warp: the row's partial result, or
+// its output.  Slow; for rows whose sum came out non-finite.
+struct RowOut {
+  __nv_bfloat16* out;  // whole rows
+  int64_t gate_at;     // -1: no gate
+  float* part_o;       // partial rows
+  float2* part_ml;     // may be null: another warp writes it
+};
+template <int HD, bool KV8>
+__device__ __forceinline__ void redo_row(const ChunkArgs& a, int seq, int token, int head, int lo,
+                                      int hi, int col0, int cols, RowOut o) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* q = a.q + token * a.q_t + head * a.q_h;
+  const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
+  const int64_t kv = int64_t(head / a.G) * a.sh;
+  const float qk = a.scale_log2 * (KV8 ? a.k_scale : 1.0f);
+  float m = -INFINITY, l = 0.0f, acc[HD / 32];
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
+  for (int c0 = lo; c0 < hi; c0 += 32) {
+    const int c = c0 + lane;
+    float s = -INFINITY;
+    int64_t at = -1;
+    if (c < hi) {
+      const int64_t id = block_of(a, table, c);
+      if (id >= 0) {
+        at = id * a.sb + int64_t(c % a.B) * a.so + kv;
+        float dot = 0.0f;
+        for (int i = 0; i < HD; ++i) dot += __bfloat162float(q[i]) * cache_value<KV8>(a.kc, at + i);
+        s = dot * qk;
+      }
+    }
+    float top = s;
+    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
+    const float w = exp2f(s - base), shrink = exp2f(m - base);
+    m = m_new;
+    l = l * shrink + w;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) acc[i] *= shrink;
+    for (int k = 0; k < 32; ++k) {
+      const int64_t row = __shfl_sync(0xffffffffu, at, k);
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      if (row < 0) continue;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const int d = lane + 32 * i;
+        if (d < cols) acc[i] += wk * cache_value<KV8>(a.vc, row + col0 + d);
+      }
+    }
+  }
+  for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+  const float inv = (KV8 ? a.v_scale : 1.0f) / l;
+  for (int i = 0; i < HD / 32; ++i) {
+    const int d = lane + 32 * i;
+    if (d >= cols) break;
+    if (o.out) {
+      float y = acc[i] * inv;
+      if (o.gate_at >= 0) y *= load_gate(a, o.gate_at + d);
+      o.out[d] = __float2bfloat16_rn(y);
+    } else {
+      o.part_o[d] = acc[i];
+    }
+  }
+  if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
+}
+
+// Eight consecutive gate values.
+__device__ __forceinline__ void load_gate8(const ChunkArgs& a, int64_t at, float (&g)[8]) {
+  if (a.gate_dtype == DORY_DTYPE_F32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.gate) + at);
+    const float4 x = p[0], y = p[1];
+    g[0] = x.x; g[1] = x.y; g[2] = x.z; g[3] = x.w;
+    g[4] = y.x; g[5] = y.y; g[6] = y.z; g[7] = y.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.gate) + at);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (a.gate_dtype == DORY_DTYPE_BF16) {
+        g[2 * i] = __uint_as_float(u[i] << 16);
+        g[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        g[2 * i] = f.x;
+        g[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+
+// A bit for each of 32 columns that lies above `last` or below `first`.
+__device__ __forceinline__ uint32_t outside(int last, int first) {
+  const uint32_t above = last < 0 ? 0xffffffffu : last >= 31 ? 0u : 0xfffffffeu << last;
+  const uint32_t below = first <= 0 ? 0u : first >= 32 ? 0xffffffffu : (1u << first) - 1u;
+  return above | below;
+}
+// A bit for each of the 32 columns from `col` that belongs to a copy with a bad block id.
+__device__ __forceinline__ uint32_t bad_columns(uint32_t bad, int col, int copy_shift) {
+  return (bad >> (col >> copy_shift) & 1 ? 0x0000ffffu : 0u) |
+         (bad >> ((col + 16) >> copy_shift) & 1 ? 0xffff0000u : 0u);
+}
+
+template <int HD>
+__device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles, int warp, int lane) {
+  using Sh = Shape<HD>;
+  constexpr bool kTwo = Sh::kTiles == 2;
+  const int wg = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+  const int t = kTwo ? wg : 0, share = kTwo ? 0 : wg;  // tile, and which half of its columns
+  const uint32_t tmem = c.tmem + (uint32_t(quad * 32) << 16);
+  const uint32_t o_addr = tmem + Sh::kO + t * Sh::kOStride + share * Sh::kOutCols;
+  const uint32_t stages = tiles + Sh::kQBytes;
+  const int row_tok = row / a.G, row_head = row - row_tok * a.G;
+  const bool row_real = row < a.TB * a.G;
+  const float sl = a.scale_log2, slack = kSlack / a.scale_log2;
+  int queued = 0;
+  uint32_t scored = 0, summed = 0, tiles_seen_before = 0, stage_no = 0;
+  for (;;) {
+    const int at = queued % kQueue;
+    if (!wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err)) return;
+    const Item it = c.items[at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
+    ++queued;
+    if (it.flags & kItemEnd) return;
+    int b, e;
+    tile_range<HD>(a, it, t, b, e);
+    const int tok = t * a.TB + row_tok, pos = it.pos0 + tok;
+    const bool live = row_real && tok < it.ntok;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    const int see_hi = min(pos, it.cap - 1), see_lo = a.window ? max(0, pos - a.window + 1) : 0;
+    const int item_lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
+    const int item_hi = min(it.pos0 + it.ntok, it.cap);
+    float m = -INFINITY, l = 0.0f;
+    for (int j = b; j < e; ++j) {
+      const int buffer = kTwo ? t : int(scored & 1);
+      const uint32_t s_addr = tmem + buffer * kN;
+      if (!wait_warp(c.s_full[buffer], kTwo ? scored & 1 : (scored >> 1) & 1, &c.abort, a.err))
+        return;
+      tc_fence_after();
+      const uint32_t bad = c.bad[(tiles_seen_before + (j - it.kv0)) % kBadRing];
+      if (warp_live) {
+        float s[Sh::kScoreCols];
+#pragma unroll
+        for (int x = 0; x < Sh::kScoreCols; x += 32)
+          tmem_ld32(s_addr + share * Sh::kScoreCols + x, reinterpret_cast<uint32_t*>(s + x));
+        tmem_wait_ld();
+        const int base = j * kN + share * Sh::kScoreCols;
+        const int last = see_hi - base, first = see_lo - base;
+        const bool edge = live && (last < Sh::kScoreCols - 1 || first > 0);
+        if (bad || __any_sync(0xffffffffu, edge)) {
+#pragma unroll
+          for (int w = 0; w < Sh::kScoreCols / 32; ++w) {
+            uint32_t hide = outside(last - 32 * w, first - 32 * w);
+            if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + 32 * w, a.copy_shift);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (hide >> x & 1) s[32 * w + x] = -INFINITY;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top[x] = fmaxf(s[x], s[x + 4]);
+#pragma unroll
+        for (int x = 8; x < Sh::kScoreCols; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
+        float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (!kTwo) {  // the other half of the row's columns
+          float* mine = c.swap[scored & 1][share];
+          mine[row] = mt;
+          named_barrier(1 + quad, 64);
+          mt = fmaxf(mt, c.swap[scored & 1][share ^ 1][row]);
+        }
+        if (j == b) {
+          m = mt;
+        } else if (__any_sync(0xffffffffu, mt > m + slack)) {
+          const float grown = fmaxf(m, mt);
+          const float f = m == -INFINITY ? 0.0f : exp2_approx((m - grown) * sl);
+          l *= f;
+          m = grown;
+          if (!kTwo) {  // the sum over the tile before may still be running
+            if (!wait_warp(c.o_full[0], (summed - 1) & 1, &c.abort, a.err)) return;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int x = 0; x < Sh::kOutCols; x += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + x, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tmem_st32(o_addr + x, o);
+          }
+          tmem_wait_st();
+        }
+        const float ref = m == -INFINITY ? 0.0f : m * sl;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int x = 0; x < Sh::kScoreCols; x += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            const float p0 = exp2_approx(fmaf(s[x + y], sl, -ref));
+            const float p1 = exp2_approx(fmaf(s[x + y + 1], sl, -ref));
+            sum[y & 2] += p0;
+            sum[(y & 2) + 1] += p1;
+            p[y / 2] = pack_bf16(p0, p1);
+          }
+          tmem_st16(s_addr + (share * Sh::kScoreCols + x) / 2, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+      }
+      // V rows of this tile that no row of the item sees, in copies that hold others it does
+      const int z_lo = item_lo - j * kN, z_hi = item_hi - j * kN;
+      if (z_lo > 0 || z_hi < kN) {
+        const int i = j - it.kv0;  // the tile's place in the piece, and so its V stages
+        const uint32_t v_no =
+            stage_no + (kTwo ? 2 * i + 1 : 2 * Sh::kHalves * i + (i + 1 < it.kvn ? 2 : 1) * Sh::kHalves);
+        const int r1 = z_lo > 0 ? (z_lo & ~(a.copy_rows - 1)) : 0, r2 = max(z_lo, 0);
+        const int r3 = min(z_hi, kN), r4 = (r3 + a.copy_rows - 1) & ~(a.copy_rows - 1);
+        for (int h = 0; h < Sh::kHalves; ++h) {
+          const uint32_t no = v_no + h;
+          const int st = no % Sh::kStages;
+          if (!wait_warp(c.kv_full[st], (no / Sh::kStages) & 1, &c.abort, a.err)) return;
+          constexpr int kPieces = Sh::kCols / 8;  // 16-byte pieces of a row
+          const int rows = (r2 - r1) + (r4 - r3);
+          for (int x = (kTwo ? quad : warp) * 32 + lane; x < rows * kPieces; x += (kTwo ? 4 : 8) * 32) {
+            int r = x / kPieces;
+            const int piece = x % kPieces;
+            r = r < r2 - r1 ? r1 + r : r3 + (r - (r2 - r1));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             stages + st * Sh::kStageBytes + (piece / 8) * kChunkBytes + r * 128 +
+                             (piece % 8) * 16),
+                         "r"(0)
+                         : "memory");
+          }
+        }
+        fence_async_smem();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c.p_full[t]));
+      ++scored;
+      if (!kTwo) ++summed;
+    }
+    tiles_seen_before += it.kvn;
+    stage_no += 2 * Sh::kHalves * it.kvn;
+
+    // the item's rows
+    if (e > b) {
+      if (kTwo) ++summed;
+      // 256-dim heads: one phase a tile, and the last scores only vouch for the sum of the tile
+      // two before; a parity can only be asked for with at most one phase outstanding
+      if (!kTwo && e - b > 1 && !wait_warp(c.o_full[0], summed & 1, &c.abort, a.err)) return;
+      if (!wait_warp(c.o_full[t], (summed - 1) & 1, &c.abort, a.err)) return;
+      tc_fence_after();
+    }
+    if (!warp_live) continue;
+    if (!kTwo) {
+      // the sums of the two halves; the buffer of the tile before the last is free
+      float* mine = c.swap[scored & 1][share];
+      mine[row] = l;
+      named_barrier(1 + quad, 64);
+      l += c.swap[scored & 1][share ^ 1][row];
+      named_barrier(1 + quad, 64);
+    }
+    const int token = it.tok0 + tok, head = it.kvh * a.G + row_head;
+    const int col0 = share * Sh::kOutCols;
+    const int64_t column = int64_t(head) * HD + col0;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + t * kM + row;
+    RowOut ro;
+    ro.out = it.slot < 0 ? a.out + token * a.out_t + column : nullptr;
+    ro.gate_at = a.gate ? token * a.gate_t + column : -1;
+    ro.part_o = a.part_o + slot_row * HD + col0;
+    ro.part_ml = share == 0 ? a.part_ml + slot_row : nullptr;
+    float odd = 0.0f;  // NaN once a value is not finite
+#pragma unroll 1
+    for (int x = 0; x < Sh::kOutCols; x += 32) {
+      float o[32];
+      if (e > b) {
+        tmem_ld32(o_addr + x, reinterpret_cast<uint32_t*>(o));
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+      }
+      if (live) {
+#pragma unroll
+      for (int y = 0; y < 32; ++y) odd = fmaf(o[y], 0.0f, odd);
+      if (it.slot >= 0) {
+#pragma unroll
+        for (int y = 0; y < 32; y += 4)
+          *reinterpret_cast<float4*>(ro.part_o + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 32; y += 8) {
+          float g[8];
+          if (a.gate) {
+            load_gate8(a, ro.gate_at + x + y, g);
+#pragma unroll
+            for (int z = 0; z < 8; ++z) g[z] *= inv;
+          } else {
+#pragma unroll
+            for (int z = 0; z < 8; ++z) g[z] = inv;
+          }
+          uint4 w;
+          w.x = pack_bf16(o[y] * g[0], o[y + 1] * g[1]);
+          w.y = pack_bf16(o[y + 2] * g[2], o[y + 3] * g[3]);
+          w.z = pack_bf16(o[y + 4] * g[4], o[y + 5] * g[5]);
+          w.w = pack_bf16(o[y + 6] * g[6], o[y + 7] * g[7]);
+          *reinterpret_cast<uint4*>(ro.out + x + y) = w;
+        }
+      }
+      }
+      __syncwarp();
+    }
+    if (live && it.slot >= 0 && share == 0)
+      *ro.part_ml = make_float2(m == -INFINITY ? 0.0f : m * sl, l);
+    uint32_t again = __ballot_sync(0xffffffffu, live && isnan(odd) && isfinite(l));
+    while (again) {
+      const int src = __ffs(again) - 1;
+      again &= again - 1;
+      const int r_tok = __shfl_sync(0xffffffffu, token, src);
+      const int r_head = __shfl_sync(0xffffffffu, head, src);
+      const int lo = max(__shfl_sync(0xffffffffu, see_lo, src), it.kv0 * kN);
+      const int hi = min(__shfl_sync(0xffffffffu, see_hi, src) + 1, (it.kv0 + it.kvn) * kN);
+      RowOut r;
+      r.out = reinterpret_cast<__nv_bfloat16*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.out), src));
+      r.gate_at = __shfl_sync(0xffffffffu, ro.gate_at, src);
+      r.part_o = reinterpret_cast<float*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.part_o), src));
+      r.part_ml = reinterpret_cast<float2*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.part_ml), src));
+      if (it.slot < 0) r.part_ml = nullptr;
+      redo_row<HD, false>(a, it.seq, r_tok, r_head, lo, hi, col0, Sh::kOutCols, r);
+      __syncwarp();
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_kernel(const ChunkArgs a, const __grid_constant__ Maps maps) {
+  using Sh = Shape<HD>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Control<HD>& c = *reinterpret_cast<Control<HD>*>(smem + Sh::kQBytes + Sh::kStages * Sh::kStageBytes);
+  const uint32_t tiles = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_launch();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Sh::kStages; ++i) {
+      mbar_init(smem_u32(&c.kv_full[i]), 1);
+      mbar_init(smem_u32(&c.kv_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&c.q_full), 1);
+    mbar_init(smem_u32(&c.q_empty), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&c.s_full[i]), 1);
+      mbar_init(smem_u32(&c.p_full[i]), Sh::kTiles == 2 ? 4 : 8);
+      mbar_init(smem_u32(&c.o_full[i]), 1);
+    }
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(smem_u32(&c.item_full[i]), 1);
+      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxWarps + 2);
+    }
+    mbar_init(smem_u32(&c.drained), 1);
+    c.abort = 0;
+    fence_mbar_init();
+    fence_async_smem();
+  }
+  if (warp == kMmaWarp) tmem_alloc(smem_u32(&c.tmem), 512);
+  if (warp == kLoadWarp && lane == 0) {
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp < kSoftmaxWarps) {
+    regs_up<kSoftmaxRegs>();
+    softmax_role<HD>(a, c, tiles, warp, lane);
+  } else {
+    regs_down<kOtherRegs>();
+    if (warp == kLoadWarp) {
+      load_role<HD>(a, maps, c, tiles, lane);
+    } else if (warp == kMmaWarp) {
+      if (lane == 0) {
+        mma_items<HD>(a, c, tiles);
+        mma_commit(smem_u32(&c.drained));  // no product or arrival is under way after this
+        const long long start = clock64();
+        while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
+        }
+      }
+    } else if (warp == kPlanWarp) {
+      plan_role<HD>(a, c, lane);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_free(c.tmem, 512);
+}
+
+// Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
+// starts at the end of CTA c's piece, a warp a row.
+constexpr int kJoinSlices = 8;
+template <int HD>
+__global__ void __launch_bounds__(256) join_kernel(const ChunkArgs a) {
+  using Sh = Shape<HD>;
+  constexpr int kPer = HD / 32;  // columns of a lane
+  grid_wait();
+  const int32_t* join = a.joins + blockIdx.x * 8;
+  const int parts = join[0], tok0 = join[1], ntok = join[2], kvh = join[3];
+  if (!parts) return;
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 8 * kJoinSlices) {
+    const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
+    const int tok = t * a.TB + row_tok;
+    if (in_tile >= a.TB * a.G || tok >= ntok) continue;
+    auto slot = [&](int i) {
+      return int64_t(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * Sh::kItemRows + r;
+    };
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 ml = a.part_ml[slot(i)];
+      if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+    }
+    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    float l = 0.0f, acc[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) acc[x] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float2 ml = a.part_ml[slot(i)];
+      if (ml.y == 0.0f) continue;  // saw nothing
+      const float w = exp2_approx(ml.x - m);
+      const float* o = a.part_o + slot(i) * HD + lane * kPer;
+      l += w * ml.y;
+      if constexpr (kPer == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(o);
+        acc[0] += w * v.x;
+        acc[1] += w * v.y;
+      } else {
+#pragma unroll
+        for (int x = 0; x < kPer; x += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(o + x);
+          acc[x] += w * v.x;
+          acc[x + 1] += w * v.y;
+          acc[x + 2] += w * v.z;
+          acc[x + 3] += w * v.w;
+        }
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int token = tok0 + tok;
+    const int64_t column = int64_t(kvh * a.G + in_tile - row_tok * a.G) * HD + lane * kPer;
+#pragma unroll
+    for (int x = 0; x < kPer; x += 2) {
+      float y0 = acc[x] * inv, y1 = acc[x + 1] * inv;
+      if (a.gate) {
+        y0 *= load_gate(a, token * a.gate_t + column + x);
+        y1 *= load_gate(a, token * a.gate_t + column + x + 1);
+      }
+      *reinterpret_cast<uint32_t*>(a.out + token * a.out_t + column + x) = pack_bf16(y0, y1);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------
+struct ScratchLayout {
+  int64_t joins, ml, o, total;
+};
+ScratchLayout scratch_layout(int ctas, int head_dim) {
+  const int64_t rows = head_dim == 256 ? kM : 2 * kM;
+  ScratchLayout s;
+  s.joins = 256;  // [0, 256): header; word 0 = device error flags
+  s.ml = s.joins + (int64_t(ctas) * 32 + 255) / 256 * 256;
+  s.o = s.ml + 2 * ctas * rows * 8;
+  s.total = s.o + 2 * ctas * rows * head_dim * 4;
+  return s;
+}
+
+int device_sms(int* device) {  // 0 on failure
+  static int counts[64] = {0};
+  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= 64) return 0;
+  if (!counts[*device]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) == cudaSuccess)
+      counts[*device] = n;
+  }
+  return counts[*device];
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// A map of 16-bit elements with the 128-byte swizzle.  A dimension of one element needs no
+// stride of its own: any valid one does.
+bool encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
+            const int64_t* strides, const int* box) {
+  cuuint64_t d[5], st[5];
+  cuuint32_t b[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = cuuint64_t(dims[i]);
+    b[i] = cuuint32_t(box[i]);
+    es[i] = 1;
+    if (i > 0) st[i - 1] = dims[i] == 1 ? 128 : cuuint64_t(strides[i]) * 2;
+  }
+  auto fn = encoder();
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base),
+                  d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD>
+int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaStream_t stream) {
+  using Sh = Shape<HD>;
+  constexpr int kBytes = Sh::kQBytes + Sh::kStages * Sh::kStageBytes + int(sizeof(Control<HD>));
+  static_assert(kBytes <= 232448, "more shared memory than a CTA may have");
+  static bool ready[64] = {false};
+  if (!ready[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        chunk_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess)
+      return fail(DORY_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    ready[device] = true;
+  }
+  chunk_kernel<HD><<<ctas, kThreads, kBytes, stream>>>(a, maps);
+  int32_t status = dory::launched(cudaSuccess);
+  if (status != DORY_OK) return status;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(ctas, kJoinSlices);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return dory::launched(cudaLaunchKernelEx(&cfg, join_kernel<HD>, a));
+}
+
 }  // namespace
 
 extern "C" {
@@ -150,7 +1273,9 @@ int64_t dory_chunk_scratch_bytes(int32_t num_heads, int32_t num_kv_heads, int32_
   if (num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads ||
       num_heads / num_kv_heads > 64 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return 256;
+  int device;
+  const int sms = device_sms(&device);
+  return scratch_layout(sms > 0 ? sms : 148, head_dim).total;
 }
 
 int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
@@ -228,17 +1353,45 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   a.NKV = p.num_kv_heads;
   a.G = G;
   a.B = p.block_size;
-  a.window = p.window;
+  a.window = p.window < kMaxPosition ? p.window : kMaxPosition;
   a.gate_dtype = p.gate_dtype;
-  const dim3 grid(p.num_tokens, (p.num_heads + 3) / 4);
+  a.TB = kM / G;
+  a.copy_rows = p.block_size & -p.block_size;
+  if (a.copy_rows > kN) a.copy_rows = kN;
+  while ((1 << a.copy_shift) < a.copy_rows) ++a.copy_shift;
+  const int64_t span = int64_t(p.max_blocks) * p.block_size;
+  a.table_span = span < kMaxPosition ? int(span) : kMaxPosition;
+  a.min_units = 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (kv8) {
+    const dim3 grid(p.num_tokens, (p.num_heads + 3) / 4);
     if (p.head_dim == 128) chunk_rows<128, true><<<grid, 128, 0, s>>>(a);
     else chunk_rows<256, true><<<grid, 128, 0, s>>>(a);
-  } else if (p.head_dim == 64) chunk_rows<64, false><<<grid, 128, 0, s>>>(a);
-  else if (p.head_dim == 128) chunk_rows<128, false><<<grid, 128, 0, s>>>(a);
-  else chunk_rows<256, false><<<grid, 128, 0, s>>>(a);
-  return dory::launched(cudaSuccess);
+    return dory::launched(cudaSuccess);
+  }
+  int device;
+  const int ctas = device_sms(&device);
+  if (ctas <= 0) return fail(DORY_ERR_CUDA, "no current CUDA device");
+  uint8_t* scratch = static_cast<uint8_t*>(p.scratch);
+  const ScratchLayout layout = scratch_layout(ctas, p.head_dim);
+  a.joins = reinterpret_cast<int32_t*>(scratch + layout.joins);
+  a.part_ml = reinterpret_cast<float2*>(scratch + layout.ml);
+  a.part_o = reinterpret_cast<float*>(scratch + layout.o);
+  Maps maps;
+  const int64_t q_dims[3] = {p.head_dim, p.num_heads, p.num_tokens};
+  const int64_t q_strides[3] = {1, p.q_stride_head, p.q_stride_token};
+  const int q_box[3] = {64, G, a.TB};
+  const int64_t c_dims[4] = {p.head_dim, p.block_size, p.num_kv_heads, p.num_cache_blocks};
+  const int64_t c_strides[4] = {1, p.stride_offset, p.stride_head, p.stride_block};
+  const int c_box[4] = {64, a.copy_rows, 1, 1};
+  if (!encode(&maps.q, p.q, 3, q_dims, q_strides, q_box) ||
+      !encode(&maps.k, p.key_cache, 4, c_dims, c_strides, c_box) ||
+      !encode(&maps.v, p.value_cache, 4, c_dims, c_strides, c_box))
+    return fail(DORY_ERR_UNSUPPORTED, "no tensor map for the query or cache view (strides must be "
+                                      "positive)");
+  if (p.head_dim == 64) return launch<64>(a, maps, device, ctas, s);
+  if (p.head_dim == 128) return launch<128>(a, maps, device, ctas, s);
+  return launch<256>(a, maps, device, ctas, s);
 }
 
 }  // extern "C"
