@@ -61,8 +61,8 @@ constexpr int kQueue = 4;            // items handed out ahead
 constexpr int kBadRing = 16;         // tiles whose bad-page masks are kept
 constexpr int kMaxPosition = 1 << 30;
 constexpr float kSlack = 8.0f;       // log2 a row's maximum may grow before O is rescaled
-// ~4 s, then give up: above a whole item of redo_row, which the other roles wait for.
-constexpr long long kWaitLimitCycles = 8000000000LL;
+// ~2 s, then give up: above a whole item of redo_row, which the other roles wait for.
+constexpr long long kWaitLimitCycles = 4000000000LL;
 
 struct ChunkArgs {
   const __nv_bfloat16* q;
@@ -684,8 +684,8 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
       for (int j = j0; j < j1; ++j) {
         if (j + 1 < j1 && !next_scores()) return false;
         if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1)) commit(c.q_empty);
-        WAIT(c.p_full[0], p_count[0] & 1);
         const int buffer = p_count[0] & 1;
+        WAIT(c.p_full[buffer], (p_count[0] >> 1) & 1);
         ++p_count[0];
         for (int h = 0; h < Sh::kHalves; ++h) {
           if (!wait_stage()) return false;
@@ -694,7 +694,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
           sum(Sh::kO + h * Sh::kCols, buffer, st, j > j0);
           commit(c.kv_empty[st]);
         }
-        commit(c.o_full[0]);
+        commit(c.o_full[buffer]);
       }
     }
   }
@@ -819,6 +819,14 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
   const float sl = a.scale_log2, slack = kSlack / a.scale_log2;
   int queued = 0;
   uint32_t scored = 0, summed = 0, tiles_seen_before = 0, stage_no = 0;
+  // The last sum given to the tensor cores is complete.  A parity can only be asked for with one
+  // phase of its barrier outstanding.  Two tiles: a phase an item.  256-dim heads: a phase a
+  // tile, on two barriers in turn, because scores j only vouch for the sum of tile j - 2.
+  auto wait_sum = [&]() {
+    const uint32_t last = summed - 1;
+    return kTwo ? wait_warp(c.o_full[t], last & 1, &c.abort, a.err)
+                : wait_warp(c.o_full[last & 1], (last >> 1) & 1, &c.abort, a.err);
+  };
   for (;;) {
     const int at = queued % kQueue;
     if (!wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err)) return;
@@ -882,7 +890,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           l *= f;
           m = grown;
           if (!kTwo) {  // the sum over the tile before may still be running
-            if (!wait_warp(c.o_full[0], (summed - 1) & 1, &c.abort, a.err)) return;
+            if (!wait_sum()) return;
             tc_fence_after();
           }
 #pragma unroll 1
@@ -943,7 +951,8 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c.p_full[t]));
+      // 256-dim heads: a warp may already be a tile ahead of another, so a barrier a buffer
+      if (lane == 0) mbar_arrive(smem_u32(&c.p_full[buffer]));
       ++scored;
       if (!kTwo) ++summed;
     }
@@ -953,10 +962,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     // the item's rows
     if (e > b) {
       if (kTwo) ++summed;
-      // 256-dim heads: one phase a tile, and the last scores only vouch for the sum of the tile
-      // two before; a parity can only be asked for with at most one phase outstanding
-      if (!kTwo && e - b > 1 && !wait_warp(c.o_full[0], summed & 1, &c.abort, a.err)) return;
-      if (!wait_warp(c.o_full[t], (summed - 1) & 1, &c.abort, a.err)) return;
+      if (!wait_sum()) return;
       tc_fence_after();
     }
     if (!warp_live) continue;

@@ -233,6 +233,17 @@ def test_flat_and_steep_scores(D, spread):
     b.check(b.run())
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_long_prompt_many_times(D):
+    """Many tiles an item and many items an SM, so every role gets ahead of the others."""
+    b = Batch([(4096, 4096)], D=D, seed=15)
+    attn = b.attention()
+    first = b.run(attn=attn).clone()
+    b.check(first)
+    for _ in range(20):
+        assert torch.equal(b.run(attn=attn), first)
+
+
 def test_long_cache_offsets_pass_32_bits():
     """Block strides that take element and byte offsets past 2^32."""
     NKV, D, B, blocks = 8, 128, 16, 140_000  # 32,768 elements a block: 4.6e9 elements
