@@ -209,6 +209,8 @@ struct Shape {
   static constexpr int kScoreCols = kTiles == 2 ? kN : kN / 2;  // of a row, per softmax thread
   static constexpr int kOutCols = kTiles == 2 ? HD : HD / 2;
   static constexpr int kItemRows = kTiles * kM;
+  // of kPolyOf pairs of exponentials, kPoly go to the FP32 pipe
+  static constexpr int kPoly = 1, kPolyOf = 4;
   // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
   static constexpr int kO = 2 * kN;
   static constexpr int kOStride = HD <= 128 ? 128 : 0;       // between the tiles' O
@@ -236,7 +238,7 @@ struct Item {
 template <int HD>
 struct Control {  // shared memory behind the tiles
   alignas(8) uint64_t kv_full[Shape<HD>::kStages], kv_empty[Shape<HD>::kStages];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], item_full[kQueue],
+  uint64_t q_full, q_empty, s_full[2], p_full[2][2], o_full[2], item_full[kQueue],
       item_empty[kQueue], drained;
   Item items[kQueue];
   uint32_t bad[kBadRing];
@@ -257,12 +259,6 @@ __device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatil
     }
   }
   return true;
-}
-// One thread's wait; false once any role of the CTA has given up.
-__device__ __forceinline__ bool wait_one(const uint64_t& bar, uint32_t parity, int* abort,
-                                         uint32_t* err) {
-  const uint32_t b = smem_u32(&bar);
-  return mbar_try(b, parity) || wait_slow(b, parity, abort, err);
 }
 // A whole warp's wait, the same answer in every lane.
 __device__ __forceinline__ bool wait_warp(const uint64_t& bar, uint32_t parity, int* abort,
@@ -471,18 +467,22 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
   uint32_t issued = 0;
   bool ok = true;
   // One ring stage: columns [64 col, 64 col + kCols) of a cache tile whose copy `lane` has
-  // block `id` (-1: zeros) and first row `off`.
+  // block `id` (a.blocks, beyond the cache: zeros) and first row `off`.
   auto fill = [&](const CUtensorMap* map, int col, int kvh, int id, int off) {
     if (!wait_warp(c.kv_empty[stage], phase, &c.abort, a.err)) return false;
     const uint32_t bar = smem_u32(&c.kv_full[stage]);
     const uint32_t dst = stages + stage * Sh::kStageBytes;
-    if (lane == 0) mbar_expect(bar, Sh::kStageBytes);
+    if (elect_one()) mbar_expect(bar, Sh::kStageBytes);
     __syncwarp();
-    if (lane < copies) {
+    for (int i = 0; i < copies; ++i) {
+      const int block = uniform(lane == i ? id : INT_MIN), row = uniform(lane == i ? off : INT_MIN);
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < Sh::kCols / 64; ++k)
-        tma_load_4d(dst + k * kChunkBytes + lane * a.copy_rows * 128, map, col + 64 * k, off, kvh,
-                    id < 0 ? int(a.blocks) : id, bar);
+        for (int k = 0; k < Sh::kCols / 64; ++k)
+          tma_load_4d(dst + k * kChunkBytes + i * a.copy_rows * 128, map, col + 64 * k, row, kvh,
+                      block, bar);
+      }
+      __syncwarp();
     }
     ++issued;
     if (++stage == Sh::kStages) {
@@ -496,21 +496,24 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     if (!(ok = wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err))) break;
     const Item it = c.items[at];
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
+    if (elect_one()) mbar_arrive(smem_u32(&c.item_empty[at]));
     ++queued;
-    if (it.flags & kItemEnd) break;
-    if (!it.kvn) continue;
+    if (uniform(it.flags) & kItemEnd) break;
+    const int kvn = uniform(it.kvn), kvh = uniform(it.kvh);
+    if (!kvn) continue;
     // the queries
     if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
     ++q_uses;
-    if (lane == 0) {
-      const int filled = min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB);
+    const int tok0 = uniform(it.tok0);
+    const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
+    if (elect_one()) {
       const uint32_t bar = smem_u32(&c.q_full);
       mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
       for (int t = 0; t < filled; ++t)
+#pragma unroll
         for (int k = 0; k < HD / 64; ++k)
-          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, it.kvh * a.G,
-                      it.tok0 + t * a.TB, bar);
+          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
+                      tok0 + t * a.TB, bar);
     }
     __syncwarp();
     // the cache tiles: K of tile j + 1 goes in before V of tile j (256-dim heads need it first)
@@ -521,16 +524,16 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
       const int pos = j * kN + lane * a.copy_rows;
       const int block = pos / a.B;
       off = pos - block * a.B;
-      id = -1;
+      id = int(a.blocks);
       bool bad = false;
       if (lane < copies && pos < hi && pos + a.copy_rows > lo) {
-        id = table[block];
-        bad = id < 0 || id >= a.blocks;
-        if (bad) id = -1;
+        const int entry = table[block];
+        bad = entry < 0 || entry >= a.blocks;
+        if (!bad) id = entry;
       }
       return __ballot_sync(0xffffffffu, bad);
     };
-    int id = -1, off = 0, next_id = -1, next_off = 0;
+    int id = 0, off = 0, next_id = 0, next_off = 0;
     uint32_t bad = look_up(it.kv0, id, off), next_bad = 0;
     auto fill_k = [&](uint32_t mask, int i, int o) {
       if (lane == 0) {
@@ -539,16 +542,16 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
       }
       ++tile_no;
       for (int h = 0; h < Sh::kHalves; ++h)
-        if (!fill(&maps.k, h * Sh::kCols, it.kvh, i, o)) return false;
+        if (!fill(&maps.k, h * Sh::kCols, kvh, i, o)) return false;
       return true;
     };
     if (!(ok = fill_k(bad, id, off))) break;
-    for (int j = 0; j < it.kvn; ++j) {
-      const bool more = j + 1 < it.kvn;
+    for (int j = 0; j < kvn; ++j) {
+      const bool more = j + 1 < kvn;
       if (more) next_bad = look_up(it.kv0 + j + 1, next_id, next_off);
       if (Sh::kTiles == 1 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
       for (int h = 0; h < Sh::kHalves && ok; ++h)
-        ok = fill(&maps.v, h * Sh::kCols, it.kvh, id, off);
+        ok = fill(&maps.v, h * Sh::kCols, kvh, id, off);
       if (!ok) break;
       if (Sh::kTiles == 2 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
       id = next_id;
@@ -570,18 +573,18 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
   }
 }
 
-// ---- products: one thread ----
+// ---- products ----
 template <int HD>
 __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
   using Sh = Shape<HD>;
-  const uint32_t tmem = c.tmem, stages = tiles + Sh::kQBytes;
+  const uint32_t tmem = uniform(c.tmem), stages = tiles + Sh::kQBytes;
   constexpr uint32_t kScores = instruction(true, false, kM, kN);
   constexpr uint32_t kSum = instruction(true, true, kM, Sh::kCols);
   int stage = 0, queued = 0;
   uint32_t phase = 0, q_phase = 0, p_count[2] = {0, 0}, buffers = 0;
 #define WAIT(bar, parity) \
-  if (!wait_one(bar, parity, &c.abort, a.err)) return false
-  auto wait_stage = [&]() { return wait_one(c.kv_full[stage], phase, &c.abort, a.err); };
+  if (!wait_warp(bar, parity, &c.abort, a.err)) return false
+  auto wait_stage = [&]() { return wait_warp(c.kv_full[stage], phase, &c.abort, a.err); };
   auto take = [&]() {
     const int was = stage;
     if (++stage == Sh::kStages) {
@@ -593,39 +596,62 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
   auto scores = [&](int t, int buffer, int st, int half, bool add) {
     const uint32_t q = tiles + (t * (HD / 64) + half * (Sh::kCols / 64)) * kChunkBytes;
     const uint32_t k = stages + st * Sh::kStageBytes;
+    const uint64_t q_desc = desc_k_major(q), k_desc = desc_k_major(k);
+    if (elect_one()) {
 #pragma unroll
-    for (int x = 0; x < Sh::kCols / 64; ++x)
+      for (int x = 0; x < Sh::kCols / 64; ++x)
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        mma_ss(tmem + buffer * kN, desc_k_major(q + x * kChunkBytes + 32 * y),
-               desc_k_major(k + x * kChunkBytes + 32 * y), kScores, add || x + y > 0);
+        for (int y = 0; y < 4; ++y) {
+          const uint64_t step = (x * kChunkBytes + 32 * y) >> 4;
+          mma_ss(tmem + buffer * kN, q_desc + step, k_desc + step, kScores, add || x + y > 0);
+        }
+    }
+    __syncwarp();
   };
-  auto sum = [&](int o_col, int buffer, int st, bool add) {
-    const uint32_t v = stages + st * Sh::kStageBytes;
+  // Half of a tile's positions: those whose weights the softmax threads write first (part 0) or
+  // last.  Two tiles: the lower and upper 64.  256-dim heads: each warpgroup's 64 in halves.
+  auto sum = [&](int o_col, int buffer, int st, int part, bool add) {
+    const uint64_t v_desc = desc_mn_major(stages + st * Sh::kStageBytes, kChunkBytes);
+    if (elect_one()) {
 #pragma unroll
-    for (int x = 0; x < kN / 16; ++x)
-      mma_ts(tmem + o_col, tmem + buffer * kN + 8 * x,
-             desc_mn_major(v + x * 16 * 128, kChunkBytes), kSum, add || x > 0);
+      for (int i = 0; i < kN / 32; ++i) {
+        const int x = Sh::kTiles == 2 ? 4 * part + i : 2 * part + (i & 1) + 4 * (i >> 1);
+        mma_ts(tmem + o_col, tmem + buffer * kN + 8 * x, v_desc + (x * 16 * 128 >> 4), kSum,
+               add || part + i > 0);
+      }
+    }
+    __syncwarp();
   };
-  auto commit = [&](const uint64_t& bar) { mma_commit(smem_u32(&bar)); };
+  auto commit = [&](const uint64_t& bar) {
+    if (elect_one()) mma_commit(smem_u32(&bar));
+    __syncwarp();
+  };
   for (;;) {
     const int at = queued % kQueue;
     WAIT(c.item_full[at], (queued / kQueue) & 1);
     const Item it = c.items[at];
-    mbar_arrive(smem_u32(&c.item_empty[at]));
+    __syncwarp();
+    if (elect_one()) mbar_arrive(smem_u32(&c.item_empty[at]));
     ++queued;
-    if (it.flags & kItemEnd) return true;
-    if (!it.kvn) continue;
-    const int j0 = it.kv0, j1 = it.kv0 + it.kvn;
+    if (uniform(it.flags) & kItemEnd) return true;
+    const int kvn = uniform(it.kvn);
+    if (!kvn) continue;
+    const int j0 = uniform(it.kv0), j1 = j0 + kvn;
     WAIT(c.q_full, q_phase);
     q_phase ^= 1;
     if constexpr (Sh::kTiles == 2) {
       int b[2], e[2];
       tile_range<HD>(a, it, 0, b[0], e[0]);
       tile_range<HD>(a, it, 1, b[1], e[1]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        b[t] = uniform(b[t]);
+        e[t] = uniform(e[t]);
+      }
       if (!wait_stage()) return false;
       tc_fence_after();
       int k_st = take();
+#pragma unroll
       for (int t = 0; t < 2; ++t)
         if (b[t] <= j0 && j0 < e[t]) {
           scores(t, t, k_st, 0, false);
@@ -641,10 +667,13 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (b[t] <= j && j < e[t]) {
-            WAIT(c.p_full[t], p_count[t] & 1);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              WAIT(c.p_full[t][part], p_count[t] & 1);
+              tc_fence_after();
+              sum(Sh::kO + t * Sh::kOStride, t, v_st, part, j > b[t]);
+            }
             ++p_count[t];
-            tc_fence_after();
-            sum(Sh::kO + t * Sh::kOStride, t, v_st, j > b[t]);
             if (j + 1 == e[t]) commit(c.o_full[t]);
           }
           if (more && b[t] <= j + 1 && j + 1 < e[t]) {
@@ -685,14 +714,22 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
         if (j + 1 < j1 && !next_scores()) return false;
         if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1)) commit(c.q_empty);
         const int buffer = p_count[0] & 1;
-        WAIT(c.p_full[buffer], (p_count[0] >> 1) & 1);
-        ++p_count[0];
-        for (int h = 0; h < Sh::kHalves; ++h) {
-          if (!wait_stage()) return false;
+        const uint32_t p_phase = (p_count[0]++ >> 1) & 1;
+        int v_st[Sh::kHalves];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          WAIT(c.p_full[buffer][part], p_phase);
           tc_fence_after();
-          const int st = take();
-          sum(Sh::kO + h * Sh::kCols, buffer, st, j > j0);
-          commit(c.kv_empty[st]);
+#pragma unroll
+          for (int h = 0; h < Sh::kHalves; ++h) {
+            if (part == 0) {
+              if (!wait_stage()) return false;
+              tc_fence_after();
+              v_st[h] = take();
+            }
+            sum(Sh::kO + h * Sh::kCols, buffer, v_st[h], part, j > j0);
+            if (part == 1) commit(c.kv_empty[v_st[h]]);
+          }
         }
         commit(c.o_full[buffer]);
       }
@@ -851,77 +888,12 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         return;
       tc_fence_after();
       const uint32_t bad = c.bad[(tiles_seen_before + (j - it.kv0)) % kBadRing];
-      if (warp_live) {
-        float s[Sh::kScoreCols];
-#pragma unroll
-        for (int x = 0; x < Sh::kScoreCols; x += 32)
-          tmem_ld32(s_addr + share * Sh::kScoreCols + x, reinterpret_cast<uint32_t*>(s + x));
-        tmem_wait_ld();
-        const int base = j * kN + share * Sh::kScoreCols;
-        const int last = see_hi - base, first = see_lo - base;
-        const bool edge = live && (last < Sh::kScoreCols - 1 || first > 0);
-        if (bad || __any_sync(0xffffffffu, edge)) {
-#pragma unroll
-          for (int w = 0; w < Sh::kScoreCols / 32; ++w) {
-            uint32_t hide = outside(last - 32 * w, first - 32 * w);
-            if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + 32 * w, a.copy_shift);
-#pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (hide >> x & 1) s[32 * w + x] = -INFINITY;
-          }
-        }
-        float top[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) top[x] = fmaxf(s[x], s[x + 4]);
-#pragma unroll
-        for (int x = 8; x < Sh::kScoreCols; ++x) top[x & 3] = fmaxf(top[x & 3], s[x]);
-        float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (!kTwo) {  // the other half of the row's columns
-          float* mine = c.swap[scored & 1][share];
-          mine[row] = mt;
-          named_barrier(1 + quad, 64);
-          mt = fmaxf(mt, c.swap[scored & 1][share ^ 1][row]);
-        }
-        if (j == b) {
-          m = mt;
-        } else if (__any_sync(0xffffffffu, mt > m + slack)) {
-          const float grown = fmaxf(m, mt);
-          const float f = m == -INFINITY ? 0.0f : exp2_approx((m - grown) * sl);
-          l *= f;
-          m = grown;
-          if (!kTwo) {  // the sum over the tile before may still be running
-            if (!wait_sum()) return;
-            tc_fence_after();
-          }
-#pragma unroll 1
-          for (int x = 0; x < Sh::kOutCols; x += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + x, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-            tmem_st32(o_addr + x, o);
-          }
-          tmem_wait_st();
-        }
-        const float ref = m == -INFINITY ? 0.0f : m * sl;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int x = 0; x < Sh::kScoreCols; x += 32) {
-          uint32_t p[16];
-#pragma unroll
-          for (int y = 0; y < 32; y += 2) {
-            const float p0 = exp2_approx(fmaf(s[x + y], sl, -ref));
-            const float p1 = exp2_approx(fmaf(s[x + y + 1], sl, -ref));
-            sum[y & 2] += p0;
-            sum[(y & 2) + 1] += p1;
-            p[y / 2] = pack_bf16(p0, p1);
-          }
-          tmem_st16(s_addr + (share * Sh::kScoreCols + x) / 2, p);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-      }
+      // 256-dim heads: a warp may already be a tile ahead of another, so a barrier a buffer
+      auto ready = [&](int part) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c.p_full[buffer][part]));
+      };
       // V rows of this tile that no row of the item sees, in copies that hold others it does
       const int z_lo = item_lo - j * kN, z_hi = item_hi - j * kN;
       if (z_lo > 0 || z_hi < kN) {
@@ -949,10 +921,96 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         }
         fence_async_smem();
       }
-      tc_fence_before();
-      __syncwarp();
-      // 256-dim heads: a warp may already be a tile ahead of another, so a barrier a buffer
-      if (lane == 0) mbar_arrive(smem_u32(&c.p_full[buffer]));
+      if (!warp_live) {
+        ready(0);
+        ready(1);
+      } else {
+        float s[Sh::kScoreCols];
+#pragma unroll
+        for (int x = 0; x < Sh::kScoreCols; x += 32)
+          tmem_ld32(s_addr + share * Sh::kScoreCols + x, reinterpret_cast<uint32_t*>(s + x));
+        tmem_wait_ld();
+        const int base = j * kN + share * Sh::kScoreCols;
+        const int last = see_hi - base, first = see_lo - base;
+        const bool edge = live && (last < Sh::kScoreCols - 1 || first > 0);
+        if (bad || __any_sync(0xffffffffu, edge)) {
+#pragma unroll
+          for (int w = 0; w < Sh::kScoreCols / 32; ++w) {
+            uint32_t hide = outside(last - 32 * w, first - 32 * w);
+            if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + 32 * w, a.copy_shift);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (hide >> x & 1) s[32 * w + x] = -INFINITY;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top[x] = max3(s[3 * x], s[3 * x + 1], s[3 * x + 2]);
+#pragma unroll
+        for (int x = 12; x + 1 < Sh::kScoreCols; x += 2)
+          top[x / 2 & 3] = max3(top[x / 2 & 3], s[x], s[x + 1]);
+        float mt = max2(max2(top[0], top[1]), max2(top[2], top[3]));
+        if (!kTwo) {  // the other half of the row's columns
+          float* mine = c.swap[scored & 1][share];
+          mine[row] = mt;
+          named_barrier(1 + quad, 64);
+          mt = max2(mt, c.swap[scored & 1][share ^ 1][row]);
+        }
+        if (j == b) {
+          m = mt;
+        } else if (__any_sync(0xffffffffu, !(mt <= m + slack))) {  // NaN too
+          const float grown = max2(m, mt);
+          const float f = m == -INFINITY ? 0.0f : exp2_approx((m - grown) * sl);
+          l *= f;
+          m = grown;
+          if (!kTwo) {  // the sum over the tile before may still be running
+            if (!wait_sum()) return;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int x = 0; x < Sh::kOutCols; x += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + x, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tmem_st32(o_addr + x, o);
+          }
+          tmem_wait_st();
+        }
+        // +inf gives NaN, as inf - inf would in every weight
+        const float ref = m == -INFINITY ? 0.0f : fmaf(m, sl, m - m);
+        const uint64_t sl2 = pair(sl, sl), ref2 = pair(-ref, -ref);
+        uint64_t sums[2] = {0, 0};
+#pragma unroll
+        for (int x = 0; x < Sh::kScoreCols; x += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            const uint64_t z = fma2(pair(s[x + y], s[x + y + 1]), sl2, ref2);
+            float p0, p1;
+            if (y / 2 % Sh::kPolyOf < Sh::kPoly) {
+              exp2_poly2(z, p0, p1);
+            } else {
+              split(z, p0, p1);
+              p0 = exp2_approx(p0);
+              p1 = exp2_approx(p1);
+            }
+            sums[y / 2 & 1] = add2(sums[y / 2 & 1], pair(p0, p1));
+            p[y / 2] = pack_bf16(p0, p1);
+          }
+          tmem_st16(s_addr + (share * Sh::kScoreCols + x) / 2, p);
+          if (x + 32 == Sh::kScoreCols / 2) {
+            tmem_wait_st();
+            ready(0);
+          }
+        }
+        float l0, l1;
+        split(add2(sums[0], sums[1]), l0, l1);
+        l += l0 + l1;
+        tmem_wait_st();
+        ready(1);
+      }
       ++scored;
       if (!kTwo) ++summed;
     }
@@ -1068,7 +1126,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(smem_u32(&c.q_empty), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&c.s_full[i]), 1);
-      mbar_init(smem_u32(&c.p_full[i]), Sh::kTiles == 2 ? 4 : 8);
+      for (int part = 0; part < 2; ++part)
+        mbar_init(smem_u32(&c.p_full[i][part]), Sh::kTiles == 2 ? 4 : 8);
       mbar_init(smem_u32(&c.o_full[i]), 1);
     }
     for (int i = 0; i < kQueue; ++i) {
@@ -1097,12 +1156,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kLoadWarp) {
       load_role<HD>(a, maps, c, tiles, lane);
     } else if (warp == kMmaWarp) {
-      if (lane == 0) {
-        mma_items<HD>(a, c, tiles);
-        mma_commit(smem_u32(&c.drained));  // no product or arrival is under way after this
-        const long long start = clock64();
-        while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
-        }
+      mma_items<HD>(a, c, tiles);
+      // one lane issued every product: it is the one elected here too
+      if (elect_one()) mma_commit(smem_u32(&c.drained));
+      __syncwarp();  // no product or arrival is under way after this:
+      const long long start = clock64();
+      while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
       }
     } else if (warp == kPlanWarp) {
       plan_role<HD>(a, c, lane);

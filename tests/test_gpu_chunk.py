@@ -2,8 +2,9 @@
 
 Tolerance of an element, with A = sum_c w_c |v_c| (the oracle's second result): the weights are
 rounded to bf16 (2^-8 of each: 2^-8 A), a score is off by at most (D + 4) 2^-24 scale |q| |k| and
-a weight by twice that share, the exponential and the two sums by (8 + L) 2^-24 at most, and the
-result is rounded to bf16 (2^-8 |out|).
+a weight by twice that share, the exponential by 3e-6 (its polynomial) and as much in the sum it
+is divided by, the two sums by (8 + L) 2^-24 at most, and the result is rounded to bf16 (2^-8
+|out|).
 """
 
 from __future__ import annotations
@@ -88,7 +89,7 @@ class Batch:
         longest = max([n for _, n in self.lens] + [1])
         k = self.key.float().nan_to_num(0, 0, 0).norm(dim=-1).max().item() * self.scales[0]
         score = (self.D + 4) * F32 * self.scale * self.q.float().norm(dim=-1).max().item() * k
-        rel = 2.0 ** -8 + 2 * score + (8 + longest) * F32
+        rel = 2.0 ** -8 + 2 * score + 6e-6 + (8 + longest) * F32
         tol = rel * size + 2.0 ** -8 * want.abs() * (1 + rel) + 2.0 ** -130
         off = (out.double() - want).abs()
         bad = ~(off <= tol) & owned[:, None]
