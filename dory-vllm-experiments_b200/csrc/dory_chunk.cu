@@ -37,6 +37,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 
@@ -218,10 +219,7 @@ struct Shape {
 
 constexpr int kSoftmaxWarps = 8;
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kPlanWarp = 10;
-constexpr int kThreads = 12 * 32;  // three whole warpgroups: registers are handed over by group
-// Registers a thread: 168 at launch (384 threads, 64,512 in all); the softmax groups, which hold
-// a row's 128 scores, take what the third group gives up: 2 x 128 x 200 + 128 x 104 = 64,512.
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+constexpr int kThreads = 12 * 32;
 
 enum : int { kItemEnd = 1 };
 struct Item {
@@ -247,7 +245,7 @@ struct Control {  // shared memory behind the tiles
   float swap[2][2][kM];  // the warpgroups' halves of a row's maximum and sum (256-dim heads)
 };
 
-__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
                                        uint32_t* err) {
   const long long start = clock64();
   while (!mbar_try(bar, parity)) {
@@ -456,34 +454,38 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
 }
 
 // ---- loader ----
+// Ring stages are used in the order K0 V0 K1 V1 .. of an item's tiles; with 256-dim heads (two
+// stages a tile, and K of the next tile wanted before V of this one) K0 K1 V0 K2 V1 ...
 template <int HD>
 __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, uint32_t tiles,
                           int lane) {
   using Sh = Shape<HD>;
+  constexpr int kCopies = kN / 16;  // of a tile, at most
   const uint32_t stages = tiles + Sh::kQBytes;
   const int copies = kN / a.copy_rows;
+  const bool one_copy_blocks = a.copy_rows == a.B;
   int stage = 0, queued = 0, q_uses = 0;
-  uint32_t phase = 1, tile_no = 0;  // of the stage's empty barrier: free at first
-  uint32_t issued = 0;
+  uint32_t phase = 1, tile_no = 0, issued = 0;  // phase of the stage's empty barrier: free at first
   bool ok = true;
-  // One ring stage: columns [64 col, 64 col + kCols) of a cache tile whose copy `lane` has
-  // block `id` (a.blocks, beyond the cache: zeros) and first row `off`.
-  auto fill = [&](const CUtensorMap* map, int col, int kvh, int id, int off) {
+  struct Pages {  // a tile's copies: block and first row, uniform values
+    int block[kCopies], row[kCopies];
+  };
+  // One ring stage: columns [col, col + kCols) of a cache tile.
+  auto fill = [&](const CUtensorMap* map, int col, int kvh, const Pages& p) {
     if (!wait_warp(c.kv_empty[stage], phase, &c.abort, a.err)) return false;
-    const uint32_t bar = smem_u32(&c.kv_full[stage]);
-    const uint32_t dst = stages + stage * Sh::kStageBytes;
-    if (elect_one()) mbar_expect(bar, Sh::kStageBytes);
-    __syncwarp();
-    for (int i = 0; i < copies; ++i) {
-      const int block = uniform(lane == i ? id : INT_MIN), row = uniform(lane == i ? off : INT_MIN);
-      if (elect_one()) {
+    if (elect_one()) {
+      const uint32_t bar = smem_u32(&c.kv_full[stage]);
+      const uint32_t dst = stages + stage * Sh::kStageBytes;
+      mbar_expect(bar, Sh::kStageBytes);
 #pragma unroll
-        for (int k = 0; k < Sh::kCols / 64; ++k)
-          tma_load_4d(dst + k * kChunkBytes + i * a.copy_rows * 128, map, col + 64 * k, row, kvh,
-                      block, bar);
-      }
-      __syncwarp();
+      for (int x = 0; x < kCopies; ++x)
+        if (x < copies)
+#pragma unroll
+          for (int k = 0; k < Sh::kCols / 64; ++k)
+            tma_load_4d(dst + k * kChunkBytes + x * a.copy_rows * 128, map, col + 64 * k, p.row[x],
+                        kvh, p.block[x], bar);
     }
+    __syncwarp();
     ++issued;
     if (++stage == Sh::kStages) {
       stage = 0;
@@ -499,7 +501,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     if (elect_one()) mbar_arrive(smem_u32(&c.item_empty[at]));
     ++queued;
     if (uniform(it.flags) & kItemEnd) break;
-    const int kvn = uniform(it.kvn), kvh = uniform(it.kvh);
+    const int kvn = uniform(it.kvn), kv0 = uniform(it.kv0), kvh = uniform(it.kvh);
     if (!kvn) continue;
     // the queries
     if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
@@ -516,61 +518,75 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
                       tok0 + t * a.TB, bar);
     }
     __syncwarp();
-    // the cache tiles: K of tile j + 1 goes in before V of tile j (256-dim heads need it first)
     const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
     const int hi = min(it.pos0 + it.ntok, it.cap);
     const int32_t* table = a.tables + int64_t(it.seq) * a.table_stride;
-    auto look_up = [&](int j, int& id, int& off) {
-      const int pos = j * kN + lane * a.copy_rows;
-      const int block = pos / a.B;
-      off = pos - block * a.B;
-      id = int(a.blocks);
-      bool bad = false;
-      if (lane < copies && pos < hi && pos + a.copy_rows > lo) {
-        const int entry = table[block];
+    // Lane x's copy of tile i: its block, or one beyond the cache, which loads as zeros.
+    auto look_up = [&](int i, bool& bad) {
+      const int pos = (kv0 + i) * kN + lane * a.copy_rows;
+      int id = int(a.blocks);
+      bad = false;
+      if (lane < copies && i < kvn && pos < hi && pos + a.copy_rows > lo) {
+        const int entry = table[pos / a.B];
         bad = entry < 0 || entry >= a.blocks;
         if (!bad) id = entry;
       }
-      return __ballot_sync(0xffffffffu, bad);
+      return id;
     };
-    int id = 0, off = 0, next_id = 0, next_off = 0;
-    uint32_t bad = look_up(it.kv0, id, off), next_bad = 0;
-    auto fill_k = [&](uint32_t mask, int i, int o) {
-      if (lane == 0) {
+    bool bad;
+    int id = look_up(0, bad);
+    Pages now, next;
+    // Tile i's pages and its mask of bad ones; the look-up of tile i + 1 is in flight afterwards.
+    auto pages = [&](int i, Pages& p) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+      if (elect_one()) {
         c.bad[tile_no % kBadRing] = mask;
         if (mask) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
       }
+      __syncwarp();
       ++tile_no;
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x) {
+        p.block[x] = uniform(lane == x ? id : INT_MIN);
+        p.row[x] = one_copy_blocks ? 0 : ((kv0 + i) * kN + x * a.copy_rows) % a.B;
+      }
+      id = look_up(i + 1, bad);
+    };
+    auto fill_tile = [&](const CUtensorMap* map, const Pages& p) {
+#pragma unroll
       for (int h = 0; h < Sh::kHalves; ++h)
-        if (!fill(&maps.k, h * Sh::kCols, kvh, i, o)) return false;
+        if (!fill(map, h * Sh::kCols, kvh, p)) return false;
       return true;
     };
-    if (!(ok = fill_k(bad, id, off))) break;
-    for (int j = 0; j < kvn; ++j) {
-      const bool more = j + 1 < kvn;
-      if (more) next_bad = look_up(it.kv0 + j + 1, next_id, next_off);
-      if (Sh::kTiles == 1 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
-      for (int h = 0; h < Sh::kHalves && ok; ++h)
-        ok = fill(&maps.v, h * Sh::kCols, kvh, id, off);
-      if (!ok) break;
-      if (Sh::kTiles == 2 && more && !(ok = fill_k(next_bad, next_id, next_off))) break;
-      id = next_id;
-      off = next_off;
+    pages(0, now);
+    ok = fill_tile(&maps.k, now);
+    for (int i = 0; ok && i < kvn; ++i) {
+      const bool more = i + 1 < kvn;
+      if (more) pages(i + 1, next);
+      if (Sh::kTiles == 1 && more) ok = fill_tile(&maps.k, next);
+      if (ok) ok = fill_tile(&maps.v, now);
+      if (Sh::kTiles == 2 && more && ok) ok = fill_tile(&maps.k, next);
+      now = next;
     }
     if (!ok) break;
   }
   if (!ok) {  // given up: no copy may land after the CTA has gone
-    for (uint32_t i = issued > Sh::kStages ? issued - Sh::kStages : 0; i < issued; ++i) {
-      const long long start = clock64();
-      while (!mbar_try(smem_u32(&c.kv_full[i % Sh::kStages]), (i / Sh::kStages) & 1) &&
-             clock64() - start < 100000000LL) {
-      }
-    }
     const long long start = clock64();
+    for (uint32_t i = issued > Sh::kStages ? issued - Sh::kStages : 0; i < issued; ++i)
+      while (!mbar_try(smem_u32(&c.kv_full[i % Sh::kStages]), (i / Sh::kStages) & 1) &&
+             clock64() - start < 200000000LL) {
+      }
     while (q_uses && !mbar_try(smem_u32(&c.q_full), (q_uses - 1) & 1) &&
-           clock64() - start < 100000000LL) {
+           clock64() - start < 300000000LL) {
     }
   }
+}
+
+// Column, within a score buffer, of the weights of positions [16 x, 16 x + 16): each warpgroup
+// puts its own over the scores it has read.
+template <int HD>
+__host__ __device__ constexpr int weight_column(int x) {
+  return Shape<HD>::kTiles == 2 || x < 4 ? 8 * x : kN / 2 + 8 * (x - 4);
 }
 
 // ---- products ----
@@ -616,7 +632,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
 #pragma unroll
       for (int i = 0; i < kN / 32; ++i) {
         const int x = Sh::kTiles == 2 ? 4 * part + i : 2 * part + (i & 1) + 4 * (i >> 1);
-        mma_ts(tmem + o_col, tmem + buffer * kN + 8 * x, v_desc + (x * 16 * 128 >> 4), kSum,
+        mma_ts(tmem + o_col, tmem + buffer * kN + weight_column<HD>(x), v_desc + (x * 16 * 128 >> 4), kSum,
                add || part + i > 0);
       }
     }
@@ -748,7 +764,7 @@ struct RowOut {
   float2* part_ml;     // may be null: another warp writes it
 };
 template <int HD, bool KV8>
-__device__ __forceinline__ void redo_row(const ChunkArgs& a, int seq, int token, int head, int lo,
+__device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, int head, int lo,
                                       int hi, int col0, int cols, RowOut o) {
   const int lane = threadIdx.x & 31;
   const __nv_bfloat16* q = a.q + token * a.q_t + head * a.q_h;
@@ -806,27 +822,23 @@ __device__ __forceinline__ void redo_row(const ChunkArgs& a, int seq, int token,
   if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
 }
 
-// Eight consecutive gate values.
-__device__ __forceinline__ void load_gate8(const ChunkArgs& a, int64_t at, float (&g)[8]) {
-  if (a.gate_dtype == DORY_DTYPE_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.gate) + at);
-    const float4 x = p[0], y = p[1];
-    g[0] = x.x; g[1] = x.y; g[2] = x.z; g[3] = x.w;
-    g[4] = y.x; g[5] = y.y; g[6] = y.z; g[7] = y.w;
+// Four gate values of the bits loaded for them (16-bit types: the first two words).
+__device__ __forceinline__ void apply_gate4(int dtype, const uint4& w, float* v) {
+  if (dtype == DORY_DTYPE_F32) {
+    v[0] *= __uint_as_float(w.x);
+    v[1] *= __uint_as_float(w.y);
+    v[2] *= __uint_as_float(w.z);
+    v[3] *= __uint_as_float(w.w);
+  } else if (dtype == DORY_DTYPE_BF16) {
+    v[0] *= __uint_as_float(w.x << 16);
+    v[1] *= __uint_as_float(w.x & 0xffff0000u);
+    v[2] *= __uint_as_float(w.y << 16);
+    v[3] *= __uint_as_float(w.y & 0xffff0000u);
   } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.gate) + at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (a.gate_dtype == DORY_DTYPE_BF16) {
-        g[2 * i] = __uint_as_float(u[i] << 16);
-        g[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        g[2 * i] = f.x;
-        g[2 * i + 1] = f.y;
-      }
-    }
+    v[0] *= __half2float(__ushort_as_half(w.x & 0xffff));
+    v[1] *= __half2float(__ushort_as_half(w.x >> 16));
+    v[2] *= __half2float(__ushort_as_half(w.y & 0xffff));
+    v[3] *= __half2float(__ushort_as_half(w.y >> 16));
   }
 }
 
@@ -867,19 +879,16 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
   for (;;) {
     const int at = queued % kQueue;
     if (!wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err)) return;
-    const Item it = c.items[at];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
-    ++queued;
+    // left in shared memory: what the loop over the tiles does not use would only hold registers
+    const Item& it = c.items[at];
     if (it.flags & kItemEnd) return;
     int b, e;
     tile_range<HD>(a, it, t, b, e);
-    const int tok = t * a.TB + row_tok, pos = it.pos0 + tok;
+    const int tok = t * a.TB + row_tok;
     const bool live = row_real && tok < it.ntok;
     const bool warp_live = __any_sync(0xffffffffu, live);
+    const int pos = it.pos0 + tok;
     const int see_hi = min(pos, it.cap - 1), see_lo = a.window ? max(0, pos - a.window + 1) : 0;
-    const int item_lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
-    const int item_hi = min(it.pos0 + it.ntok, it.cap);
     float m = -INFINITY, l = 0.0f;
     for (int j = b; j < e; ++j) {
       const int buffer = kTwo ? t : int(scored & 1);
@@ -895,7 +904,8 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         if (lane == 0) mbar_arrive(smem_u32(&c.p_full[buffer][part]));
       };
       // V rows of this tile that no row of the item sees, in copies that hold others it does
-      const int z_lo = item_lo - j * kN, z_hi = item_hi - j * kN;
+      const int z_lo = (a.window ? max(0, it.pos0 - a.window + 1) : 0) - j * kN;
+      const int z_hi = min(it.pos0 + it.ntok, it.cap) - j * kN;
       if (z_lo > 0 || z_hi < kN) {
         const int i = j - it.kv0;  // the tile's place in the piece, and so its V stages
         const uint32_t v_no =
@@ -925,31 +935,45 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         ready(0);
         ready(1);
       } else {
-        float s[Sh::kScoreCols];
-#pragma unroll
-        for (int x = 0; x < Sh::kScoreCols; x += 32)
-          tmem_ld32(s_addr + share * Sh::kScoreCols + x, reinterpret_cast<uint32_t*>(s + x));
-        tmem_wait_ld();
+        const uint32_t own_scores = s_addr + share * Sh::kScoreCols;
         const int base = j * kN + share * Sh::kScoreCols;
         const int last = see_hi - base, first = see_lo - base;
-        const bool edge = live && (last < Sh::kScoreCols - 1 || first > 0);
-        if (bad || __any_sync(0xffffffffu, edge)) {
+        const bool edge = bad || __any_sync(0xffffffffu,
+                                            live && (last < Sh::kScoreCols - 1 || first > 0));
+        // scores x .. x + 31 of the row, the hidden ones -infinity
+        auto load_scores = [&](int x, float* s) {
+          tmem_ld32(own_scores + x, reinterpret_cast<uint32_t*>(s));
+          tmem_wait_ld();
+          if (edge) {
+            uint32_t hide = outside(last - x, first - x);
+            if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + x, a.copy_shift);
 #pragma unroll
-          for (int w = 0; w < Sh::kScoreCols / 32; ++w) {
-            uint32_t hide = outside(last - 32 * w, first - 32 * w);
-            if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + 32 * w, a.copy_shift);
+            for (int y = 0; y < 32; ++y)
+              if (hide >> y & 1) s[y] = -INFINITY;
+          }
+        };
+        float mt = -INFINITY;
+        if (!edge) {
+          float s[Sh::kScoreCols], top[4];
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (hide >> x & 1) s[32 * w + x] = -INFINITY;
+          for (int x = 0; x < Sh::kScoreCols; x += 32)
+            tmem_ld32(own_scores + x, reinterpret_cast<uint32_t*>(s + x));
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) top[x] = max3(s[3 * x], s[3 * x + 1], s[3 * x + 2]);
+#pragma unroll
+          for (int x = 12; x < Sh::kScoreCols; x += 2)
+            top[x / 2 & 3] = max3(top[x / 2 & 3], s[x], s[x + 1]);
+          mt = max2(max2(top[0], top[1]), max2(top[2], top[3]));
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < Sh::kScoreCols; x += 32) {
+            float s[32];
+            load_scores(x, s);
+#pragma unroll
+            for (int y = 0; y < 32; y += 2) mt = max3(mt, s[y], s[y + 1]);
           }
         }
-        float top[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) top[x] = max3(s[3 * x], s[3 * x + 1], s[3 * x + 2]);
-#pragma unroll
-        for (int x = 12; x + 1 < Sh::kScoreCols; x += 2)
-          top[x / 2 & 3] = max3(top[x / 2 & 3], s[x], s[x + 1]);
-        float mt = max2(max2(top[0], top[1]), max2(top[2], top[3]));
         if (!kTwo) {  // the other half of the row's columns
           float* mine = c.swap[scored & 1][share];
           mine[row] = mt;
@@ -982,12 +1006,16 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         const float ref = m == -INFINITY ? 0.0f : fmaf(m, sl, m - m);
         const uint64_t sl2 = pair(sl, sl), ref2 = pair(-ref, -ref);
         uint64_t sums[2] = {0, 0};
-#pragma unroll
+        // The scores are read again, a piece at a time: a loop, not 128 unrolled columns, because
+        // the instructions of a straight run have to come from L2 time and again.
+#pragma unroll 1
         for (int x = 0; x < Sh::kScoreCols; x += 32) {
+          float s[32];
           uint32_t p[16];
+          load_scores(x, s);
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            const uint64_t z = fma2(pair(s[x + y], s[x + y + 1]), sl2, ref2);
+            const uint64_t z = fma2(pair(s[y], s[y + 1]), sl2, ref2);
             float p0, p1;
             if (y / 2 % Sh::kPolyOf < Sh::kPoly) {
               exp2_poly2(z, p0, p1);
@@ -999,7 +1027,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
             sums[y / 2 & 1] = add2(sums[y / 2 & 1], pair(p0, p1));
             p[y / 2] = pack_bf16(p0, p1);
           }
-          tmem_st16(s_addr + (share * Sh::kScoreCols + x) / 2, p);
+          tmem_st16(own_scores + x / 2, p);
           if (x + 32 == Sh::kScoreCols / 2) {
             tmem_wait_st();
             ready(0);
@@ -1023,7 +1051,15 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       if (!wait_sum()) return;
       tc_fence_after();
     }
-    if (!warp_live) continue;
+    auto done = [&]() {  // with the item
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
+      ++queued;
+    };
+    if (!warp_live) {
+      done();
+      continue;
+    }
     if (!kTwo) {
       // the sums of the two halves; the buffer of the tile before the last is free
       float* mine = c.swap[scored & 1][share];
@@ -1032,85 +1068,127 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       l += c.swap[scored & 1][share ^ 1][row];
       named_barrier(1 + quad, 64);
     }
-    const int token = it.tok0 + tok, head = it.kvh * a.G + row_head;
-    const int col0 = share * Sh::kOutCols;
-    const int64_t column = int64_t(head) * HD + col0;
+    // Opaque here, or the compiler computes everything below that depends on them alone once,
+    // ahead of the items, and spills it across the loop over the tiles.
+    int own_lane = lane, own_row = t * kM + row, col0 = share * Sh::kOutCols;
+    asm volatile("" : "+r"(own_lane), "+r"(own_row), "+r"(col0));
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + t * kM + row;
-    RowOut ro;
-    ro.out = it.slot < 0 ? a.out + token * a.out_t + column : nullptr;
-    ro.gate_at = a.gate ? token * a.gate_t + column : -1;
-    ro.part_o = a.part_o + slot_row * HD + col0;
-    ro.part_ml = share == 0 ? a.part_ml + slot_row : nullptr;
+    const bool whole = it.slot < 0;
+    // A thread holds a row's columns; memory wants a row's columns side by side in a warp.  So
+    // eight lanes exchange 16-byte pieces, 32 columns at a time: lane i then has piece i of each
+    // of its group's eight rows, and a load or store covers whole 128-byte lines.  (A row a
+    // thread instead takes 32 lines an instruction: 20,500 clocks an item with an FP32 gate.)
+    const int group = own_lane & ~7, piece = (own_lane & 7) * 4;
+    const uint32_t alive = __ballot_sync(0xffffffffu, live) >> group;
+    const int where = row_head << 16 | tok;  // tok < 256
+    int64_t out_at[8], gate_at[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int w = __shfl_sync(0xffffffffu, where, group + k);
+      const int64_t token = it.tok0 + (w & 0xffff);
+      const int64_t column = int64_t(it.kvh * a.G + (w >> 16)) * HD + col0 + piece;
+      if (whole) {
+        out_at[k] = token * a.out_t + column;
+        gate_at[k] = token * a.gate_t + column;
+      } else {
+        out_at[k] = (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + group + k) * HD + col0 +
+                    piece;
+        gate_at[k] = 0;
+      }
+    }
     float odd = 0.0f;  // NaN once a value is not finite
 #pragma unroll 1
     for (int x = 0; x < Sh::kOutCols; x += 32) {
       float o[32];
-      if (e > b) {
-        tmem_ld32(o_addr + x, reinterpret_cast<uint32_t*>(o));
-        tmem_wait_ld();
-      } else {
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-      }
-      if (live) {
+      for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+      if (e > b) tmem_ld32(o_addr + x, reinterpret_cast<uint32_t*>(o));
+      uint4 g[8];
 #pragma unroll
-      for (int y = 0; y < 32; ++y) odd = fmaf(o[y], 0.0f, odd);
-      if (it.slot >= 0) {
+      for (int k = 0; k < 8; ++k) g[k] = make_uint4(0, 0, 0, 0);  // or they live from the start on
+      if (whole && a.gate) {
+        if (a.gate_dtype == DORY_DTYPE_F32) {
 #pragma unroll
-        for (int y = 0; y < 32; y += 4)
-          *reinterpret_cast<float4*>(ro.part_o + x + y) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-      } else {
+          for (int k = 0; k < 8; ++k)
+            if (alive >> k & 1)
+              g[k] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + gate_at[k] + x);
+        } else {
 #pragma unroll
-        for (int y = 0; y < 32; y += 8) {
-          float g[8];
-          if (a.gate) {
-            load_gate8(a, ro.gate_at + x + y, g);
-#pragma unroll
-            for (int z = 0; z < 8; ++z) g[z] *= inv;
-          } else {
-#pragma unroll
-            for (int z = 0; z < 8; ++z) g[z] = inv;
-          }
-          uint4 w;
-          w.x = pack_bf16(o[y] * g[0], o[y + 1] * g[1]);
-          w.y = pack_bf16(o[y + 2] * g[2], o[y + 3] * g[3]);
-          w.z = pack_bf16(o[y + 4] * g[4], o[y + 5] * g[5]);
-          w.w = pack_bf16(o[y + 6] * g[6], o[y + 7] * g[7]);
-          *reinterpret_cast<uint4*>(ro.out + x + y) = w;
+          for (int k = 0; k < 8; ++k)
+            if (alive >> k & 1) {
+              const uint2 w =
+                  *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.gate) + gate_at[k] + x);
+              g[k].x = w.x;
+              g[k].y = w.y;
+            }
         }
       }
+      tmem_wait_ld();
+#pragma unroll
+      for (int y = 0; y < 32; ++y) odd = fmaf(o[y], 0.0f, odd);
+      if (whole) {
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] *= inv;
+      }
+#pragma unroll
+      for (int step = 1; step < 8; step <<= 1) {
+        const bool upper = own_lane & step;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k & step) continue;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            float& low = o[4 * k + y];
+            float& high = o[4 * (k | step) + y];
+            const float got = __shfl_xor_sync(0xffffffffu, upper ? low : high, step);
+            low = upper ? got : low;
+            high = upper ? high : got;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (!(alive >> k & 1)) continue;
+        float* v = o + 4 * k;
+        if (whole) {
+          if (a.gate) apply_gate4(a.gate_dtype, g[k], v);
+          *reinterpret_cast<uint2*>(a.out + out_at[k] + x) =
+              make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + out_at[k] + x) = make_float4(v[0], v[1], v[2], v[3]);
+        }
       }
       __syncwarp();
     }
-    if (live && it.slot >= 0 && share == 0)
-      *ro.part_ml = make_float2(m == -INFINITY ? 0.0f : m * sl, l);
+    const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
+    if (live && !whole && share == 0)
+      a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl, l);
     uint32_t again = __ballot_sync(0xffffffffu, live && isnan(odd) && isfinite(l));
     while (again) {
       const int src = __ffs(again) - 1;
       again &= again - 1;
-      const int r_tok = __shfl_sync(0xffffffffu, token, src);
-      const int r_head = __shfl_sync(0xffffffffu, head, src);
+      const int r_token = it.tok0 + __shfl_sync(0xffffffffu, tok, src);
+      const int r_head = it.kvh * a.G + __shfl_sync(0xffffffffu, row_head, src);
       const int lo = max(__shfl_sync(0xffffffffu, see_lo, src), it.kv0 * kN);
       const int hi = min(__shfl_sync(0xffffffffu, see_hi, src) + 1, (it.kv0 + it.kvn) * kN);
+      const int64_t r_slot = __shfl_sync(0xffffffffu, slot_row, src);
+      const int64_t column = int64_t(r_head) * HD + col0;
       RowOut r;
-      r.out = reinterpret_cast<__nv_bfloat16*>(
-          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.out), src));
-      r.gate_at = __shfl_sync(0xffffffffu, ro.gate_at, src);
-      r.part_o = reinterpret_cast<float*>(
-          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.part_o), src));
-      r.part_ml = reinterpret_cast<float2*>(
-          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ro.part_ml), src));
-      if (it.slot < 0) r.part_ml = nullptr;
-      redo_row<HD, false>(a, it.seq, r_tok, r_head, lo, hi, col0, Sh::kOutCols, r);
+      r.out = whole ? a.out + r_token * a.out_t + column : nullptr;
+      r.gate_at = a.gate ? r_token * a.gate_t + column : -1;
+      r.part_o = a.part_o + r_slot * HD + col0;
+      r.part_ml = !whole && share == 0 ? a.part_ml + r_slot : nullptr;
+      __syncwarp();
+      redo_row<HD, false>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
       __syncwarp();
     }
+    done();
   }
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
-    chunk_kernel(const ChunkArgs a, const __grid_constant__ Maps maps) {
+    chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ Maps maps) {
   using Sh = Shape<HD>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Control<HD>& c = *reinterpret_cast<Control<HD>*>(smem + Sh::kQBytes + Sh::kStages * Sh::kStageBytes);
@@ -1149,10 +1227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp < kSoftmaxWarps) {
-    regs_up<kSoftmaxRegs>();
     softmax_role<HD>(a, c, tiles, warp, lane);
   } else {
-    regs_down<kOtherRegs>();
     if (warp == kLoadWarp) {
       load_role<HD>(a, maps, c, tiles, lane);
     } else if (warp == kMmaWarp) {

@@ -194,16 +194,6 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) {
   return __reduce_max_sync(0xffffffffu, x);
 }
 
-// ---- registers of a warpgroup ----
-template <int N>
-__device__ __forceinline__ void regs_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // ---- arithmetic ----
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
