@@ -19,12 +19,11 @@
 //              table into a ring; pages outside the item's positions, and bad block ids, load
 //              as zeros without touching memory;
 //   products   tcgen05: S = Q K^T into tensor memory, O += P V with P read from there;
-//   softmax    two warpgroups, a row (or half a row) per thread: scores to registers, running
-//              maximum, exponentials, P back to tensor memory as 16-bit floats, and at the
-//              end of an item O / sum, gate and store.
+//   softmax    four warpgroups, a half (256-dim heads: a quarter) of a row per thread: scores to
+//              registers, running maximum, exponentials, P back to tensor memory as 16-bit
+//              floats, and at the end of an item O / sum, gate and store.
 // With 64/128-dim heads an item has two tiles and the products of one overlap the softmax of
-// the other.  With 256-dim heads tensor memory holds one tile's O and two score buffers, and
-// the two warpgroups share each tile's columns.
+// the other.  With 256-dim heads tensor memory holds one tile's O and two score buffers.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8: the weights stay below
 // 2^8, far from the range's end, and most tiles touch O not at all.
@@ -58,6 +57,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kM = 128;              // rows of a tensor-core tile
 constexpr int kN = 128;              // positions of a cache tile
 constexpr int kChunkBytes = kN * 128;  // 64 columns of a tile: 128 rows of 128 bytes
+constexpr int kItemUnits = 3;        // cost of an item's output, in cache tiles
 constexpr int kQueue = 4;            // items handed out ahead
 constexpr int kBadRing = 16;         // tiles whose bad-page masks are kept
 constexpr int kMaxPosition = 1 << 30;
@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(128) chunk_rows(const ChunkArgs a) {
 // ------------------------------------------------------------------------------------
 // The tensor-core kernel
 // ------------------------------------------------------------------------------------
+constexpr int kWide128 = 1, kWide256 = 4;
 template <int HD>
 struct Shape {
   static constexpr int kTiles = HD == 256 ? 1 : 2;           // tensor-core tiles of an item
@@ -207,19 +208,20 @@ struct Shape {
   static constexpr int kStageBytes = kCols / 64 * kChunkBytes;
   static constexpr int kStages = HD == 64 ? 8 : 5;
   static constexpr int kQBytes = kTiles * HD / 64 * kChunkBytes;
-  static constexpr int kScoreCols = kTiles == 2 ? kN : kN / 2;  // of a row, per softmax thread
-  static constexpr int kOutCols = kTiles == 2 ? HD : HD / 2;
+  static constexpr int kShares = HD == 256 ? kWide256 : kWide128;  // softmax warpgroups of a tile
+  static constexpr int kScoreCols = kN / kShares;            // of a row, per softmax thread
+  static constexpr int kOutCols = HD / kShares;
+  static constexpr int kParts = kScoreCols > 32 ? 2 : 1;     // the weights are handed over in
+  static constexpr int kPartCols = kScoreCols / kParts;
+  static constexpr int kSoftmaxWarps = 4 * kShares * kTiles;
+  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1,
+                       kPlanWarp = kSoftmaxWarps + 2;
+  static constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
   static constexpr int kItemRows = kTiles * kM;
-  // of kPolyOf pairs of exponentials, kPoly go to the FP32 pipe
-  static constexpr int kPoly = 1, kPolyOf = 4;
   // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
   static constexpr int kO = 2 * kN;
   static constexpr int kOStride = HD <= 128 ? 128 : 0;       // between the tiles' O
 };
-
-constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kPlanWarp = 10;
-constexpr int kThreads = 12 * 32;
 
 enum : int { kItemEnd = 1 };
 struct Item {
@@ -242,7 +244,7 @@ struct Control {  // shared memory behind the tiles
   uint32_t bad[kBadRing];
   uint32_t tmem;
   int abort;
-  float swap[2][2][kM];  // the warpgroups' halves of a row's maximum and sum (256-dim heads)
+  float swap[Shape<HD>::kTiles][Shape<HD>::kShares][kM];  // a row's maxima and sums, by share
 };
 
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
@@ -305,10 +307,12 @@ __device__ __forceinline__ Seq sequence(const ChunkArgs& a, int i) {
   }
   return s;
 }
+// An item's units: its cache tiles (one at least: an item that sees nothing still writes its
+// zeros), then kItemUnits for what it costs besides them.
 __device__ __forceinline__ int item_units(const ChunkArgs& a, const Seq& s, int m, int tokens,
                                           int& first, int& tiles) {
   tiles = tiles_seen(s.pos + m * tokens, min(tokens, s.n - m * tokens), s.cap, a.window, first);
-  return max(tiles, 1);  // an item that sees nothing still writes its zeros
+  return max(tiles, 1) + kItemUnits;
 }
 // Units of one KV head of every lane's sequence.
 __device__ __forceinline__ long long head_units(const ChunkArgs& a, const Seq& s, int tokens,
@@ -413,28 +417,31 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
     for (long long at = u0; at < u1;) {
       const int units = item_units(a, s, m, tokens, first, tiles);
       const int take = int(min((long long)(units - off), u1 - at));
-      const bool whole = off == 0 && take == units;
-      Item it;
-      it.flags = 0;
-      it.kv0 = first + off;
-      it.kvn = tiles ? take : 0;
-      it.tok0 = s.t0 + m * tokens;
-      it.ntok = min(tokens, s.n - m * tokens);
-      it.pos0 = s.pos + m * tokens;
-      it.kvh = kvh;
-      it.seq = seq;
-      it.cap = s.cap;
-      it.slot = whole ? -1 : (off == 0 ? 2 * cta + 1 : 2 * cta);
-      if (!whole && off == 0) {
-        cut = 1;
-        if (lane == 0) {
-          join[0] = int((at + units - 1) / per) - cta + 1;  // CTAs that hold a part
-          join[1] = it.tok0;
-          join[2] = it.ntok;
-          join[3] = kvh;
+      const int work = units - kItemUnits;  // cache tiles, or 1
+      if (off < work) {
+        const bool whole = off == 0 && take >= work;
+        Item it;
+        it.flags = 0;
+        it.kv0 = first + off;
+        it.kvn = tiles ? min(take, work - off) : 0;
+        it.tok0 = s.t0 + m * tokens;
+        it.ntok = min(tokens, s.n - m * tokens);
+        it.pos0 = s.pos + m * tokens;
+        it.kvh = kvh;
+        it.seq = seq;
+        it.cap = s.cap;
+        it.slot = whole ? -1 : (off == 0 ? 2 * cta + 1 : 2 * cta);
+        if (!whole && off == 0) {
+          cut = 1;
+          if (lane == 0) {
+            join[0] = int((at + work - 1) / per) - cta + 1;  // CTAs that hold a part
+            join[1] = it.tok0;
+            join[2] = it.ntok;
+            join[3] = kvh;
+          }
         }
+        if (!push(it)) return;
       }
-      if (!push(it)) return;
       at += take;
       off = 0;
       if (++m * tokens >= s.n) {
@@ -454,45 +461,38 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
 }
 
 // ---- loader ----
-// Ring stages are used in the order K0 V0 K1 V1 .. of an item's tiles; with 256-dim heads (two
-// stages a tile, and K of the next tile wanted before V of this one) K0 K1 V0 K2 V1 ...
+// What ring stage q of an item's n tiles holds.  Stages are used in the order K0 V0 K1 V1 ..;
+// with 256-dim heads (two stages a tile, and K of the next tile wanted before V of this one)
+// K0 K1 V0 K2 V1 .. Vn-1.
+template <int HD>
+__device__ __forceinline__ void stage_holds(int q, int n, bool& is_v, int& tile, int& half) {
+  if (Shape<HD>::kTiles == 2) {
+    is_v = q & 1;
+    tile = q >> 1;
+    half = 0;
+    return;
+  }
+  const int r = q - 2, step = r >> 2;  // K of tile step + 1, then V of tile step
+  half = q & 1;
+  is_v = r >= 0 && (r & 2 || step + 1 >= n);
+  tile = r < 0 ? 0 : is_v ? step : step + 1;
+}
+// The first stage of V of tile i.
+template <int HD>
+__device__ __forceinline__ uint32_t stage_of_v(int i, int n) {
+  if (Shape<HD>::kTiles == 2) return 2 * i + 1;
+  return i + 1 < n ? 4 * i + 4 : 4 * i + 2;
+}
+
 template <int HD>
 __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, uint32_t tiles,
                           int lane) {
   using Sh = Shape<HD>;
-  constexpr int kCopies = kN / 16;  // of a tile, at most
   const uint32_t stages = tiles + Sh::kQBytes;
   const int copies = kN / a.copy_rows;
-  const bool one_copy_blocks = a.copy_rows == a.B;
   int stage = 0, queued = 0, q_uses = 0;
   uint32_t phase = 1, tile_no = 0, issued = 0;  // phase of the stage's empty barrier: free at first
   bool ok = true;
-  struct Pages {  // a tile's copies: block and first row, uniform values
-    int block[kCopies], row[kCopies];
-  };
-  // One ring stage: columns [col, col + kCols) of a cache tile.
-  auto fill = [&](const CUtensorMap* map, int col, int kvh, const Pages& p) {
-    if (!wait_warp(c.kv_empty[stage], phase, &c.abort, a.err)) return false;
-    if (elect_one()) {
-      const uint32_t bar = smem_u32(&c.kv_full[stage]);
-      const uint32_t dst = stages + stage * Sh::kStageBytes;
-      mbar_expect(bar, Sh::kStageBytes);
-#pragma unroll
-      for (int x = 0; x < kCopies; ++x)
-        if (x < copies)
-#pragma unroll
-          for (int k = 0; k < Sh::kCols / 64; ++k)
-            tma_load_4d(dst + k * kChunkBytes + x * a.copy_rows * 128, map, col + 64 * k, p.row[x],
-                        kvh, p.block[x], bar);
-    }
-    __syncwarp();
-    ++issued;
-    if (++stage == Sh::kStages) {
-      stage = 0;
-      phase ^= 1;
-    }
-    return true;
-  };
   for (;;) {
     const int at = queued % kQueue;
     if (!(ok = wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err))) break;
@@ -503,30 +503,18 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     if (uniform(it.flags) & kItemEnd) break;
     const int kvn = uniform(it.kvn), kv0 = uniform(it.kv0), kvh = uniform(it.kvh);
     if (!kvn) continue;
-    // the queries
-    if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
-    ++q_uses;
-    const int tok0 = uniform(it.tok0);
-    const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
-    if (elect_one()) {
-      const uint32_t bar = smem_u32(&c.q_full);
-      mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
-      for (int t = 0; t < filled; ++t)
-#pragma unroll
-        for (int k = 0; k < HD / 64; ++k)
-          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
-                      tok0 + t * a.TB, bar);
-    }
-    __syncwarp();
     const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
     const int hi = min(it.pos0 + it.ntok, it.cap);
     const int32_t* table = a.tables + int64_t(it.seq) * a.table_stride;
-    // Lane x's copy of tile i: its block, or one beyond the cache, which loads as zeros.
-    auto look_up = [&](int i, bool& bad) {
-      const int pos = (kv0 + i) * kN + lane * a.copy_rows;
+    // Lane x's copy of stage q: its block, or one beyond the cache, which loads as zeros.
+    auto look_up = [&](int q, bool& bad) {
+      bool is_v;
+      int tile, half;
+      stage_holds<HD>(q, kvn, is_v, tile, half);
+      const int pos = (kv0 + tile) * kN + lane * a.copy_rows;
       int id = int(a.blocks);
       bad = false;
-      if (lane < copies && i < kvn && pos < hi && pos + a.copy_rows > lo) {
+      if (lane < copies && tile < kvn && pos < hi && pos + a.copy_rows > lo) {
         const int entry = table[pos / a.B];
         bad = entry < 0 || entry >= a.blocks;
         if (!bad) id = entry;
@@ -535,43 +523,78 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     };
     bool bad;
     int id = look_up(0, bad);
-    Pages now, next;
-    // Tile i's pages and its mask of bad ones; the look-up of tile i + 1 is in flight afterwards.
-    auto pages = [&](int i, Pages& p) {
-      const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+    // the queries
+    if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
+    ++q_uses;
+    const int tok0 = uniform(it.tok0);
+    const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
+    if (elect_one()) {
+      const uint32_t bar = smem_u32(&c.q_full);
+      mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
+#pragma unroll 1
+      for (int t = 0; t < filled; ++t)
+#pragma unroll 1
+        for (int k = 0; k < HD / 64; ++k)
+          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
+                      tok0 + t * a.TB, bar);
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
+      bool is_v;
+      int tile, half;
+      stage_holds<HD>(q, kvn, is_v, tile, half);
+      if (!is_v && half == 0) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+        if (elect_one()) {
+          c.bad[tile_no % kBadRing] = mask;
+          if (mask) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
+        }
+        __syncwarp();
+        ++tile_no;
+      }
+      const int own = id;
+      id = look_up(q + 1, bad);  // in flight while this stage's copies are issued
+      if (!(ok = wait_warp(c.kv_empty[stage], phase, &c.abort, a.err))) break;
+      const uint32_t bar = smem_u32(&c.kv_full[stage]);
+      const uint32_t dst = stages + stage * Sh::kStageBytes;
+      const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+      // Every copy's block in registers first, then one elected run of copies: 28 clocks a copy
+      // of 2 KB; a loop that fetches each block as it goes took 47, a copy a lane 66.
+      int block[kN / 16], row[kN / 16];
+#pragma unroll
+      for (int x = 0; x < kN / 16; ++x) {
+        block[x] = __shfl_sync(0xffffffffu, own, x);
+        row[x] = 0;
+      }
+      if (a.copy_rows != a.B) {
+#pragma unroll
+        for (int x = 0; x < kN / 16; ++x)
+          row[x] = ((kv0 + tile) * kN + x * a.copy_rows) % a.B;
+      }
       if (elect_one()) {
-        c.bad[tile_no % kBadRing] = mask;
-        if (mask) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
+        mbar_expect(bar, Sh::kStageBytes);
+#pragma unroll
+        for (int x = 0; x < kN / 16; ++x) {
+          if (x < copies)
+#pragma unroll
+            for (int k = 0; k < Sh::kCols / 64; ++k)
+              tma_load_4d(dst + k * kChunkBytes + x * a.copy_rows * 128, map,
+                          half * Sh::kCols + 64 * k, row[x], kvh, block[x], bar);
+        }
       }
       __syncwarp();
-      ++tile_no;
-#pragma unroll
-      for (int x = 0; x < kCopies; ++x) {
-        p.block[x] = uniform(lane == x ? id : INT_MIN);
-        p.row[x] = one_copy_blocks ? 0 : ((kv0 + i) * kN + x * a.copy_rows) % a.B;
+      ++issued;
+      if (++stage == Sh::kStages) {
+        stage = 0;
+        phase ^= 1;
       }
-      id = look_up(i + 1, bad);
-    };
-    auto fill_tile = [&](const CUtensorMap* map, const Pages& p) {
-#pragma unroll
-      for (int h = 0; h < Sh::kHalves; ++h)
-        if (!fill(map, h * Sh::kCols, kvh, p)) return false;
-      return true;
-    };
-    pages(0, now);
-    ok = fill_tile(&maps.k, now);
-    for (int i = 0; ok && i < kvn; ++i) {
-      const bool more = i + 1 < kvn;
-      if (more) pages(i + 1, next);
-      if (Sh::kTiles == 1 && more) ok = fill_tile(&maps.k, next);
-      if (ok) ok = fill_tile(&maps.v, now);
-      if (Sh::kTiles == 2 && more && ok) ok = fill_tile(&maps.k, next);
-      now = next;
     }
     if (!ok) break;
   }
   if (!ok) {  // given up: no copy may land after the CTA has gone
     const long long start = clock64();
+#pragma unroll 1
     for (uint32_t i = issued > Sh::kStages ? issued - Sh::kStages : 0; i < issued; ++i)
       while (!mbar_try(smem_u32(&c.kv_full[i % Sh::kStages]), (i / Sh::kStages) & 1) &&
              clock64() - start < 200000000LL) {
@@ -586,7 +609,8 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
 // puts its own over the scores it has read.
 template <int HD>
 __host__ __device__ constexpr int weight_column(int x) {
-  return Shape<HD>::kTiles == 2 || x < 4 ? 8 * x : kN / 2 + 8 * (x - 4);
+  constexpr int kSteps = Shape<HD>::kScoreCols / 16;
+  return x / kSteps * Shape<HD>::kScoreCols + x % kSteps * 8;
 }
 
 // ---- products ----
@@ -597,7 +621,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
   constexpr uint32_t kScores = instruction(true, false, kM, kN);
   constexpr uint32_t kSum = instruction(true, true, kM, Sh::kCols);
   int stage = 0, queued = 0;
-  uint32_t phase = 0, q_phase = 0, p_count[2] = {0, 0}, buffers = 0;
+  uint32_t phase = 0, q_phase = 0, p_phase = 0, p_count = 0, buffers = 0;
 #define WAIT(bar, parity) \
   if (!wait_warp(bar, parity, &c.abort, a.err)) return false
   auto wait_stage = [&]() { return wait_warp(c.kv_full[stage], phase, &c.abort, a.err); };
@@ -624,15 +648,17 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
     }
     __syncwarp();
   };
-  // Half of a tile's positions: those whose weights the softmax threads write first (part 0) or
-  // last.  Two tiles: the lower and upper 64.  256-dim heads: each warpgroup's 64 in halves.
+  // A part of a tile's positions: the same part of each softmax warpgroup's.
   auto sum = [&](int o_col, int buffer, int st, int part, bool add) {
-    const uint64_t v_desc = desc_mn_major(stages + st * Sh::kStageBytes, kChunkBytes);
+    constexpr int kSteps = Sh::kPartCols / 16;
+    const uint32_t weights = tmem + buffer * kN + 8 * kSteps * part;
+    const uint64_t v_desc = desc_mn_major(stages + st * Sh::kStageBytes, kChunkBytes) +
+                            (part * kSteps * 16 * 128 >> 4);
     if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < kN / 32; ++i) {
-        const int x = Sh::kTiles == 2 ? 4 * part + i : 2 * part + (i & 1) + 4 * (i >> 1);
-        mma_ts(tmem + o_col, tmem + buffer * kN + weight_column<HD>(x), v_desc + (x * 16 * 128 >> 4), kSum,
+      for (int i = 0; i < kSteps * Sh::kShares; ++i) {
+        const int x = i / kSteps * (Sh::kScoreCols / 16) + i % kSteps;  // in part 0
+        mma_ts(tmem + o_col, weights + weight_column<HD>(x), v_desc + (x * 16 * 128 >> 4), kSum,
                add || part + i > 0);
       }
     }
@@ -656,20 +682,19 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
     WAIT(c.q_full, q_phase);
     q_phase ^= 1;
     if constexpr (Sh::kTiles == 2) {
-      int b[2], e[2];
-      tile_range<HD>(a, it, 0, b[0], e[0]);
-      tile_range<HD>(a, it, 1, b[1], e[1]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        b[t] = uniform(b[t]);
-        e[t] = uniform(e[t]);
-      }
+      int b0, b1, e0, e1;
+      tile_range<HD>(a, it, 0, b0, e0);
+      tile_range<HD>(a, it, 1, b1, e1);
+      b0 = uniform(b0);
+      b1 = uniform(b1);
+      e0 = uniform(e0);
+      e1 = uniform(e1);
       if (!wait_stage()) return false;
       tc_fence_after();
       int k_st = take();
-#pragma unroll
+#pragma unroll 1
       for (int t = 0; t < 2; ++t)
-        if (b[t] <= j0 && j0 < e[t]) {
+        if ((t ? b1 : b0) <= j0 && j0 < (t ? e1 : e0)) {
           scores(t, t, k_st, 0, false);
           commit(c.s_full[t]);
         }
@@ -680,19 +705,20 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
         const int v_st = take();
         const bool more = j + 1 < j1;
         k_st = -1;
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-          if (b[t] <= j && j < e[t]) {
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              WAIT(c.p_full[t][part], p_count[t] & 1);
+          const int b = t ? b1 : b0, e = t ? e1 : e0;
+          if (b <= j && j < e) {
+#pragma unroll 1
+            for (int part = 0; part < Sh::kParts; ++part) {
+              WAIT(c.p_full[t][part], p_phase >> t & 1);
               tc_fence_after();
-              sum(Sh::kO + t * Sh::kOStride, t, v_st, part, j > b[t]);
+              sum(Sh::kO + t * Sh::kOStride, t, v_st, part, j > b);
             }
-            ++p_count[t];
-            if (j + 1 == e[t]) commit(c.o_full[t]);
+            p_phase ^= 1u << t;
+            if (j + 1 == e) commit(c.o_full[t]);
           }
-          if (more && b[t] <= j + 1 && j + 1 < e[t]) {
+          if (more && b <= j + 1 && j + 1 < e) {
             if (k_st < 0) {
               if (!wait_stage()) return false;
               tc_fence_after();
@@ -729,12 +755,12 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
       for (int j = j0; j < j1; ++j) {
         if (j + 1 < j1 && !next_scores()) return false;
         if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1)) commit(c.q_empty);
-        const int buffer = p_count[0] & 1;
-        const uint32_t p_phase = (p_count[0]++ >> 1) & 1;
+        const int buffer = p_count & 1;
+        const uint32_t parity = (p_count++ >> 1) & 1;
         int v_st[Sh::kHalves];
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          WAIT(c.p_full[buffer][part], p_phase);
+        for (int part = 0; part < Sh::kParts; ++part) {
+          WAIT(c.p_full[buffer][part], parity);
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < Sh::kHalves; ++h) {
@@ -744,7 +770,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
               v_st[h] = take();
             }
             sum(Sh::kO + h * Sh::kCols, buffer, v_st[h], part, j > j0);
-            if (part == 1) commit(c.kv_empty[v_st[h]]);
+            if (part + 1 == Sh::kParts) commit(c.kv_empty[v_st[h]]);
           }
         }
         commit(c.o_full[buffer]);
@@ -774,6 +800,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
   float m = -INFINITY, l = 0.0f, acc[HD / 32];
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
+#pragma unroll 1
   for (int c0 = lo; c0 < hi; c0 += 32) {
     const int c = c0 + lane;
     float s = -INFINITY;
@@ -783,6 +810,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
       if (id >= 0) {
         at = id * a.sb + int64_t(c % a.B) * a.so + kv;
         float dot = 0.0f;
+#pragma unroll 4
         for (int i = 0; i < HD; ++i) dot += __bfloat162float(q[i]) * cache_value<KV8>(a.kc, at + i);
         s = dot * qk;
       }
@@ -795,6 +823,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
     l = l * shrink + w;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) acc[i] *= shrink;
+#pragma unroll 1
     for (int k = 0; k < 32; ++k) {
       const int64_t row = __shfl_sync(0xffffffffu, at, k);
       const float wk = __shfl_sync(0xffffffffu, w, k);
@@ -822,6 +851,12 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
   if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
 }
 
+__device__ __forceinline__ uint4 load_gate4(const ChunkArgs& a, int64_t at) {
+  if (a.gate_dtype == DORY_DTYPE_F32)
+    return *reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + at);
+  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.gate) + at);
+  return make_uint4(w.x, w.y, 0, 0);
+}
 // Four gate values of the bits loaded for them (16-bit types: the first two words).
 __device__ __forceinline__ void apply_gate4(int dtype, const uint4& w, float* v) {
   if (dtype == DORY_DTYPE_F32) {
@@ -858,8 +893,10 @@ template <int HD>
 __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles, int warp, int lane) {
   using Sh = Shape<HD>;
   constexpr bool kTwo = Sh::kTiles == 2;
-  const int wg = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
-  const int t = kTwo ? wg : 0, share = kTwo ? 0 : wg;  // tile, and which half of its columns
+  const int quad = warp & 3, row = quad * 32 + lane;
+  const int t = (warp >> 2) / Sh::kShares, share = (warp >> 2) % Sh::kShares;
+  // the warps that share rows, of one tile
+  auto meet = [&]() { named_barrier(1 + t * 4 + quad, Sh::kShares * 32); };
   const uint32_t tmem = c.tmem + (uint32_t(quad * 32) << 16);
   const uint32_t o_addr = tmem + Sh::kO + t * Sh::kOStride + share * Sh::kOutCols;
   const uint32_t stages = tiles + Sh::kQBytes;
@@ -889,6 +926,14 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     const bool warp_live = __any_sync(0xffffffffu, live);
     const int pos = it.pos0 + tok;
     const int see_hi = min(pos, it.cap - 1), see_lo = a.window ? max(0, pos - a.window + 1) : 0;
+    if (live && a.gate && it.slot < 0) {  // the gate's row, wanted at the end
+      const int size = a.gate_dtype == DORY_DTYPE_F32 ? 4 : 2;
+      const char* at_gate =
+          static_cast<const char*>(a.gate) +
+          ((it.tok0 + tok) * a.gate_t + int64_t(it.kvh * a.G + row_head) * HD + share * Sh::kOutCols) * size;
+      for (int x = 0; x < Sh::kOutCols * size; x += 128)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(at_gate + x));
+    }
     float m = -INFINITY, l = 0.0f;
     for (int j = b; j < e; ++j) {
       const int buffer = kTwo ? t : int(scored & 1);
@@ -908,8 +953,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       const int z_hi = min(it.pos0 + it.ntok, it.cap) - j * kN;
       if (z_lo > 0 || z_hi < kN) {
         const int i = j - it.kv0;  // the tile's place in the piece, and so its V stages
-        const uint32_t v_no =
-            stage_no + (kTwo ? 2 * i + 1 : 2 * Sh::kHalves * i + (i + 1 < it.kvn ? 2 : 1) * Sh::kHalves);
+        const uint32_t v_no = stage_no + stage_of_v<HD>(i, it.kvn);
         const int r1 = z_lo > 0 ? (z_lo & ~(a.copy_rows - 1)) : 0, r2 = max(z_lo, 0);
         const int r3 = min(z_hi, kN), r4 = (r3 + a.copy_rows - 1) & ~(a.copy_rows - 1);
         for (int h = 0; h < Sh::kHalves; ++h) {
@@ -918,7 +962,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           if (!wait_warp(c.kv_full[st], (no / Sh::kStages) & 1, &c.abort, a.err)) return;
           constexpr int kPieces = Sh::kCols / 8;  // 16-byte pieces of a row
           const int rows = (r2 - r1) + (r4 - r3);
-          for (int x = (kTwo ? quad : warp) * 32 + lane; x < rows * kPieces; x += (kTwo ? 4 : 8) * 32) {
+          for (int x = (share * 4 + quad) * 32 + lane; x < rows * kPieces; x += Sh::kShares * 128) {
             int r = x / kPieces;
             const int piece = x % kPieces;
             r = r < r2 - r1 ? r1 + r : r3 + (r - (r2 - r1));
@@ -932,18 +976,19 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         fence_async_smem();
       }
       if (!warp_live) {
-        ready(0);
-        ready(1);
+        for (int part = 0; part < Sh::kParts; ++part) ready(part);
       } else {
         const uint32_t own_scores = s_addr + share * Sh::kScoreCols;
         const int base = j * kN + share * Sh::kScoreCols;
         const int last = see_hi - base, first = see_lo - base;
         const bool edge = bad || __any_sync(0xffffffffu,
                                             live && (last < Sh::kScoreCols - 1 || first > 0));
-        // scores x .. x + 31 of the row, the hidden ones -infinity
-        auto load_scores = [&](int x, float* s) {
+        // scores x .. x + 31 of the row: asked for, and there, the hidden ones -infinity
+        auto ask_scores = [&](int x, float* s) {
           tmem_ld32(own_scores + x, reinterpret_cast<uint32_t*>(s));
-          tmem_wait_ld();
+        };
+        auto get_scores = [&](int x, float* s) {
+          tmem_wait_ld32(reinterpret_cast<uint32_t*>(s));
           if (edge) {
             uint32_t hide = outside(last - x, first - x);
             if (bad) hide |= bad_columns(bad, share * Sh::kScoreCols + x, a.copy_shift);
@@ -957,8 +1002,10 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           float s[Sh::kScoreCols], top[4];
 #pragma unroll
           for (int x = 0; x < Sh::kScoreCols; x += 32)
-            tmem_ld32(own_scores + x, reinterpret_cast<uint32_t*>(s + x));
-          tmem_wait_ld();
+            ask_scores(x, s + x);
+          tmem_wait_ld32(reinterpret_cast<uint32_t*>(s));
+#pragma unroll
+          for (int x = 32; x < Sh::kScoreCols; x += 32) tmem_more32(reinterpret_cast<uint32_t*>(s + x));
 #pragma unroll
           for (int x = 0; x < 4; ++x) top[x] = max3(s[3 * x], s[3 * x + 1], s[3 * x + 2]);
 #pragma unroll
@@ -969,16 +1016,18 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
 #pragma unroll 1
           for (int x = 0; x < Sh::kScoreCols; x += 32) {
             float s[32];
-            load_scores(x, s);
+            ask_scores(x, s);
+            get_scores(x, s);
 #pragma unroll
             for (int y = 0; y < 32; y += 2) mt = max3(mt, s[y], s[y + 1]);
           }
         }
-        if (!kTwo) {  // the other half of the row's columns
-          float* mine = c.swap[scored & 1][share];
-          mine[row] = mt;
-          named_barrier(1 + quad, 64);
-          mt = max2(mt, c.swap[scored & 1][share ^ 1][row]);
+        if constexpr (Sh::kShares > 1) {  // the rest of the row's columns
+          c.swap[t][share][row] = mt;
+          meet();
+#pragma unroll
+          for (int x = 1; x < Sh::kShares; ++x) mt = max2(mt, c.swap[t][(share + x) % Sh::kShares][row]);
+          if (!kTwo) meet();  // a warp may go on to the next tile while another still reads
         }
         if (j == b) {
           m = mt;
@@ -995,7 +1044,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           for (int x = 0; x < Sh::kOutCols; x += 32) {
             uint32_t o[32];
             tmem_ld32(o_addr + x, o);
-            tmem_wait_ld();
+            tmem_wait_ld32(o);
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
             tmem_st32(o_addr + x, o);
@@ -1012,23 +1061,19 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         for (int x = 0; x < Sh::kScoreCols; x += 32) {
           float s[32];
           uint32_t p[16];
-          load_scores(x, s);
+          ask_scores(x, s);
+          get_scores(x, s);
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            const uint64_t z = fma2(pair(s[y], s[y + 1]), sl2, ref2);
             float p0, p1;
-            if (y / 2 % Sh::kPolyOf < Sh::kPoly) {
-              exp2_poly2(z, p0, p1);
-            } else {
-              split(z, p0, p1);
-              p0 = exp2_approx(p0);
-              p1 = exp2_approx(p1);
-            }
+            split(fma2(pair(s[y], s[y + 1]), sl2, ref2), p0, p1);
+            p0 = exp2_approx(p0);
+            p1 = exp2_approx(p1);
             sums[y / 2 & 1] = add2(sums[y / 2 & 1], pair(p0, p1));
             p[y / 2] = pack_bf16(p0, p1);
           }
           tmem_st16(own_scores + x / 2, p);
-          if (x + 32 == Sh::kScoreCols / 2) {
+          if (Sh::kParts > 1 && x + 32 == Sh::kPartCols) {
             tmem_wait_st();
             ready(0);
           }
@@ -1037,7 +1082,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
         split(add2(sums[0], sums[1]), l0, l1);
         l += l0 + l1;
         tmem_wait_st();
-        ready(1);
+        ready(Sh::kParts - 1);
       }
       ++scored;
       if (!kTwo) ++summed;
@@ -1060,13 +1105,14 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       done();
       continue;
     }
-    if (!kTwo) {
-      // the sums of the two halves; the buffer of the tile before the last is free
-      float* mine = c.swap[scored & 1][share];
-      mine[row] = l;
-      named_barrier(1 + quad, 64);
-      l += c.swap[scored & 1][share ^ 1][row];
-      named_barrier(1 + quad, 64);
+    if constexpr (Sh::kShares > 1) {
+      // the sums of the shares; each warp is past its last tile's maxima: the sum just waited for
+      // needed every share's weights
+      c.swap[t][share][row] = l;
+      meet();
+#pragma unroll
+      for (int x = 1; x < Sh::kShares; ++x) l += c.swap[t][(share + x) % Sh::kShares][row];
+      meet();
     }
     // Opaque here, or the compiler computes everything below that depends on them alone once,
     // ahead of the items, and spills it across the loop over the tiles.
@@ -1087,43 +1133,29 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       const int w = __shfl_sync(0xffffffffu, where, group + k);
       const int64_t token = it.tok0 + (w & 0xffff);
       const int64_t column = int64_t(it.kvh * a.G + (w >> 16)) * HD + col0 + piece;
-      if (whole) {
-        out_at[k] = token * a.out_t + column;
-        gate_at[k] = token * a.gate_t + column;
-      } else {
-        out_at[k] = (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + group + k) * HD + col0 +
-                    piece;
-        gate_at[k] = 0;
-      }
+      out_at[k] = whole ? token * a.out_t + column
+                        : (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + group + k) * HD +
+                              col0 + piece;
+      gate_at[k] = token * a.gate_t + column;
     }
     float odd = 0.0f;  // NaN once a value is not finite
+    uint4 g[8];  // the gate's bits, for the 32 columns to come
+    const bool gated = whole && a.gate;
+    auto ask_gate = [&](int x) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (alive >> k & 1) g[k] = load_gate4(a, gate_at[k] + x);
+    };
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g[k] = make_uint4(0, 0, 0, 0);  // or they live from the start on
+    if (gated) ask_gate(0);
 #pragma unroll 1
     for (int x = 0; x < Sh::kOutCols; x += 32) {
       float o[32];
 #pragma unroll
       for (int y = 0; y < 32; ++y) o[y] = 0.0f;
       if (e > b) tmem_ld32(o_addr + x, reinterpret_cast<uint32_t*>(o));
-      uint4 g[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = make_uint4(0, 0, 0, 0);  // or they live from the start on
-      if (whole && a.gate) {
-        if (a.gate_dtype == DORY_DTYPE_F32) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (alive >> k & 1)
-              g[k] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + gate_at[k] + x);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (alive >> k & 1) {
-              const uint2 w =
-                  *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.gate) + gate_at[k] + x);
-              g[k].x = w.x;
-              g[k].y = w.y;
-            }
-        }
-      }
-      tmem_wait_ld();
+      tmem_wait_ld32(reinterpret_cast<uint32_t*>(o));
 #pragma unroll
       for (int y = 0; y < 32; ++y) odd = fmaf(o[y], 0.0f, odd);
       if (whole) {
@@ -1146,17 +1178,20 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           }
         }
       }
+      if (gated) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) apply_gate4(a.gate_dtype, g[k], o + 4 * k);
+        if (x + 32 < Sh::kOutCols) ask_gate(x + 32);
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (!(alive >> k & 1)) continue;
-        float* v = o + 4 * k;
-        if (whole) {
-          if (a.gate) apply_gate4(a.gate_dtype, g[k], v);
+        const float* v = o + 4 * k;
+        if (whole)
           *reinterpret_cast<uint2*>(a.out + out_at[k] + x) =
               make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-        } else {
+        else
           *reinterpret_cast<float4*>(a.part_o + out_at[k] + x) = make_float4(v[0], v[1], v[2], v[3]);
-        }
       }
       __syncwarp();
     }
@@ -1187,7 +1222,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
     chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ Maps maps) {
   using Sh = Shape<HD>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -1205,20 +1240,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&c.s_full[i]), 1);
       for (int part = 0; part < 2; ++part)
-        mbar_init(smem_u32(&c.p_full[i][part]), Sh::kTiles == 2 ? 4 : 8);
+        mbar_init(smem_u32(&c.p_full[i][part]), 4 * Sh::kShares);
       mbar_init(smem_u32(&c.o_full[i]), 1);
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxWarps + 2);
+      mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + 2);
     }
     mbar_init(smem_u32(&c.drained), 1);
     c.abort = 0;
     fence_mbar_init();
     fence_async_smem();
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_u32(&c.tmem), 512);
-  if (warp == kLoadWarp && lane == 0) {
+  if (warp == Sh::kMmaWarp) tmem_alloc(smem_u32(&c.tmem), 512);
+  if (warp == Sh::kLoadWarp && lane == 0) {
     prefetch_map(&maps.q);
     prefetch_map(&maps.k);
     prefetch_map(&maps.v);
@@ -1226,12 +1261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp < kSoftmaxWarps) {
+  if (warp < Sh::kSoftmaxWarps) {
     softmax_role<HD>(a, c, tiles, warp, lane);
   } else {
-    if (warp == kLoadWarp) {
+    if (warp == Sh::kLoadWarp) {
       load_role<HD>(a, maps, c, tiles, lane);
-    } else if (warp == kMmaWarp) {
+    } else if (warp == Sh::kMmaWarp) {
       mma_items<HD>(a, c, tiles);
       // one lane issued every product: it is the one elected here too
       if (elect_one()) mma_commit(smem_u32(&c.drained));
@@ -1239,7 +1274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long long start = clock64();
       while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
       }
-    } else if (warp == kPlanWarp) {
+    } else {
       plan_role<HD>(a, c, lane);
     }
   }
@@ -1247,7 +1282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_free(c.tmem, 512);
+  if (warp == Sh::kMmaWarp) tmem_free(c.tmem, 512);
 }
 
 // Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
@@ -1388,7 +1423,7 @@ int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaS
       return fail(DORY_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     ready[device] = true;
   }
-  chunk_kernel<HD><<<ctas, kThreads, kBytes, stream>>>(a, maps);
+  chunk_kernel<HD><<<ctas, Sh::kThreads, kBytes, stream>>>(a, maps);
   int32_t status = dory::launched(cudaSuccess);
   if (status != DORY_OK) return status;
   cudaLaunchConfig_t cfg;

@@ -91,8 +91,29 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// Every load of this thread is complete; what reads these registers depends on it.  `more`:
+// another load's registers, ordered behind a wait already made.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                 "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_more32(uint32_t* r) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                 "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31]));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -229,35 +250,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// 2^x for two x below 2^7 on the FP32 pipe, for when the special-function unit is the bottleneck:
-// x = n + f with n the nearest whole number, 2^f by a degree-4 polynomial (own minimax fit of
-// the relative error on [-1/2, 1/2] with p(0) = 1: 2.9e-6 in FP32), n added to the exponent.
-// Results below 2^-126 come out as some positive value below 2^-126; -infinity, clamped to
-// -127, as exactly 0 (f = 0, p = 1, exponent 0), so a hidden position's weight is zero.
-__device__ __forceinline__ void exp2_poly2(uint64_t x, float& y0, float& y1) {
-  float x0, x1;
-  split(x, x0, x1);
-  x = pair(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
-  const float magic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the whole number
-  const uint64_t t = add2(x, pair(magic, magic));
-  const uint64_t n = add2(t, pair(-magic, -magic));
-  const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
-  uint64_t p = pair(0.00958285574f, 0.00958285574f);
-  p = fma2(p, f, pair(0.0559064299f, 0.0559064299f));
-  p = fma2(p, f, pair(0.240240991f, 0.240240991f));
-  p = fma2(p, f, pair(0.693124175f, 0.693124175f));
-  p = fma2(p, f, pair(1.0f, 1.0f));
-  float t0, t1, p0, p1;
-  split(t, t0, t1);
-  split(p, p0, p1);
-  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 // {lo, hi} as two 16-bit floats, lo in the lower half.
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
