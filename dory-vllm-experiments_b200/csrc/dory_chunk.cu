@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(128) chunk_rows(const ChunkArgs a) {
 // ------------------------------------------------------------------------------------
 // The tensor-core kernel
 // ------------------------------------------------------------------------------------
-constexpr int kWide128 = 1, kWide256 = 4;
+constexpr int kWide128 = 1, kWide256 = 2;
 template <int HD>
 struct Shape {
   static constexpr int kTiles = HD == 256 ? 1 : 2;           // tensor-core tiles of an item
@@ -214,8 +214,7 @@ struct Shape {
   static constexpr int kParts = kScoreCols > 32 ? 2 : 1;     // the weights are handed over in
   static constexpr int kPartCols = kScoreCols / kParts;
   static constexpr int kSoftmaxWarps = 4 * kShares * kTiles;
-  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1,
-                       kPlanWarp = kSoftmaxWarps + 2;
+  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;  // the last: plan
   static constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
   static constexpr int kItemRows = kTiles * kM;
   // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
@@ -315,12 +314,12 @@ __device__ __forceinline__ int item_units(const ChunkArgs& a, const Seq& s, int 
   return max(tiles, 1) + kItemUnits;
 }
 // Units of one KV head of every lane's sequence.
-__device__ __forceinline__ long long head_units(const ChunkArgs& a, const Seq& s, int tokens,
+__device__ __forceinline__ int head_units(const ChunkArgs& a, const Seq& s, int tokens,
                                                 int lane) {
   const int items = (s.n + tokens - 1) / tokens;
-  long long u = 0;
-  int first, tiles;
+  int u = 0, first, tiles;
   if (items <= 4)
+#pragma unroll 1
     for (int m = 0; m < items; ++m) u += item_units(a, s, m, tokens, first, tiles);
   uint32_t big = __ballot_sync(0xffffffffu, items > 4);
   while (big) {  // long sequences: the warp shares the items
@@ -331,16 +330,17 @@ __device__ __forceinline__ long long head_units(const ChunkArgs& a, const Seq& s
     o.n = __shfl_sync(0xffffffffu, s.n, src);
     o.pos = __shfl_sync(0xffffffffu, s.pos, src);
     o.cap = __shfl_sync(0xffffffffu, s.cap, src);
-    long long sum = 0;
+    int sum = 0;
     for (int m = lane; m * tokens < o.n; m += 32) sum += item_units(a, o, m, tokens, first, tiles);
-    for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == src) u = sum;
   }
   return u;
 }
-__device__ __forceinline__ long long scan_add(long long x, int lane) {  // inclusive
+__device__ __forceinline__ int scan_add(int x, int lane) {  // inclusive
+#pragma unroll 1
   for (int k = 1; k < 32; k <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, k);
+    const int y = __shfl_up_sync(0xffffffffu, x, k);
     if (lane >= k) x += y;
   }
   return x;
@@ -368,21 +368,20 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
   memset(&end, 0, sizeof(end));
   end.flags = kItemEnd;
 
-  long long total = 0, mine = 0;
+  int total = 0, mine = 0;
   for (int base = 0; base < a.S; base += 32) {
     mine = head_units(a, sequence(a, base + lane), tokens, lane) * a.NKV;
-    total += __shfl_sync(0xffffffffu, scan_add(mine, lane), 31);
+    total += __reduce_add_sync(0xffffffffu, mine);
   }
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_units);
-  const long long u0 = cta * per, u1 = min(u0 + per, total);
+  const int per = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_units);
+  const int u0 = min(cta * per, total), u1 = min(u0 + per, total);
   int cut = 0;  // whether this CTA holds the first part of a cut item
   if (u0 < u1) {
     // the sequence, KV head and item that hold unit u0
-    long long before = 0;
-    int seq = 0;
+    int before = 0, seq = 0;
     for (int base = 0; base < a.S; base += 32) {
       if (a.S > 32) mine = head_units(a, sequence(a, base + lane), tokens, lane) * a.NKV;
-      const long long upto = before + scan_add(mine, lane);
+      const int upto = before + scan_add(mine, lane);
       const uint32_t past = __ballot_sync(0xffffffffu, upto > u0);
       if (past) {
         const int src = __ffs(past) - 1;
@@ -393,16 +392,16 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
       before = __shfl_sync(0xffffffffu, upto, 31);
     }
     Seq s = sequence(a, seq);
-    const long long per_head =
+    const int per_head =
         __shfl_sync(0xffffffffu, head_units(a, lane ? Seq{0, 0, 0, 0} : s, tokens, lane), 0);
-    long long rest = u0 - before;
-    int kvh = int(rest / per_head), m = 0;
+    int rest = u0 - before;
+    int kvh = rest / per_head, m = 0;
     rest -= kvh * per_head;
     int first, tiles;
     for (int base = 0;; base += 32) {
       const bool real = (base + lane) * tokens < s.n;
-      const long long u = real ? item_units(a, s, base + lane, tokens, first, tiles) : 0;
-      const long long upto = scan_add(u, lane);
+      const int u = real ? item_units(a, s, base + lane, tokens, first, tiles) : 0;
+      const int upto = scan_add(u, lane);
       const uint32_t past = __ballot_sync(0xffffffffu, upto > rest);
       if (past) {
         const int src = __ffs(past) - 1;
@@ -413,10 +412,11 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
       rest -= __shfl_sync(0xffffffffu, upto, 31);
       if ((base + 32) * tokens >= s.n) break;  // not reached: rest lies within the head
     }
-    int off = int(rest);
-    for (long long at = u0; at < u1;) {
+    int off = rest;
+#pragma unroll 1
+    for (int at = u0; at < u1;) {
       const int units = item_units(a, s, m, tokens, first, tiles);
-      const int take = int(min((long long)(units - off), u1 - at));
+      const int take = min(units - off, u1 - at);
       const int work = units - kItemUnits;  // cache tiles, or 1
       if (off < work) {
         const bool whole = off == 0 && take >= work;
@@ -434,7 +434,7 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
         if (!whole && off == 0) {
           cut = 1;
           if (lane == 0) {
-            join[0] = int((at + work - 1) / per) - cta + 1;  // CTAs that hold a part
+            join[0] = (at + work - 1) / per - cta + 1;  // CTAs that hold a part
             join[1] = it.tok0;
             join[2] = it.ntok;
             join[3] = kvh;
@@ -851,29 +851,22 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
   if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
 }
 
-__device__ __forceinline__ uint4 load_gate4(const ChunkArgs& a, int64_t at) {
+// Two consecutive gate values: their bits (16-bit types: the first word), and their product.
+__device__ __forceinline__ uint2 load_gate2(const ChunkArgs& a, int64_t at) {
   if (a.gate_dtype == DORY_DTYPE_F32)
-    return *reinterpret_cast<const uint4*>(static_cast<const float*>(a.gate) + at);
-  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.gate) + at);
-  return make_uint4(w.x, w.y, 0, 0);
+    return *reinterpret_cast<const uint2*>(static_cast<const float*>(a.gate) + at);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.gate) + at), 0);
 }
-// Four gate values of the bits loaded for them (16-bit types: the first two words).
-__device__ __forceinline__ void apply_gate4(int dtype, const uint4& w, float* v) {
+__device__ __forceinline__ void apply_gate2(int dtype, const uint2& w, float* v) {
   if (dtype == DORY_DTYPE_F32) {
     v[0] *= __uint_as_float(w.x);
     v[1] *= __uint_as_float(w.y);
-    v[2] *= __uint_as_float(w.z);
-    v[3] *= __uint_as_float(w.w);
   } else if (dtype == DORY_DTYPE_BF16) {
     v[0] *= __uint_as_float(w.x << 16);
     v[1] *= __uint_as_float(w.x & 0xffff0000u);
-    v[2] *= __uint_as_float(w.y << 16);
-    v[3] *= __uint_as_float(w.y & 0xffff0000u);
   } else {
     v[0] *= __half2float(__ushort_as_half(w.x & 0xffff));
     v[1] *= __half2float(__ushort_as_half(w.x >> 16));
-    v[2] *= __half2float(__ushort_as_half(w.y & 0xffff));
-    v[3] *= __half2float(__ushort_as_half(w.y >> 16));
   }
 }
 
@@ -1119,86 +1112,97 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     int own_lane = lane, own_row = t * kM + row, col0 = share * Sh::kOutCols;
     asm volatile("" : "+r"(own_lane), "+r"(own_row), "+r"(col0));
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const bool whole = it.slot < 0;
-    // A thread holds a row's columns; memory wants a row's columns side by side in a warp.  So
-    // eight lanes exchange 16-byte pieces, 32 columns at a time: lane i then has piece i of each
-    // of its group's eight rows, and a load or store covers whole 128-byte lines.  (A row a
-    // thread instead takes 32 lines an instruction: 20,500 clocks an item with an FP32 gate.)
-    const int group = own_lane & ~7, piece = (own_lane & 7) * 4;
-    const uint32_t alive = __ballot_sync(0xffffffffu, live) >> group;
+    const bool whole = it.slot < 0, gated = whole && a.gate;
+    // O is read as product fragments: a lane has two columns of four rows, four lanes eight
+    // columns side by side, so every load of the gate and store covers whole 32-byte sectors
+    // (after neighbours have exchanged halves of their packed columns).  A row a thread takes
+    // 32 lines an instruction: 20,500 clocks an item with an FP32 gate.
+    const int quarter = own_lane & 3;
     const int where = row_head << 16 | tok;  // tok < 256
-    int64_t out_at[8], gate_at[8];
+    float row_inv[4], odd[4];                // odd: NaN once a value of the row is not finite
+    int64_t out_at[4], gate_at[4];
+    uint32_t alive = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int w = __shfl_sync(0xffffffffu, where, group + k);
+    for (int r = 0; r < 4; ++r) {  // rows 8 r + lane / 4
+      const int src = 8 * r + (own_lane >> 2);
+      const int w = __shfl_sync(0xffffffffu, where, src);
+      row_inv[r] = whole ? __shfl_sync(0xffffffffu, inv, src) : 1.0f;
+      alive |= uint32_t(__shfl_sync(0xffffffffu, int(live), src)) << r;
       const int64_t token = it.tok0 + (w & 0xffff);
-      const int64_t column = int64_t(it.kvh * a.G + (w >> 16)) * HD + col0 + piece;
-      out_at[k] = whole ? token * a.out_t + column
-                        : (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + group + k) * HD +
-                              col0 + piece;
-      gate_at[k] = token * a.gate_t + column;
+      const int64_t column = int64_t(it.kvh * a.G + (w >> 16)) * HD + col0;
+      out_at[r] = whole ? token * a.out_t + column
+                        : (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + src) * HD + col0;
+      gate_at[r] = token * a.gate_t + column + 2 * quarter;
+      odd[r] = 0.0f;
     }
-    float odd = 0.0f;  // NaN once a value is not finite
-    uint4 g[8];  // the gate's bits, for the 32 columns to come
-    const bool gated = whole && a.gate;
+    uint2 g[4][4];  // the gate's bits, asked for a piece ahead
     auto ask_gate = [&](int x) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (alive >> k & 1) g[k] = load_gate4(a, gate_at[k] + x);
-    };
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] = make_uint4(0, 0, 0, 0);  // or they live from the start on
-    if (gated) ask_gate(0);
+        for (int i = 0; i < 4; ++i) {
+          g[r][i] = make_uint2(0, 0);  // defined on every path, or it lives from the start on
+          if (gated && (alive >> r & 1)) g[r][i] = load_gate2(a, gate_at[r] + x + 8 * i);
+        }
+    };
+    ask_gate(0);
 #pragma unroll 1
     for (int x = 0; x < Sh::kOutCols; x += 32) {
-      float o[32];
+      float o[32];  // row r's columns 8 i + 2 quarter + y at 16 (r / 2) + 4 i + 2 (r % 2) + y
 #pragma unroll
       for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-      if (e > b) tmem_ld32(o_addr + x, reinterpret_cast<uint32_t*>(o));
+      if (e > b) {
+        tmem_ld_fragment(o_addr + x, reinterpret_cast<uint32_t*>(o));
+        tmem_ld_fragment(o_addr + (16u << 16) + x, reinterpret_cast<uint32_t*>(o + 16));
+      }
       tmem_wait_ld32(reinterpret_cast<uint32_t*>(o));
 #pragma unroll
-      for (int y = 0; y < 32; ++y) odd = fmaf(o[y], 0.0f, odd);
-      if (whole) {
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] *= inv;
-      }
+        for (int i = 0; i < 4; ++i) {
+          float* v = o + 16 * (r / 2) + 4 * i + 2 * (r % 2);
+          odd[r] = fmaf(v[0], 0.0f, fmaf(v[1], 0.0f, odd[r]));
+          v[0] *= row_inv[r];
+          v[1] *= row_inv[r];
+          if (gated) apply_gate2(a.gate_dtype, g[r][i], v);
+        }
+      if (x + 32 < Sh::kOutCols) ask_gate(x + 32);
 #pragma unroll
-      for (int step = 1; step < 8; step <<= 1) {
-        const bool upper = own_lane & step;
+      for (int r = 0; r < 4; ++r) {
+        uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k & step) continue;
+        for (int i = 0; i < 4; ++i) {
+          const float* v = o + 16 * (r / 2) + 4 * i + 2 * (r % 2);
+          w[i] = pack_bf16(v[0], v[1]);
+          if (!whole && (alive >> r & 1))
+            *reinterpret_cast<float2*>(a.part_o + out_at[r] + x + 8 * i + 2 * quarter) =
+                make_float2(v[0], v[1]);
+        }
+        if (whole) {
+          const bool second = quarter & 1;  // of two neighbours: takes the odd eights
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            float& low = o[4 * k + y];
-            float& high = o[4 * (k | step) + y];
-            const float got = __shfl_xor_sync(0xffffffffu, upper ? low : high, step);
-            low = upper ? got : low;
-            high = upper ? high : got;
+          for (int i = 0; i < 4; i += 2) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? w[i] : w[i + 1], 1);
+            if (alive >> r & 1)
+              *reinterpret_cast<uint2*>(a.out + out_at[r] + x + 8 * (i + second) + 4 * (quarter >> 1)) =
+                  second ? make_uint2(got, w[i + 1]) : make_uint2(w[i], got);
           }
         }
       }
-      if (gated) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) apply_gate4(a.gate_dtype, g[k], o + 4 * k);
-        if (x + 32 < Sh::kOutCols) ask_gate(x + 32);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (!(alive >> k & 1)) continue;
-        const float* v = o + 4 * k;
-        if (whole)
-          *reinterpret_cast<uint2*>(a.out + out_at[k] + x) =
-              make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-        else
-          *reinterpret_cast<float4*>(a.part_o + out_at[k] + x) = make_float4(v[0], v[1], v[2], v[3]);
-      }
-      __syncwarp();
     }
+    __syncwarp();
     const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
     if (live && !whole && share == 0)
       a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl, l);
-    uint32_t again = __ballot_sync(0xffffffffu, live && isnan(odd) && isfinite(l));
+    uint32_t again = 0;  // rows, as lanes
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t lanes = __ballot_sync(0xffffffffu, isnan(odd[r]));
+      if (lanes)
+        for (int y = 0; y < 8; ++y)
+          if (lanes >> (4 * y) & 15) again |= 1u << (8 * r + y);
+    }
+    again &= __ballot_sync(0xffffffffu, live && isfinite(l));
     while (again) {
       const int src = __ffs(again) - 1;
       again &= again - 1;
@@ -1285,11 +1289,29 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
   if (warp == Sh::kMmaWarp) tmem_free(c.tmem, 512);
 }
 
+template <int N>
+__device__ __forceinline__ void load_row(const float* p, float* v) {
+  if constexpr (N == 2) {
+    const float2 w = *reinterpret_cast<const float2*>(p);
+    v[0] = w.x;
+    v[1] = w.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 w = *reinterpret_cast<const float4*>(p + i);
+      v[i] = w.x;
+      v[i + 1] = w.y;
+      v[i + 2] = w.z;
+      v[i + 3] = w.w;
+    }
+  }
+}
+
 // Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
 // starts at the end of CTA c's piece, a warp a row.
 constexpr int kJoinSlices = 8;
 template <int HD>
-__global__ void __launch_bounds__(256) join_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
   using Sh = Shape<HD>;
   constexpr int kPer = HD / 32;  // columns of a lane
   grid_wait();
@@ -1297,42 +1319,36 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkArgs a) {
   const int parts = join[0], tok0 = join[1], ntok = join[2], kvh = join[3];
   if (!parts) return;
   const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 8 * kJoinSlices) {
+  for (int r = blockIdx.y * 16 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 16 * kJoinSlices) {
     const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
     const int tok = t * a.TB + row_tok;
     if (in_tile >= a.TB * a.G || tok >= ntok) continue;
     auto slot = [&](int i) {
       return int64_t(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * Sh::kItemRows + r;
     };
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 ml = a.part_ml[slot(i)];
-      if (ml.y != 0.0f) m = fmaxf(m, ml.x);
-    }
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-    float l = 0.0f, acc[kPer];
+    float m = -INFINITY, l = 0.0f, acc[kPer];
 #pragma unroll
     for (int x = 0; x < kPer; ++x) acc[x] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float2 ml = a.part_ml[slot(i)];
-      if (ml.y == 0.0f) continue;  // saw nothing
-      const float w = exp2_approx(ml.x - m);
-      const float* o = a.part_o + slot(i) * HD + lane * kPer;
-      l += w * ml.y;
-      if constexpr (kPer == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(o);
-        acc[0] += w * v.x;
-        acc[1] += w * v.y;
-      } else {
+    for (int i = 0; i < parts; i += 4) {  // four parts on their way at once
+      float2 ml[4];
+      float o[4][kPer];
 #pragma unroll
-        for (int x = 0; x < kPer; x += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(o + x);
-          acc[x] += w * v.x;
-          acc[x + 1] += w * v.y;
-          acc[x + 2] += w * v.z;
-          acc[x + 3] += w * v.w;
+      for (int y = 0; y < 4; ++y) {
+        ml[y] = make_float2(0.0f, 0.0f);
+        if (i + y < parts) {
+          ml[y] = a.part_ml[slot(i + y)];
+          load_row<kPer>(a.part_o + slot(i + y) * HD + lane * kPer, o[y]);
         }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (ml[y].y == 0.0f) continue;  // not there, or saw nothing
+        const float top = max2(m, ml[y].x);
+        const float keep = exp2_approx(m - top), w = exp2_approx(ml[y].x - top);
+        m = top;
+        l = l * keep + w * ml[y].y;
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) acc[x] = acc[x] * keep + w * o[y][x];
       }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1429,7 +1445,7 @@ int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaS
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(ctas, kJoinSlices);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(512);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1538,6 +1554,11 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   const int64_t span = int64_t(p.max_blocks) * p.block_size;
   a.table_span = span < kMaxPosition ? int(span) : kMaxPosition;
   a.min_units = 1;
+  // The device counts units in 32 bits.
+  const int64_t most = (int64_t(p.num_tokens) / (a.TB * (p.head_dim == 256 ? 1 : 2)) + p.num_seqs + 1) *
+                       (a.table_span / kN + 2 + kItemUnits);
+  if (most > (int64_t(1) << 30) / p.num_kv_heads)
+    return fail(DORY_ERR_UNSUPPORTED, "more work than one call counts (tokens x positions)");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (kv8) {
     const dim3 grid(p.num_tokens, (p.num_heads + 3) / 4);

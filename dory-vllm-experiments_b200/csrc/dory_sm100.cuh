@@ -91,6 +91,18 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+// 32 columns of 16 of this warp's lanes (the first, or with 16 added to the address's lane the
+// last) as a product fragment: r[4 i + 2 u + y] is row 8 u + lane / 4, column 8 i + 2 (lane % 4) + y.
+__device__ __forceinline__ void tmem_ld_fragment(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 // Every load of this thread is complete; what reads these registers depends on it.  `more`:
 // another load's registers, ordered behind a wait already made.
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
