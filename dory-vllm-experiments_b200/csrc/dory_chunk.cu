@@ -18,6 +18,7 @@
 //   loader     tensor copies: the queries, and K and V tiles page by page through the block
 //              table into a ring; pages outside the item's positions, and bad block ids, load
 //              as zeros without touching memory;
+//   conversion (FP8 caches, four warps) e4m3 tiles to f16 tiles, bf16 queries to scaled f16 ones;
 //   products   tcgen05: S = Q K^T into tensor memory, O += P V with P read from there;
 //   softmax    four warpgroups, a half (256-dim heads: a quarter) of a row per thread: scores to
 //              registers, running maximum, exponentials, P back to tensor memory as 16-bit
@@ -98,10 +99,14 @@ __device__ __forceinline__ float load_gate(const ChunkArgs& a, int64_t i) {
   return __half2float(static_cast<const __half*>(a.gate)[i]);
 }
 
+// Two e4m3 values, the low byte the lower one, in f16: exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two_bytes)));
+  return r;
+}
 __device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(b)));
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(e4m3x2_to_f16x2(b))));
 }
 template <bool KV8>
 __device__ __forceinline__ float cache_value(const void* p, int64_t i) {
@@ -126,87 +131,22 @@ __device__ __forceinline__ int64_t block_of(const ChunkArgs& a, const int32_t* t
   return id;
 }
 
-template <int HD, bool KV8>
-__global__ void __launch_bounds__(128) chunk_rows(const ChunkArgs a) {
-  __shared__ float sq[4][HD];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x, h = blockIdx.y * 4 + warp;
-  if (h >= a.NH) return;
-  // the row's sequence: the last one that starts at or before it and is not empty
-  int seq = -1, t0 = 0, t1 = 0;
-  for (int i = 0; i < a.S; ++i) {
-    int u0, u1;
-    rows_of(a, i, u0, u1);
-    if (u0 <= t && t < u1) {
-      seq = i;
-      t0 = u0;
-      t1 = u1;
-      break;
-    }
-  }
-  if (seq < 0) return;
-  for (int i = lane; i < HD; i += 32)
-    sq[warp][i] = __bfloat162float(a.q[t * a.q_t + h * a.q_h + i]);
-  __syncwarp();
-  const int p = a.seq_lens[seq] - (t1 - t0) + (t - t0);
-  const int lo = a.window ? max(0, p + 1 - a.window) : 0;
-  const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
-  const int64_t head = int64_t(h / a.G) * a.sh;
-  float m = -INFINITY, l = 0.0f, acc[HD / 32];
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
-  const float qk = a.scale_log2 * (KV8 ? a.k_scale : 1.0f);
-  for (int c0 = lo; c0 <= p; c0 += 32) {
-    const int c = c0 + lane;
-    float s = -INFINITY;
-    int64_t at = -1;
-    if (c <= p) {
-      const int64_t id = block_of(a, table, c);
-      if (id >= 0) {
-        at = id * a.sb + int64_t(c % a.B) * a.so + head;
-        float dot = 0.0f;
-        for (int i = 0; i < HD; ++i) dot += sq[warp][i] * cache_value<KV8>(a.kc, at + i);
-        s = dot * qk;
-      }
-    }
-    float top = s;
-    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
-    const float w = exp2f(s - base), shrink = exp2f(m - base);
-    m = m_new;
-    l = l * shrink + w;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] *= shrink;
-    for (int k = 0; k < 32; ++k) {
-      const int64_t row = __shfl_sync(0xffffffffu, at, k);
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      if (row < 0) continue;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) acc[i] += wk * cache_value<KV8>(a.vc, row + lane + 32 * i);
-    }
-  }
-  for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-  const float inv = l > 0.0f ? (KV8 ? a.v_scale : 1.0f) / l : (l == 0.0f ? 0.0f : l);
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    const int e = h * HD + lane + 32 * i;
-    float y = acc[i] * inv;
-    if (a.gate) y *= load_gate(a, t * a.gate_t + e);
-    a.out[t * a.out_t + e] = __float2bfloat16_rn(y);
-  }
-}
-
 // ------------------------------------------------------------------------------------
 // The tensor-core kernel
 // ------------------------------------------------------------------------------------
 constexpr int kWide128 = 1, kWide256 = 2;
-template <int HD>
+template <int HD, bool KV8>
 struct Shape {
   static constexpr int kTiles = HD == 256 ? 1 : 2;           // tensor-core tiles of an item
   static constexpr int kCols = HD < 128 ? HD : 128;          // columns of a ring stage
   static constexpr int kHalves = HD / kCols;                 // stages of a K (or V) tile
   static constexpr int kStageBytes = kCols / 64 * kChunkBytes;
-  static constexpr int kStages = HD == 64 ? 8 : 5;
+  static constexpr int kStages = HD == 64 ? 8 : KV8 ? 3 : 5;
+  // FP8 caches: tiles of bytes as they were copied, 128 dims a row, before their conversion
+  static constexpr int kRawStages = KV8 ? 4 : 0, kRawBytes = kChunkBytes;
+  static constexpr int kConvertWarps = KV8 ? 4 : 0;
+  static constexpr int kTileBytes = kTiles * HD / 64 * kChunkBytes + kStages * kStageBytes +
+                                    kRawStages * kRawBytes;
   static constexpr int kQBytes = kTiles * HD / 64 * kChunkBytes;
   static constexpr int kShares = HD == 256 ? kWide256 : kWide128;  // softmax warpgroups of a tile
   static constexpr int kScoreCols = kN / kShares;            // of a row, per softmax thread
@@ -214,9 +154,14 @@ struct Shape {
   static constexpr int kParts = kScoreCols > 32 ? 2 : 1;     // the weights are handed over in
   static constexpr int kPartCols = kScoreCols / kParts;
   static constexpr int kSoftmaxWarps = 4 * kShares * kTiles;
-  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;  // the last: plan
-  static constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
+  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1,
+                       kPlanWarp = kSoftmaxWarps + 2;
+  [[maybe_unused]] static constexpr int kConvert = kSoftmaxWarps + 3;  // the first of these
+  static constexpr int kThreads = (kSoftmaxWarps + 3 + kConvertWarps) * 32;
   static constexpr int kItemRows = kTiles * kM;
+  // f16 weights are lifted by 2^7, to below 2^15 (kSlack), so that they are exact to 11 bits down
+  // to 2^-21 of the row's largest and end at 2^-32 of it
+  static constexpr float kLift = KV8 ? 7.0f : 0.0f;
   // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
   static constexpr int kO = 2 * kN;
   static constexpr int kOStride = HD <= 128 ? 128 : 0;       // between the tiles' O
@@ -234,16 +179,18 @@ struct Item {
   int pad[6];
 };
 
-template <int HD>
+template <int HD, bool KV8>
 struct Control {  // shared memory behind the tiles
-  alignas(8) uint64_t kv_full[Shape<HD>::kStages], kv_empty[Shape<HD>::kStages];
+  alignas(8) uint64_t kv_full[Shape<HD, KV8>::kStages], kv_empty[Shape<HD, KV8>::kStages];
+  uint64_t raw_full[4], raw_empty[4], q_raw;  // FP8 caches only
   uint64_t q_full, q_empty, s_full[2], p_full[2][2], o_full[2], item_full[kQueue],
       item_empty[kQueue], drained;
   Item items[kQueue];
   uint32_t bad[kBadRing];
+  float q_scale[KV8 ? Shape<HD, KV8>::kItemRows : 1];  // what a row's f16 query was divided by
   uint32_t tmem;
   int abort;
-  float swap[Shape<HD>::kTiles][Shape<HD>::kShares][kM];  // a row's maxima and sums, by share
+  float swap[Shape<HD, KV8>::kTiles][Shape<HD, KV8>::kShares][kM];  // a row's maxima and sums, by share
 };
 
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
@@ -280,7 +227,7 @@ __device__ __forceinline__ int tiles_seen(int p0, int n, int cap, int window, in
   return (hi + kN - 1) / kN - first;
 }
 // Those of tile t of an item within this CTA's piece: [b, e).
-template <int HD>
+template <int HD, bool KV8>
 __device__ __forceinline__ void tile_range(const ChunkArgs& a, const Item& it, int t, int& b, int& e) {
   const int skip = t * a.TB;
   const int n = tiles_seen(it.pos0 + skip, min(it.ntok - skip, a.TB), it.cap, a.window, b);
@@ -346,9 +293,9 @@ __device__ __forceinline__ int scan_add(int x, int lane) {  // inclusive
   return x;
 }
 
-template <int HD>
-__device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
-  const int tokens = Shape<HD>::kTiles * a.TB, cta = blockIdx.x;
+template <int HD, bool KV8>
+__device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
+  const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
   int32_t* join = a.joins + cta * 8;
   int queued = 0;
   auto push = [&](const Item& it) {
@@ -464,9 +411,9 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD>& c, int lane) {
 // What ring stage q of an item's n tiles holds.  Stages are used in the order K0 V0 K1 V1 ..;
 // with 256-dim heads (two stages a tile, and K of the next tile wanted before V of this one)
 // K0 K1 V0 K2 V1 .. Vn-1.
-template <int HD>
+template <int HD, bool KV8>
 __device__ __forceinline__ void stage_holds(int q, int n, bool& is_v, int& tile, int& half) {
-  if (Shape<HD>::kTiles == 2) {
+  if (Shape<HD, KV8>::kTiles == 2) {
     is_v = q & 1;
     tile = q >> 1;
     half = 0;
@@ -478,17 +425,23 @@ __device__ __forceinline__ void stage_holds(int q, int n, bool& is_v, int& tile,
   tile = r < 0 ? 0 : is_v ? step : step + 1;
 }
 // The first stage of V of tile i.
-template <int HD>
+template <int HD, bool KV8>
 __device__ __forceinline__ uint32_t stage_of_v(int i, int n) {
-  if (Shape<HD>::kTiles == 2) return 2 * i + 1;
+  if (Shape<HD, KV8>::kTiles == 2) return 2 * i + 1;
   return i + 1 < n ? 4 * i + 4 : 4 * i + 2;
 }
 
-template <int HD>
-__device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, uint32_t tiles,
+template <int HD, bool KV8>
+__device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>& c, uint32_t tiles,
                           int lane) {
-  using Sh = Shape<HD>;
-  const uint32_t stages = tiles + Sh::kQBytes;
+  using Sh = Shape<HD, KV8>;
+  // the ring the copies go to: the products' own, or the bytes' that wait for conversion
+  constexpr int kRing = KV8 ? Sh::kRawStages : Sh::kStages;
+  constexpr int kBytes = KV8 ? Sh::kRawBytes : Sh::kStageBytes;
+  constexpr int kBoxes = KV8 ? 1 : Sh::kCols / 64;  // 128-byte boxes across a row
+  const uint32_t stages = tiles + Sh::kQBytes + (KV8 ? Sh::kStages * Sh::kStageBytes : 0);
+  uint64_t* const full = KV8 ? c.raw_full : c.kv_full;
+  uint64_t* const empty = KV8 ? c.raw_empty : c.kv_empty;
   const int copies = kN / a.copy_rows;
   int stage = 0, queued = 0, q_uses = 0;
   uint32_t phase = 1, tile_no = 0, issued = 0;  // phase of the stage's empty barrier: free at first
@@ -510,7 +463,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     auto look_up = [&](int q, bool& bad) {
       bool is_v;
       int tile, half;
-      stage_holds<HD>(q, kvn, is_v, tile, half);
+      stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
       const int pos = (kv0 + tile) * kN + lane * a.copy_rows;
       int id = int(a.blocks);
       bad = false;
@@ -529,7 +482,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     const int tok0 = uniform(it.tok0);
     const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
     if (elect_one()) {
-      const uint32_t bar = smem_u32(&c.q_full);
+      const uint32_t bar = smem_u32(KV8 ? &c.q_raw : &c.q_full);
       mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
 #pragma unroll 1
       for (int t = 0; t < filled; ++t)
@@ -543,7 +496,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
     for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
       bool is_v;
       int tile, half;
-      stage_holds<HD>(q, kvn, is_v, tile, half);
+      stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
       if (!is_v && half == 0) {
         const uint32_t mask = __ballot_sync(0xffffffffu, bad);
         if (elect_one()) {
@@ -555,9 +508,9 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
       }
       const int own = id;
       id = look_up(q + 1, bad);  // in flight while this stage's copies are issued
-      if (!(ok = wait_warp(c.kv_empty[stage], phase, &c.abort, a.err))) break;
-      const uint32_t bar = smem_u32(&c.kv_full[stage]);
-      const uint32_t dst = stages + stage * Sh::kStageBytes;
+      if (!(ok = wait_warp(empty[stage], phase, &c.abort, a.err))) break;
+      const uint32_t bar = smem_u32(&full[stage]);
+      const uint32_t dst = stages + stage * kBytes;
       const CUtensorMap* map = is_v ? &maps.v : &maps.k;
       // Every copy's block in registers first, then one elected run of copies: 28 clocks a copy
       // of 2 KB; a loop that fetches each block as it goes took 47, a copy a lane 66.
@@ -573,19 +526,19 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
           row[x] = ((kv0 + tile) * kN + x * a.copy_rows) % a.B;
       }
       if (elect_one()) {
-        mbar_expect(bar, Sh::kStageBytes);
+        mbar_expect(bar, kBytes);
 #pragma unroll
         for (int x = 0; x < kN / 16; ++x) {
           if (x < copies)
 #pragma unroll
-            for (int k = 0; k < Sh::kCols / 64; ++k)
+            for (int k = 0; k < kBoxes; ++k)
               tma_load_4d(dst + k * kChunkBytes + x * a.copy_rows * 128, map,
                           half * Sh::kCols + 64 * k, row[x], kvh, block[x], bar);
         }
       }
       __syncwarp();
       ++issued;
-      if (++stage == Sh::kStages) {
+      if (++stage == kRing) {
         stage = 0;
         phase ^= 1;
       }
@@ -595,31 +548,142 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD>& c, 
   if (!ok) {  // given up: no copy may land after the CTA has gone
     const long long start = clock64();
 #pragma unroll 1
-    for (uint32_t i = issued > Sh::kStages ? issued - Sh::kStages : 0; i < issued; ++i)
-      while (!mbar_try(smem_u32(&c.kv_full[i % Sh::kStages]), (i / Sh::kStages) & 1) &&
+    for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; ++i)
+      while (!mbar_try(smem_u32(&full[i % kRing]), (i / kRing) & 1) &&
              clock64() - start < 200000000LL) {
       }
-    while (q_uses && !mbar_try(smem_u32(&c.q_full), (q_uses - 1) & 1) &&
+    while (q_uses && !mbar_try(smem_u32(KV8 ? &c.q_raw : &c.q_full), (q_uses - 1) & 1) &&
            clock64() - start < 300000000LL) {
+    }
+  }
+}
+
+// ---- conversion, FP8 caches: four warps ----
+// e4m3 is exact in f16, so K and V tiles become f16 tiles.  A query row becomes f16 after a
+// scaling by a power of two that puts its largest element in [2^10, 2^11): bf16's 8 bits fit
+// f16's 11, and only what lies 2^24 below the row's largest element loses any.  Both together
+// let the scores and the sum be f16 products, the weights rounded to 11 bits.
+template <int HD, bool KV8>
+__device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tiles, int thread) {
+  using Sh = Shape<HD, KV8>;
+  const int lane = thread & 31;
+  const uint32_t stages = tiles + Sh::kQBytes, raws = stages + Sh::kStages * Sh::kStageBytes;
+  int queued = 0, raw = 0, stage = 0;
+  uint32_t raw_phase = 0, phase = 1, q_phase = 0;
+  for (;;) {
+    const int at = queued % kQueue;
+    if (!wait_warp(c.item_full[at], (queued / kQueue) & 1, &c.abort, a.err)) return;
+    const Item it = c.items[at];
+    const int kvn = it.kvn;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c.item_empty[at]));
+    ++queued;
+    if (it.flags & kItemEnd) return;
+    if (!kvn) continue;
+    const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
+    const int hi = min(it.pos0 + it.ntok, it.cap);
+    if (!wait_warp(c.q_raw, q_phase, &c.abort, a.err)) return;
+    q_phase ^= 1;
+#pragma unroll 1
+    for (int t = 0; t < Sh::kTiles; ++t) {  // a row a thread, in place
+      const uint32_t row = tiles + t * (HD / 64) * kChunkBytes + thread * 128;
+      float top = 0.0f;
+#pragma unroll 1
+      for (int x = 0; x < HD / 8; ++x) {
+        uint32_t w[4];
+        lds128(row + x / 8 * kChunkBytes + ((x ^ thread) & 7) * 16, w);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[y] << 16)),
+                                 fabsf(__uint_as_float(w[y] & 0xffff0000u))));
+      }
+      // 2^(10 - exponent), within what FP32 holds; 1 for zero, infinite and NaN rows
+      const int exponent = int(__float_as_uint(top) >> 23) - 127;
+      const int up = top > 0.0f && exponent < 128 ? min(10 - exponent, 126) : 0;
+      const float scale = __uint_as_float(uint32_t(up + 127) << 23);
+#pragma unroll 1
+      for (int x = 0; x < HD / 8; ++x) {
+        uint32_t w[4];
+        const uint32_t piece = row + x / 8 * kChunkBytes + ((x ^ thread) & 7) * 16;
+        lds128(piece, w);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          w[y] = pack_f16(__uint_as_float(w[y] << 16) * scale,
+                          __uint_as_float(w[y] & 0xffff0000u) * scale);
+        sts128(piece, w);
+      }
+      c.q_scale[t * kM + thread] = __uint_as_float(uint32_t(127 - up) << 23);
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c.q_full));
+#pragma unroll 1
+    for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
+      if (!wait_warp(c.raw_full[raw], raw_phase, &c.abort, a.err)) return;
+      if (!wait_warp(c.kv_empty[stage], phase, &c.abort, a.err)) return;
+      const uint32_t from = raws + raw * Sh::kRawBytes, to = stages + stage * Sh::kStageBytes;
+      bool is_v;
+      int tile, half;
+      stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
+      const int seen_lo = lo - (it.kv0 + tile) * kN, seen_hi = hi - (it.kv0 + tile) * kN;
+      // 16 dims at a time: one 16-byte piece of bytes, two of f16.  Eight lanes take a row; the
+      // upper four write their second piece first, so that no two lanes share a bank.
+#pragma unroll 2
+      for (int x = thread; x < kN * 8; x += 128) {
+        const int row = x >> 3, piece = x & 7;
+        uint32_t w[4], f[8];
+        lds128(from + row * 128 + ((piece ^ row) & 7) * 16, w);
+        const bool seen = row >= seen_lo && row < seen_hi;  // by some row of the item
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          f[2 * y] = seen ? e4m3x2_to_f16x2(w[y]) : 0;
+          f[2 * y + 1] = seen ? e4m3x2_to_f16x2(w[y] >> 16) : 0;
+        }
+        const uint32_t chunk = to + (piece >> 2) * kChunkBytes + row * 128;
+        const int first = (piece & 3) * 2;
+        const bool upper = piece & 4;
+        uint32_t early[4], late[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          early[y] = upper ? f[4 + y] : f[y];
+          late[y] = upper ? f[y] : f[4 + y];
+        }
+        sts128(chunk + ((first + upper) ^ (row & 7)) * 16, early);
+        sts128(chunk + ((first + !upper) ^ (row & 7)) * 16, late);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&c.kv_full[stage]));
+        mbar_arrive(smem_u32(&c.raw_empty[raw]));
+      }
+      if (++raw == Sh::kRawStages) {
+        raw = 0;
+        raw_phase ^= 1;
+      }
+      if (++stage == Sh::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
   }
 }
 
 // Column, within a score buffer, of the weights of positions [16 x, 16 x + 16): each warpgroup
 // puts its own over the scores it has read.
-template <int HD>
+template <int HD, bool KV8>
 __host__ __device__ constexpr int weight_column(int x) {
-  constexpr int kSteps = Shape<HD>::kScoreCols / 16;
-  return x / kSteps * Shape<HD>::kScoreCols + x % kSteps * 8;
+  constexpr int kSteps = Shape<HD, KV8>::kScoreCols / 16;
+  return x / kSteps * Shape<HD, KV8>::kScoreCols + x % kSteps * 8;
 }
 
 // ---- products ----
-template <int HD>
-__device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
-  using Sh = Shape<HD>;
+template <int HD, bool KV8>
+__device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tiles) {
+  using Sh = Shape<HD, KV8>;
   const uint32_t tmem = uniform(c.tmem), stages = tiles + Sh::kQBytes;
-  constexpr uint32_t kScores = instruction(true, false, kM, kN);
-  constexpr uint32_t kSum = instruction(true, true, kM, Sh::kCols);
+  constexpr uint32_t kScores = instruction(!KV8, false, kM, kN);
+  constexpr uint32_t kSum = instruction(!KV8, true, kM, Sh::kCols);
   int stage = 0, queued = 0;
   uint32_t phase = 0, q_phase = 0, p_phase = 0, p_count = 0, buffers = 0;
 #define WAIT(bar, parity) \
@@ -658,7 +722,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
 #pragma unroll
       for (int i = 0; i < kSteps * Sh::kShares; ++i) {
         const int x = i / kSteps * (Sh::kScoreCols / 16) + i % kSteps;  // in part 0
-        mma_ts(tmem + o_col, weights + weight_column<HD>(x), v_desc + (x * 16 * 128 >> 4), kSum,
+        mma_ts(tmem + o_col, weights + weight_column<HD, KV8>(x), v_desc + (x * 16 * 128 >> 4), kSum,
                add || part + i > 0);
       }
     }
@@ -683,8 +747,8 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD>& c, uint32_t tiles) {
     q_phase ^= 1;
     if constexpr (Sh::kTiles == 2) {
       int b0, b1, e0, e1;
-      tile_range<HD>(a, it, 0, b0, e0);
-      tile_range<HD>(a, it, 1, b1, e1);
+      tile_range<HD, KV8>(a, it, 0, b0, e0);
+      tile_range<HD, KV8>(a, it, 1, b1, e1);
       b0 = uniform(b0);
       b1 = uniform(b1);
       e0 = uniform(e0);
@@ -882,9 +946,9 @@ __device__ __forceinline__ uint32_t bad_columns(uint32_t bad, int col, int copy_
          (bad >> ((col + 16) >> copy_shift) & 1 ? 0xffff0000u : 0u);
 }
 
-template <int HD>
-__device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles, int warp, int lane) {
-  using Sh = Shape<HD>;
+template <int HD, bool KV8>
+__device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tiles, int warp, int lane) {
+  using Sh = Shape<HD, KV8>;
   constexpr bool kTwo = Sh::kTiles == 2;
   const int quad = warp & 3, row = quad * 32 + lane;
   const int t = (warp >> 2) / Sh::kShares, share = (warp >> 2) % Sh::kShares;
@@ -895,7 +959,6 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
   const uint32_t stages = tiles + Sh::kQBytes;
   const int row_tok = row / a.G, row_head = row - row_tok * a.G;
   const bool row_real = row < a.TB * a.G;
-  const float sl = a.scale_log2, slack = kSlack / a.scale_log2;
   int queued = 0;
   uint32_t scored = 0, summed = 0, tiles_seen_before = 0, stage_no = 0;
   // The last sum given to the tensor cores is complete.  A parity can only be asked for with one
@@ -913,7 +976,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     const Item& it = c.items[at];
     if (it.flags & kItemEnd) return;
     int b, e;
-    tile_range<HD>(a, it, t, b, e);
+    tile_range<HD, KV8>(a, it, t, b, e);
     const int tok = t * a.TB + row_tok;
     const bool live = row_real && tok < it.ntok;
     const bool warp_live = __any_sync(0xffffffffu, live);
@@ -927,6 +990,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       for (int x = 0; x < Sh::kOutCols * size; x += 128)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(at_gate + x));
     }
+    float sl = a.scale_log2, slack = kSlack / a.scale_log2;
     float m = -INFINITY, l = 0.0f;
     for (int j = b; j < e; ++j) {
       const int buffer = kTwo ? t : int(scored & 1);
@@ -934,6 +998,10 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       if (!wait_warp(c.s_full[buffer], kTwo ? scored & 1 : (scored >> 1) & 1, &c.abort, a.err))
         return;
       tc_fence_after();
+      if (KV8 && j == b && live) {  // there since the first scores: they needed the queries
+        sl = a.scale_log2 * a.k_scale * c.q_scale[t * kM + row];
+        slack = kSlack / sl;
+      }
       const uint32_t bad = c.bad[(tiles_seen_before + (j - it.kv0)) % kBadRing];
       // 256-dim heads: a warp may already be a tile ahead of another, so a barrier a buffer
       auto ready = [&](int part) {
@@ -944,9 +1012,9 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       // V rows of this tile that no row of the item sees, in copies that hold others it does
       const int z_lo = (a.window ? max(0, it.pos0 - a.window + 1) : 0) - j * kN;
       const int z_hi = min(it.pos0 + it.ntok, it.cap) - j * kN;
-      if (z_lo > 0 || z_hi < kN) {
+      if (!KV8 && (z_lo > 0 || z_hi < kN)) {  // (the conversion sees to it)
         const int i = j - it.kv0;  // the tile's place in the piece, and so its V stages
-        const uint32_t v_no = stage_no + stage_of_v<HD>(i, it.kvn);
+        const uint32_t v_no = stage_no + stage_of_v<HD, KV8>(i, it.kvn);
         const int r1 = z_lo > 0 ? (z_lo & ~(a.copy_rows - 1)) : 0, r2 = max(z_lo, 0);
         const int r3 = min(z_hi, kN), r4 = (r3 + a.copy_rows - 1) & ~(a.copy_rows - 1);
         for (int h = 0; h < Sh::kHalves; ++h) {
@@ -991,7 +1059,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           }
         };
         float mt = -INFINITY;
-        if (!edge) {
+        if (!KV8 && !edge) {  // FP8: fewer registers a thread
           float s[Sh::kScoreCols], top[4];
 #pragma unroll
           for (int x = 0; x < Sh::kScoreCols; x += 32)
@@ -1045,7 +1113,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
           tmem_wait_st();
         }
         // +inf gives NaN, as inf - inf would in every weight
-        const float ref = m == -INFINITY ? 0.0f : fmaf(m, sl, m - m);
+        const float ref = m == -INFINITY ? 0.0f : fmaf(m, sl, m - m) - Sh::kLift;
         const uint64_t sl2 = pair(sl, sl), ref2 = pair(-ref, -ref);
         uint64_t sums[2] = {0, 0};
         // The scores are read again, a piece at a time: a loop, not 128 unrolled columns, because
@@ -1063,7 +1131,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
             p0 = exp2_approx(p0);
             p1 = exp2_approx(p1);
             sums[y / 2 & 1] = add2(sums[y / 2 & 1], pair(p0, p1));
-            p[y / 2] = pack_bf16(p0, p1);
+            p[y / 2] = KV8 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
           }
           tmem_st16(own_scores + x / 2, p);
           if (Sh::kParts > 1 && x + 32 == Sh::kPartCols) {
@@ -1111,7 +1179,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     // ahead of the items, and spills it across the loop over the tiles.
     int own_lane = lane, own_row = t * kM + row, col0 = share * Sh::kOutCols;
     asm volatile("" : "+r"(own_lane), "+r"(own_row), "+r"(col0));
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;
     const bool whole = it.slot < 0, gated = whole && a.gate;
     // O is read as product fragments: a lane has two columns of four rows, four lanes eight
     // columns side by side, so every load of the gate and store covers whole 32-byte sectors
@@ -1193,7 +1261,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
     __syncwarp();
     const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
     if (live && !whole && share == 0)
-      a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl, l);
+      a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl - Sh::kLift, l);
     uint32_t again = 0;  // rows, as lanes
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1218,28 +1286,33 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD>& c, uint32_t tiles,
       r.part_o = a.part_o + r_slot * HD + col0;
       r.part_ml = !whole && share == 0 ? a.part_ml + r_slot : nullptr;
       __syncwarp();
-      redo_row<HD, false>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
+      redo_row<HD, KV8>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
       __syncwarp();
     }
     done();
   }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
+template <int HD, bool KV8>
+__global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
     chunk_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ Maps maps) {
-  using Sh = Shape<HD>;
+  using Sh = Shape<HD, KV8>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Control<HD>& c = *reinterpret_cast<Control<HD>*>(smem + Sh::kQBytes + Sh::kStages * Sh::kStageBytes);
+  Control<HD, KV8>& c = *reinterpret_cast<Control<HD, KV8>*>(smem + Sh::kTileBytes);
   const uint32_t tiles = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < Sh::kStages; ++i) {
-      mbar_init(smem_u32(&c.kv_full[i]), 1);
+      mbar_init(smem_u32(&c.kv_full[i]), KV8 ? Sh::kConvertWarps : 1);
       mbar_init(smem_u32(&c.kv_empty[i]), 1);
     }
-    mbar_init(smem_u32(&c.q_full), 1);
+    for (int i = 0; i < Sh::kRawStages; ++i) {
+      mbar_init(smem_u32(&c.raw_full[i]), 1);
+      mbar_init(smem_u32(&c.raw_empty[i]), Sh::kConvertWarps);
+    }
+    mbar_init(smem_u32(&c.q_raw), 1);
+    mbar_init(smem_u32(&c.q_full), KV8 ? Sh::kConvertWarps : 1);
     mbar_init(smem_u32(&c.q_empty), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&c.s_full[i]), 1);
@@ -1249,7 +1322,7 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + 2);
+      mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + 2 + Sh::kConvertWarps);
     }
     mbar_init(smem_u32(&c.drained), 1);
     c.abort = 0;
@@ -1266,20 +1339,22 @@ __global__ void __launch_bounds__(Shape<HD>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp < Sh::kSoftmaxWarps) {
-    softmax_role<HD>(a, c, tiles, warp, lane);
+    softmax_role<HD, KV8>(a, c, tiles, warp, lane);
   } else {
     if (warp == Sh::kLoadWarp) {
-      load_role<HD>(a, maps, c, tiles, lane);
+      load_role<HD, KV8>(a, maps, c, tiles, lane);
     } else if (warp == Sh::kMmaWarp) {
-      mma_items<HD>(a, c, tiles);
+      mma_items<HD, KV8>(a, c, tiles);
       // one lane issued every product: it is the one elected here too
       if (elect_one()) mma_commit(smem_u32(&c.drained));
       __syncwarp();  // no product or arrival is under way after this:
       const long long start = clock64();
       while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
       }
-    } else {
-      plan_role<HD>(a, c, lane);
+    } else if (warp == Sh::kPlanWarp) {
+      plan_role<HD, KV8>(a, c, lane);
+    } else if constexpr (KV8) {
+      convert_role<HD, KV8>(a, c, tiles, threadIdx.x - Sh::kConvert * 32);
     }
   }
   __syncwarp();
@@ -1310,9 +1385,9 @@ __device__ __forceinline__ void load_row(const float* p, float* v) {
 // Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
 // starts at the end of CTA c's piece, a warp a row.
 constexpr int kJoinSlices = 8;
-template <int HD>
+template <int HD, bool KV8>
 __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
-  using Sh = Shape<HD>;
+  using Sh = Shape<HD, KV8>;
   constexpr int kPer = HD / 32;  // columns of a lane
   grid_wait();
   const int32_t* join = a.joins + blockIdx.x * 8;
@@ -1351,7 +1426,7 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
         for (int x = 0; x < kPer; ++x) acc[x] = acc[x] * keep + w * o[y][x];
       }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;
     const int token = tok0 + tok;
     const int64_t column = int64_t(kvh * a.G + in_tile - row_tok * a.G) * HD + lane * kPer;
 #pragma unroll
@@ -1407,9 +1482,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// A map of 16-bit elements with the 128-byte swizzle.  A dimension of one element needs no
-// stride of its own: any valid one does.
-bool encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
+// A map of elements of `esize` bytes (bf16 or bytes) with the 128-byte swizzle.  A dimension of
+// one element needs no stride of its own: any valid one does.
+bool encode(CUtensorMap* map, const void* base, int esize, int rank, const int64_t* dims,
             const int64_t* strides, const int* box) {
   cuuint64_t d[5], st[5];
   cuuint32_t b[5], es[5];
@@ -1417,29 +1492,30 @@ bool encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
     d[i] = cuuint64_t(dims[i]);
     b[i] = cuuint32_t(box[i]);
     es[i] = 1;
-    if (i > 0) st[i - 1] = dims[i] == 1 ? 128 : cuuint64_t(strides[i]) * 2;
+    if (i > 0) st[i - 1] = dims[i] == 1 ? 128 : cuuint64_t(strides[i]) * esize;
   }
   auto fn = encoder();
-  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base),
+  return fn && fn(map, esize == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  cuuint32_t(rank), const_cast<void*>(base),
                   d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD>
+template <int HD, bool KV8>
 int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaStream_t stream) {
-  using Sh = Shape<HD>;
-  constexpr int kBytes = Sh::kQBytes + Sh::kStages * Sh::kStageBytes + int(sizeof(Control<HD>));
+  using Sh = Shape<HD, KV8>;
+  constexpr int kBytes = Sh::kTileBytes + int(sizeof(Control<HD, KV8>));
   static_assert(kBytes <= 232448, "more shared memory than a CTA may have");
   static bool ready[64] = {false};
   if (!ready[device]) {
     const cudaError_t e = cudaFuncSetAttribute(
-        chunk_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        chunk_kernel<HD, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess)
       return fail(DORY_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     ready[device] = true;
   }
-  chunk_kernel<HD><<<ctas, Sh::kThreads, kBytes, stream>>>(a, maps);
+  chunk_kernel<HD, KV8><<<ctas, Sh::kThreads, kBytes, stream>>>(a, maps);
   int32_t status = dory::launched(cudaSuccess);
   if (status != DORY_OK) return status;
   cudaLaunchConfig_t cfg;
@@ -1452,7 +1528,7 @@ int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaS
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return dory::launched(cudaLaunchKernelEx(&cfg, join_kernel<HD>, a));
+  return dory::launched(cudaLaunchKernelEx(&cfg, join_kernel<HD, KV8>, a));
 }
 
 }  // namespace
@@ -1560,12 +1636,6 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   if (most > (int64_t(1) << 30) / p.num_kv_heads)
     return fail(DORY_ERR_UNSUPPORTED, "more work than one call counts (tokens x positions)");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv8) {
-    const dim3 grid(p.num_tokens, (p.num_heads + 3) / 4);
-    if (p.head_dim == 128) chunk_rows<128, true><<<grid, 128, 0, s>>>(a);
-    else chunk_rows<256, true><<<grid, 128, 0, s>>>(a);
-    return dory::launched(cudaSuccess);
-  }
   int device;
   const int ctas = device_sms(&device);
   if (ctas <= 0) return fail(DORY_ERR_CUDA, "no current CUDA device");
@@ -1580,15 +1650,19 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   const int q_box[3] = {64, G, a.TB};
   const int64_t c_dims[4] = {p.head_dim, p.block_size, p.num_kv_heads, p.num_cache_blocks};
   const int64_t c_strides[4] = {1, p.stride_offset, p.stride_head, p.stride_block};
-  const int c_box[4] = {64, a.copy_rows, 1, 1};
-  if (!encode(&maps.q, p.q, 3, q_dims, q_strides, q_box) ||
-      !encode(&maps.k, p.key_cache, 4, c_dims, c_strides, c_box) ||
-      !encode(&maps.v, p.value_cache, 4, c_dims, c_strides, c_box))
+  const int esize = kv8 ? 1 : 2;
+  const int c_box[4] = {128 / esize, a.copy_rows, 1, 1};
+  if (!encode(&maps.q, p.q, 2, 3, q_dims, q_strides, q_box) ||
+      !encode(&maps.k, p.key_cache, esize, 4, c_dims, c_strides, c_box) ||
+      !encode(&maps.v, p.value_cache, esize, 4, c_dims, c_strides, c_box))
     return fail(DORY_ERR_UNSUPPORTED, "no tensor map for the query or cache view (strides must be "
                                       "positive)");
-  if (p.head_dim == 64) return launch<64>(a, maps, device, ctas, s);
-  if (p.head_dim == 128) return launch<128>(a, maps, device, ctas, s);
-  return launch<256>(a, maps, device, ctas, s);
+  if (kv8)
+    return p.head_dim == 128 ? launch<128, true>(a, maps, device, ctas, s)
+                             : launch<256, true>(a, maps, device, ctas, s);
+  if (p.head_dim == 64) return launch<64, false>(a, maps, device, ctas, s);
+  if (p.head_dim == 128) return launch<128, false>(a, maps, device, ctas, s);
+  return launch<256, false>(a, maps, device, ctas, s);
 }
 
 }  // extern "C"

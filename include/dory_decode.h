@@ -436,8 +436,8 @@ int32_t dory_rotary_append(const DoryRotaryParams* params, void* stream);
  *   out[t][h] = gate[t][h] * sum_c softmax_c(softmax_scale * q[t][h] . K[c]) V[c],
  * K and V of the head's KV head at block_tables[i][c / block_size], row c % block_size (the
  * chunk's own rows already appended, dory_rotary_append).  Scores, softmax statistics and sums
- * are FP32; the weights enter the V product rounded to 11 bits or more relative to the row's
- * largest (BF16 caches: 8 bits).
+ * are FP32; the weights enter the product with V rounded to 8 bits (BF16 caches), or to 11 bits
+ * and at least 2^-32 of the row's largest weight (FP8 caches).
  *
  * A row that sees no position gives zeros; rows outside every sequence keep their contents;
  * seq_lens 0 (a padded request) gives zero rows.  Positions whose block id lies outside the

@@ -4,7 +4,9 @@ Tolerance of an element, with A = sum_c w_c |v_c| (the oracle's second result): 
 rounded to bf16 (2^-8 of each: 2^-8 A), a score is off by at most (D + 4) 2^-24 scale |q| |k| and
 a weight by twice that share, the exponential by 3e-6 (its polynomial) and as much in the sum it
 is divided by, the two sums by (8 + L) 2^-24 at most, and the result is rounded to bf16 (2^-8
-|out|).
+|out|).  FP8 caches: the weights are f16 numbers of at most 2^15 whose row's largest is 2^7 or
+more, so besides 2^-11 of each, a weight is off by up to half a step of f16's smallest, 2^-25,
+which is 2^-32 of the largest: with L of them over a sum of at least the largest, 2^-32 L max|v|.
 """
 
 from __future__ import annotations
@@ -91,6 +93,9 @@ class Batch:
         score = (self.D + 4) * F32 * self.scale * self.q.float().norm(dim=-1).max().item() * k
         rel = 2.0 ** -8 + 2 * score + 6e-6 + (8 + longest) * F32
         tol = rel * size + 2.0 ** -8 * want.abs() * (1 + rel) + 2.0 ** -130
+        if self.fp8:
+            v = self.value.float().nan_to_num(0, 0, 0).abs().max().item() * self.scales[1]
+            tol = tol + 2.0 ** -32 * longest * v * (1 if gate is None else gate.double())
         off = (out.double() - want).abs()
         bad = ~(off <= tol) & owned[:, None]
         assert not bad.any(), (bad.sum().item(), bad.nonzero()[0].tolist(),
