@@ -10,8 +10,9 @@
 // 8-element pieces that contain both members of its pairs: dims 8l and rotary_dim / 2 + 8l of
 // the half layout, 16l and 16l + 8 of the interleaved one, so in both it needs the angles 8l ..
 // 8l + 7 and no exchange between lanes (the norm alone takes log2(head_dim / 16) shuffles).  A
-// lane keeps its angles in registers and uses them for up to kHeads heads of its token, whose
-// loads are all in flight together.
+// block takes the heads of one token, then of the next: a lane keeps its head, so its share of
+// sqk stays in registers, the heads of a token share its angles in L1, and the next token's loads
+// (position, then angles) are on their way while this one is worked on.
 // rotary_any: one warp per row, a pair per lane, for every size, stride and alignment.
 
 #include <cuda_bf16.h>
@@ -21,11 +22,17 @@
 #include <string.h>
 
 #include "dory_common.h"
+#include "dory_sm100.cuh"
 
 namespace {
 
 using dory::aligned16;
 using dory::fail;
+using namespace sm100;  // packed FP32 arithmetic
+
+constexpr int kVecThreads = 384;  // of rotary_vec, in a block at most; two blocks an SM
+constexpr int kSms = 148;
+constexpr int kMaxShared = 227 * 1024;
 
 struct Rows {  // one of q, k, v or an output
   const void* in;
@@ -44,7 +51,10 @@ struct RotaryArgs {
   uint32_t* err;
   int64_t sb, so, sh, cache_slots, max_position;
   float sqk_factor, eps, k_scale, v_scale;
-  int T, NH, NKV, D, R, B, heads, groups;  // heads: rows of a token; groups: head groups
+  int T, NH, NKV, D, R, B;
+  int heads;  // rows of a token
+  int group;  // of them, in a block
+  int run;    // tokens of a block
   int cs_dtype, pos32, sqk_dtype, inter, norm;
   float sign;
 };
@@ -135,146 +145,194 @@ __device__ __forceinline__ const T* row_in(const RotaryArgs& a, int t, int h) {
 }
 
 // ------------------------------------------------------------------------------------
-// kHeads: heads a lane takes.  8 for long prompts would need more registers than it hides
-// latency; 1 spreads a few tokens over as many lanes as there are.
-template <typename T, bool APPEND, bool KV8, int kHeads>
-__global__ void __launch_bounds__(256) rotary_vec(const RotaryArgs a) {
-  const int lanes = a.D / 16;
-  const int rows = 256 / lanes;
-  const int local = threadIdx.x / lanes, l = threadIdx.x - local * lanes;
-  const int64_t row = int64_t(blockIdx.x) * rows + local;
-  const bool live = local < rows && row < int64_t(a.T) * a.groups;
-  const int t = live ? int(row / a.groups) : 0;
-  const int h0 = live ? int(row - int64_t(t) * a.groups) : a.heads;
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+constexpr int kAhead = 3;  // tokens in flight
+template <typename T>
+constexpr int kElementBytes = 16 * int(sizeof(T));  // of a thread and token
 
-  const bool turn = l < a.R / 16;
-  const bool apart = turn && !a.inter;
+template <typename T, bool APPEND, bool KV8>
+__global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a) {
+  // Tokens in flight: [token][16 bytes][thread] of elements, a thread reads its own, then
+  // [token][warp][table row] of angles, a warp reads its own.
+  extern __shared__ uint4 ring[];
+  constexpr int kQuads = int(sizeof(T));  // 16-byte words of a thread's 16 elements
+  const int lanes = a.D / 16;
+  const int local = threadIdx.x / lanes, l = threadIdx.x - local * lanes;
+  const int h = blockIdx.y * a.group + local;
+  const bool here = local < a.group && h < a.heads;
+  const bool is_q = h < a.NH, is_v = APPEND && h >= a.NH + a.NKV;
+  const int g = is_q ? h : is_v ? h - a.NH - a.NKV : h - a.NH;  // among its kind
+  const bool turn = here && !is_v && l < a.R / 16;
+  const bool apart = l < a.R / 16 && !a.inter && !is_v;
   const int oa = apart ? 8 * l : 16 * l, ob = apart ? a.R / 2 + 8 * l : 16 * l + 8;
-  Piece<T> xa[kHeads], xb[kHeads];
+  const Rows& rows = is_q ? a.q : is_v ? a.v : a.k;
+  const T* in = here ? static_cast<const T*>(rows.in) + g * rows.in_h : nullptr;
+  const int64_t in_t = rows.in_t;
+
+  uint64_t weight[8];  // with the norm, pairs: (sqk * sqk_factor)^2 of the lane's dims, 1 for k
+  if constexpr (APPEND) {
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i * a.groups;
-    if (h < a.heads) {
-      const T* p = row_in<T>(a, t, h);
-      xa[i] = load_piece(p + oa);
-      xb[i] = load_piece(p + ob);
+    for (int j = 0; j < 8; ++j) weight[j] = pair(1.0f, 1.0f);
+    if (a.norm && here && is_q) {
+      float w[16];
+      load8(a.sqk, int64_t(h) * a.D + oa, a.sqk_dtype, reinterpret_cast<float(&)[8]>(w[0]));
+      load8(a.sqk, int64_t(h) * a.D + ob, a.sqk_dtype, reinterpret_cast<float(&)[8]>(w[8]));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] = w[j] * a.sqk_factor * (w[j] * a.sqk_factor);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) weight[j] = pair(w[2 * j], w[2 * j + 1]);
     }
   }
-  float c[8], s[8];
-  bool inside = true;
-  int64_t slot = -1;
-  if (live) {
-    if (APPEND) slot = a.slots[t];
-    if (a.R > 0) {
-      const int64_t pos = position_of(a, t);
-      inside = pos >= 0 && pos < a.max_position;
-      if (turn && inside) {
-        load8(a.cos_sin, pos * a.R + 8 * l, a.cs_dtype, c);
-        load8(a.cos_sin, pos * a.R + a.R / 2 + 8 * l, a.cs_dtype, s);
+
+  const int first = blockIdx.x * a.run, last = min(first + a.run, a.T);  // this block's tokens
+  const int warps = blockDim.x >> 5;
+  const int angle_quads = a.R * (a.cs_dtype == DORY_DTYPE_F32 ? 4 : 2) / 16;
+  const uint4* const angle_ring = ring + kAhead * kQuads * blockDim.x;
+  const uint32_t own = uint32_t(__cvta_generic_to_shared(ring + threadIdx.x));
+  auto angles_of = [&](int place) {  // this warp's copy of a token's angles
+    return angle_ring + (place * warps + (threadIdx.x >> 5)) * angle_quads;
+  };
+  auto position = [&](int t) { return a.R > 0 && t < last ? position_of(a, t) : int64_t(0); };
+  auto inside = [&](int64_t pos) { return a.R == 0 || (pos >= 0 && pos < a.max_position); };
+  // Starts the loads of token t, at position pos: elements and angles by asynchronous copies,
+  // since registers for as many tokens would leave too few threads.
+  auto ask = [&](int t, int64_t pos, int place) {
+    if (t < last) {
+      if (here) {
+        const T* p = in + t * in_t;
+#pragma unroll
+        for (int i = 0; i < kQuads / 2; ++i) {
+          copy_async(own + (place * kQuads + i) * blockDim.x * 16, p + oa + i * (16 / sizeof(T)));
+          copy_async(own + (place * kQuads + kQuads / 2 + i) * blockDim.x * 16,
+                     p + ob + i * (16 / sizeof(T)));
+        }
       }
-      if (!inside && h0 == 0 && l == 0 && !(APPEND && slot < 0))
-        report(a, DORY_DEVERR_POSITION_OOB);
+      if (a.R > 0 && inside(pos)) {
+        const uint4* row = static_cast<const uint4*>(a.cos_sin) + pos * angle_quads;
+        const uint32_t to = uint32_t(__cvta_generic_to_shared(angles_of(place)));
+        for (int i = threadIdx.x & 31; i < angle_quads; i += 32) copy_async(to + i * 16, row + i);
+      }
     }
-    if (APPEND && slot >= a.cache_slots) {
-      if (h0 == 0 && l == 0) report(a, DORY_DEVERR_SLOT_OOB);
-      slot = -1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+#pragma unroll 1
+  for (int i = 0; i < kAhead - 1; ++i) ask(first + i, position(first + i), i);
+  int64_t pos = position(first), pos_ask = position(first + kAhead - 1);
+  int64_t slot = APPEND && first < last ? a.slots[first] : 0;
+  int place = 0;
+#pragma unroll 1
+  for (int t = first; t < last; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+    __syncwarp();  // the warp's angles are there, and its reads of the token before are done
+    ask(t + kAhead - 1, pos_ask, place == 0 ? kAhead - 1 : place - 1);
+    const int64_t pos_next = position(t + 1);
+    pos_ask = position(t + kAhead);
+    const int64_t slot_next = APPEND && t + 1 < last ? a.slots[t + 1] : 0;
+    const bool known = inside(pos);
+    uint64_t y[8];  // the lane's elements in pairs: four of the first piece, four of the second
+    {
+      Piece<T> xa, xb;
+#pragma unroll
+      for (int i = 0; i < kQuads / 2; ++i) {
+        xa.w[i] = ring[(place * kQuads + i) * blockDim.x + threadIdx.x];
+        xb.w[i] = ring[(place * kQuads + kQuads / 2 + i) * blockDim.x + threadIdx.x];
+      }
+      float ya[8], yb[8];
+      unpack(xa, ya);
+      unpack(xb, yb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = pair(ya[2 * j], ya[2 * j + 1]);
+        y[4 + j] = pair(yb[2 * j], yb[2 * j + 1]);
+      }
     }
-  }
+    if (!is_v && !known) {
 #pragma unroll
-  for (int i = 0; i < kHeads; ++i) {
-    const int h = h0 + i * a.groups;
-    const bool here = h < a.heads, is_v = APPEND && h >= a.NH + a.NKV;
-    float ya[8], yb[8];
-    if (here) {
-      unpack(xa[i], ya);
-      unpack(xb[i], yb);
-      if (!is_v && !inside) {
+      for (int j = 0; j < 8; ++j) y[j] = 0;
+    } else if (turn) {
+      float c[8], s[8];
+      load8(angles_of(place), 8 * l, a.cs_dtype, c);
+      load8(angles_of(place), a.R / 2 + 8 * l, a.cs_dtype, s);
+      if (a.inter) {  // a pair is one rotation: (u, w) c + (w, u) (-s, s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ya[j] = yb[j] = 0.0f;
-      } else if (!is_v && turn) {
-        if (a.inter) {
+        for (int j = 0; j < 8; ++j) {
+          float u, w;
+          split(y[j], u, w);
+          const float turn_by = a.sign * s[j];
+          y[j] = fma2(pair(w, u), pair(-turn_by, turn_by), mul2(y[j], pair(c[j], c[j])));
+        }
+      } else {  // two rotations at once
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float a0 = ya[2 * j], a1 = ya[2 * j + 1], b0 = yb[2 * j], b1 = yb[2 * j + 1];
-            const float sa = a.sign * s[j], sb = a.sign * s[4 + j];
-            ya[2 * j] = a0 * c[j] - a1 * sa;
-            ya[2 * j + 1] = a1 * c[j] + a0 * sa;
-            yb[2 * j] = b0 * c[4 + j] - b1 * sb;
-            yb[2 * j + 1] = b1 * c[4 + j] + b0 * sb;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float x = ya[j], y = yb[j], sj = a.sign * s[j];
-            ya[j] = x * c[j] - y * sj;
-            yb[j] = y * c[j] + x * sj;
-          }
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t u = y[j], w = y[4 + j], c2 = pair(c[2 * j], c[2 * j + 1]);
+          const uint64_t s2 = pair(a.sign * s[2 * j], a.sign * s[2 * j + 1]);
+          y[j] = fma2(mul2(w, pair(-1.0f, -1.0f)), s2, mul2(u, c2));
+          y[4 + j] = fma2(u, s2, mul2(w, c2));
         }
       }
     }
     if constexpr (APPEND) {
       if (a.norm) {  // every lane of the warp takes part: rows never straddle a warp
-        float sum = 0.0f;
-        if (here && !is_v) {
+        uint64_t squares = mul2(y[0], y[0]);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum += ya[j] * ya[j] + yb[j] * yb[j];
-        }
+        for (int j = 1; j < 8; ++j) squares = fma2(y[j], y[j], squares);
+        float sum, other;
+        split(squares, sum, other);
+        sum += other;
         for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-        if (here && !is_v) {
+        if (!is_v) {
           const float inv = rsqrtf(sum + a.eps);
-          float wa[8], wb[8];
-          if (h < a.NH) {
-            load8(a.sqk, int64_t(h) * a.D + oa, a.sqk_dtype, wa);
-            load8(a.sqk, int64_t(h) * a.D + ob, a.sqk_dtype, wb);
-          }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float fa = inv, fb = inv;
-            if (h < a.NH) {
-              const float u = wa[j] * a.sqk_factor, w = wb[j] * a.sqk_factor;
-              fa *= u * u;
-              fb *= w * w;
-            }
-            ya[j] *= fa;
-            yb[j] *= fb;
-          }
+          for (int j = 0; j < 8; ++j) y[j] = mul2(y[j], mul2(weight[j], pair(inv, inv)));
         }
       }
     }
-    if (!here) continue;
-    if (h < a.NH) {
-      if constexpr (APPEND) {
-        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.q.out) + t * a.q.out_t + h * a.q.out_h;
-        store_piece(o + oa, ya);
-        store_piece(o + ob, yb);
-      } else {
-        T* o = static_cast<T*>(a.q.out) + t * a.q.out_t + h * a.q.out_h;
-        store_piece(o + oa, ya);
-        store_piece(o + ob, yb);
-      }
-    } else if constexpr (!APPEND) {
-      T* o = static_cast<T*>(a.k.out) + t * a.k.out_t + (h - a.NH) * a.k.out_h;
-      store_piece(o + oa, ya);
-      store_piece(o + ob, yb);
-    } else if (slot >= 0) {
-      const int g = is_v ? h - a.NH - a.NKV : h - a.NH;
-      uint8_t* o = cache_row(a, is_v ? a.vc : a.kc, slot, g, KV8 ? 1 : 2);
-      if constexpr (KV8) {
-        const float scale = is_v ? a.v_scale : a.k_scale;
+    if (h == 0 && l == 0) {
+      if (!known && !(APPEND && slot < 0)) report(a, DORY_DEVERR_POSITION_OOB);
+      if (APPEND && slot >= a.cache_slots) report(a, DORY_DEVERR_SLOT_OOB);
+    }
+    if (here) {
+      float ya[8], yb[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float(&y)[8] = half ? yb : ya;
-          uint2 w;
-          w.x = to_e4m3x2(y[0], y[1], scale) | to_e4m3x2(y[2], y[3], scale) << 16;
-          w.y = to_e4m3x2(y[4], y[5], scale) | to_e4m3x2(y[6], y[7], scale) << 16;
-          *reinterpret_cast<uint2*>(o + (half ? ob : oa)) = w;
+      for (int j = 0; j < 4; ++j) {
+        split(y[j], ya[2 * j], ya[2 * j + 1]);
+        split(y[4 + j], yb[2 * j], yb[2 * j + 1]);
+      }
+      if (!APPEND || is_q) {
+        if constexpr (APPEND) {
+          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.q.out) + t * a.q.out_t + g * a.q.out_h;
+          store_piece(o + oa, ya);
+          store_piece(o + ob, yb);
+        } else {
+          T* o = static_cast<T*>(rows.out) + t * rows.out_t + g * rows.out_h;
+          store_piece(o + oa, ya);
+          store_piece(o + ob, yb);
         }
-      } else {
-        __nv_bfloat16* b = reinterpret_cast<__nv_bfloat16*>(o);
-        store_piece(b + oa, ya);
-        store_piece(b + ob, yb);
+      } else if (slot >= 0 && slot < a.cache_slots) {
+        uint8_t* o = cache_row(a, is_v ? a.vc : a.kc, slot, g, KV8 ? 1 : 2);
+        if constexpr (KV8) {
+          const float scale = is_v ? a.v_scale : a.k_scale;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float(&v)[8] = half ? yb : ya;
+            uint2 w;
+            w.x = to_e4m3x2(v[0], v[1], scale) | to_e4m3x2(v[2], v[3], scale) << 16;
+            w.y = to_e4m3x2(v[4], v[5], scale) | to_e4m3x2(v[6], v[7], scale) << 16;
+            *reinterpret_cast<uint2*>(o + (half ? ob : oa)) = w;
+          }
+        } else {
+          __nv_bfloat16* b = reinterpret_cast<__nv_bfloat16*>(o);
+          store_piece(b + oa, ya);
+          store_piece(b + ob, yb);
+        }
       }
     }
+    pos = pos_next;
+    slot = slot_next;
+    if (++place == kAhead) place = 0;
   }
 }
 
@@ -376,19 +434,34 @@ int32_t run(RotaryArgs& a, bool pieces, cudaStream_t stream) {
     cfg.blockDim = dim3(128);
     return dory::launched(cudaLaunchKernelEx(&cfg, rotary_any<T, APPEND, KV8>, a));
   }
-  const int lanes = a.D / 16, rows = 256 / lanes;
-  constexpr int kMany = 4;
-  // One head a lane until that fills the machine about once (148 SMs x 2,048 threads); then
-  // kMany, which share their angles.
-  const int per_lane = int64_t(a.T) * a.heads * lanes > 148 * 2048 ? kMany : 1;
-  a.groups = (a.heads + per_lane - 1) / per_lane;
-  const int64_t blocks = (int64_t(a.T) * a.groups + rows - 1) / rows;
-  if (blocks > INT32_MAX) return fail(DORY_ERR_UNSUPPORTED, "too many tokens for one launch");
-  cfg.gridDim = dim3(unsigned(blocks));
-  cfg.blockDim = dim3(256);
-  return dory::launched(
-      per_lane == 1 ? cudaLaunchKernelEx(&cfg, rotary_vec<T, APPEND, KV8, 1>, a)
-                    : cudaLaunchKernelEx(&cfg, rotary_vec<T, APPEND, KV8, kMany>, a));
+  // A block takes `group` heads of one token after the other: as many blocks as tokens while
+  // that leaves SMs idle, then about kVecThreads threads an SM, which prefetch a token ahead.
+  const int lanes = a.D / 16;
+  a.group = kVecThreads / lanes < a.heads ? kVecThreads / lanes : a.heads;
+  const int parts = (a.heads + a.group - 1) / a.group;
+  a.group = (a.heads + parts - 1) / parts;
+  const int threads = (a.group * lanes + 31) / 32 * 32;
+  const int64_t resident = int64_t(kSms) * (2 * kVecThreads / threads);
+  const int64_t blocks = (resident + parts - 1) / parts;
+  a.run = int((a.T + blocks - 1) / blocks);
+  cfg.gridDim = dim3(unsigned((a.T + a.run - 1) / a.run), unsigned(parts));
+  cfg.blockDim = dim3(unsigned(threads));
+  const int angles = a.R * (a.cs_dtype == DORY_DTYPE_F32 ? 4 : 2);
+  cfg.dynamicSmemBytes = unsigned(kAhead * (threads * kElementBytes<T> + threads / 32 * angles));
+  int device = 0;
+  static bool ready[64] = {false};
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64)
+    return fail(DORY_ERR_CUDA, "no current CUDA device");
+  if (!ready[device]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(rotary_vec<T, APPEND, KV8>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMaxShared);
+    if (e != cudaSuccess)
+      return fail(DORY_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    ready[device] = true;
+  }
+  return dory::launched(cudaLaunchKernelEx(&cfg, rotary_vec<T, APPEND, KV8>, a));
 }
 
 template <bool APPEND, bool KV8>
@@ -469,7 +542,6 @@ int32_t rotary(const DoryRotaryParams* P, bool append, void* stream) {
   a.R = p.rotary_dim;
   a.B = p.block_size;
   a.heads = a.NH + (append ? 2 : 1) * a.NKV;
-  a.groups = a.heads;
   a.cs_dtype = p.cos_sin_dtype;
   a.pos32 = p.positions_dtype;
   a.sqk_dtype = p.sqk_dtype;
@@ -492,7 +564,9 @@ int32_t rotary(const DoryRotaryParams* P, bool append, void* stream) {
     pieces = pieces && aligned16(p.key_cache) && aligned16(p.value_cache) &&
              !((a.sb | a.so | a.sh) & 7);
   }
-  pieces = pieces && aligned16(p.cos_sin) && aligned16(p.sqk);
+  // A block's ring is then at most 3 x (384 threads x 64 bytes + 12 warps x 1 KB) = 108 KB.
+  const int angle_bytes = p.rotary_dim * (p.cos_sin_dtype == DORY_DTYPE_F32 ? 4 : 2);
+  pieces = pieces && aligned16(p.cos_sin) && aligned16(p.sqk) && angle_bytes <= 1024;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!append) return run_type<false, false>(a, p.io_dtype, pieces, s);
   return kv8 ? run_type<true, true>(a, p.io_dtype, pieces, s)
