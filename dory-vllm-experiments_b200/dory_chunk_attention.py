@@ -57,6 +57,8 @@ class ChunkAttention:
             self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             _native.check(self._lib.dory_decode_scratch_init(
                 self.scratch.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+        self._call = self._lib.dory_chunk_attention
+        self._scratch = (self.scratch.data_ptr(), self.scratch.numel())
         self._dev_index = self.scratch.get_device()
 
     def __call__(self, q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -118,17 +120,15 @@ class ChunkAttention:
         packed = _pack(
             q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
             query_start.data_ptr(), seq_lens.data_ptr(), gate_ptr, out.data_ptr(),
-            self.scratch.data_ptr(), self.scratch.numel(), q_token, q_head, out.stride(0),
+            *self._scratch, q_token, q_head, out.stride(0),
             gate_token, block_tables.stride(0), strides[0], strides[1], strides[2], cache[0],
             float(softmax_scale), float(k_scale), float(v_scale), tokens, seqs, table[1], heads,
             self.num_kv_heads, dim, cache[1], int(window), gate_code, self._kv_code)
-        if torch.cuda.current_device() != dev:
+        if torch._C._cuda_getDevice() != dev:
             with torch.cuda.device(dev):
-                status = self._lib.dory_chunk_attention(
-                    packed, torch._C._cuda_getCurrentRawStream(dev))
+                status = self._call(packed, torch._C._cuda_getCurrentRawStream(dev))
         else:
-            status = self._lib.dory_chunk_attention(packed,
-                                                    torch._C._cuda_getCurrentRawStream(dev))
+            status = self._call(packed, torch._C._cuda_getCurrentRawStream(dev))
         if status:
             _native.check(status)
 

@@ -86,31 +86,28 @@ def _heads(name: str, x: torch.Tensor, tokens: int, head_dim: int) -> tuple:
     return x.data_ptr(), stride[0], stride[1], shape[1]
 
 
-def _span(x: torch.Tensor) -> tuple[int, int]:
-    """First and past-the-last byte address of x's elements."""
-    start = x.data_ptr()
-    if not x.numel():
-        return start, start
-    reach = sum((n - 1) * st for n, st in zip(x.shape, x.stride()))
-    return start, start + (reach + 1) * x.element_size()
-
-
-def _check_output(name: str, out: torch.Tensor, x: torch.Tensor, in_place: bool) -> None:
-    """ValueError if rows of `out` lie on one another, or `out` over its input `x` (unless it
-    is that tensor itself and in_place allows it)."""
-    if not out.numel():
+def _check_output(name: str, out: tuple, out_size: int, x: tuple, x_size: int, tokens: int,
+                  dim: int, in_place: bool) -> None:
+    """ValueError if rows of an output lie on one another, or the output over its input `x`
+    (unless it is that tensor itself and in_place allows it).  out, x: as _heads returns them;
+    out_size, x_size: bytes of an element."""
+    ptr, token, head, heads = out
+    if not tokens or not heads:
         return
-    reach = out.shape[2]
-    for n, stride in sorted(zip(out.shape[:2], out.stride()[:2]), key=lambda d: d[1]):
-        if n > 1 and stride < reach:
-            raise ValueError(f"{name}'s rows must not overlap")
-        reach += (n - 1) * stride if n > 1 else 0
-    if x.data_ptr() == out.data_ptr() and x.stride() == out.stride() and x.dtype == out.dtype:
+    if heads > 1 and tokens > 1:
+        inner, outer, n = (head, token, heads) if head <= token else (token, head, tokens)
+        bad = inner < dim or outer < (n - 1) * inner + dim
+    else:
+        bad = (heads > 1 and head < dim) or (tokens > 1 and token < dim)
+    if bad:
+        raise ValueError(f"{name}'s rows must not overlap")
+    if ptr == x[0] and token == x[1] and head == x[2] and out_size == x_size:
         if in_place:
             return
         raise ValueError(f"{name} must not be its input")
-    (lo, hi), (a, b) = _span(out), _span(x)
-    if lo < b and a < hi:
+    end = ptr + ((tokens - 1) * token + (heads - 1) * head + dim) * out_size
+    x_end = x[0] + ((tokens - 1) * x[1] + (heads - 1) * x[2] + dim) * x_size
+    if ptr < x_end and x[0] < end:
         raise ValueError(f"{name} must lie apart from its input" +
                          (" or be that tensor itself" if in_place else ""))
 
@@ -143,9 +140,14 @@ def _error_ptr(error_word) -> int:
     return error_word.data_ptr()
 
 
+_functions: dict = {}
+
+
 def _launch(name: str, device: int, packed: bytes) -> None:
-    fn = getattr(_native.load(), name)
-    if torch.cuda.current_device() != device:
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_native.load(), name)
+    if torch._C._cuda_getDevice() != device:
         with torch.cuda.device(device):
             status = fn(packed, torch._C._cuda_getCurrentRawStream(device))
     else:
@@ -177,20 +179,21 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     device = q.get_device()
     _native.check_device_index(device, q_out, k, k_out, positions, cos_sin, error_word)
     tokens, _, dim = q.shape
-    q_ptr, q_t, q_h, heads = _heads("q", q, tokens, dim)
-    qo_ptr, qo_t, qo_h, out_heads = _heads("q_out", q_out, tokens, dim)
+    size = q.element_size()
+    q_ptr, q_t, q_h, heads = q_rows = _heads("q", q, tokens, dim)
+    qo_ptr, qo_t, qo_h, out_heads = qo_rows = _heads("q_out", q_out, tokens, dim)
     if out_heads != heads:
         raise ValueError("q_out must have q's heads")
+    _check_output("q_out", qo_rows, size, q_rows, size, tokens, dim, True)
     k_ptr = k_t = k_h = ko_ptr = ko_t = ko_h = kv_heads = 0
-    _check_output("q_out", q_out, q, True)
     if k is not None:
         if k.dtype is not q.dtype or k_out.dtype is not q.dtype:
             raise ValueError("k and k_out must have q's type")
-        k_ptr, k_t, k_h, kv_heads = _heads("k", k, tokens, dim)
-        ko_ptr, ko_t, ko_h, out_heads = _heads("k_out", k_out, tokens, dim)
+        k_ptr, k_t, k_h, kv_heads = k_rows = _heads("k", k, tokens, dim)
+        ko_ptr, ko_t, ko_h, out_heads = ko_rows = _heads("k_out", k_out, tokens, dim)
         if out_heads != kv_heads:
             raise ValueError("k_out must have k's heads")
-        _check_output("k_out", k_out, k, True)
+        _check_output("k_out", ko_rows, size, k_rows, size, tokens, dim, True)
     pos_ptr, table, rotary, max_position, table_code, pos32 = _table(cos_sin, positions, tokens, dim)
     flags = ((_native.ROTARY_INTERLEAVED if interleaved else 0) |
              (_native.ROTARY_INVERSE if inverse else 0))
@@ -238,15 +241,15 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     if q is not None:
         if q_out.dtype is not torch.bfloat16:
             raise ValueError("q_out must be bfloat16")
-        q_ptr, q_t, q_h, heads = _heads("q", q, tokens, dim)
+        q_ptr, q_t, q_h, heads = q_rows = _heads("q", q, tokens, dim)
         if q_out.dim() == 2:
             if q_out.shape[1] != heads * dim or q_out.stride(1) != 1:
                 raise ValueError("q_out must be [tokens, heads * head_dim]")
             q_out = q_out.unflatten(1, (heads, dim))
-        qo_ptr, qo_t, qo_h, out_heads = _heads("q_out", q_out, tokens, dim)
+        qo_ptr, qo_t, qo_h, out_heads = qo_rows = _heads("q_out", q_out, tokens, dim)
         if out_heads != heads:
             raise ValueError("q_out must have q's heads")
-        _check_output("q_out", q_out, q, False)
+        _check_output("q_out", qo_rows, 2, q_rows, q.element_size(), tokens, dim, False)
     pos_ptr, table, rotary, max_position, table_code, pos32 = _table(cos_sin, positions, tokens, dim)
     shape, stride = key_cache.shape, key_cache.stride()
     if stride != value_cache.stride() or stride[-1] != 1 or shape != value_cache.shape:

@@ -92,19 +92,26 @@ def test_cpu_tensors_are_refused():
 
 
 def test_output_checks():
+    def check(out, x, in_place):
+        T, _, D = x.shape
+        _check_output("o", _heads("o", out, T, D), out.element_size(), _heads("x", x, T, D),
+                      x.element_size(), T, D, in_place)
     x = torch.zeros(4, 3, 8)
-    _check_output("o", x, x, True)                      # itself
-    _check_output("o", torch.zeros(4, 3, 8), x, False)  # apart
-    _check_output("o", torch.zeros(3, 4, 8).transpose(0, 1), x, False)
+    check(x, x, True)                      # itself
+    check(torch.zeros(4, 3, 8), x, False)  # apart
+    check(torch.zeros(3, 4, 8).transpose(0, 1), x, False)
+    check(torch.zeros(1, 3, 8).expand(4, 3, 8)[:1], x[:1], False)  # one token: any stride
     with pytest.raises(ValueError, match="must not be its input"):
-        _check_output("o", x, x, False)
+        check(x, x, False)
     big = torch.zeros(5, 3, 8)
     with pytest.raises(ValueError, match="apart"):
-        _check_output("o", big[1:], big[:4], True)
+        check(big[1:], big[:4], True)
+    with pytest.raises(ValueError, match="apart"):  # another type over the same memory
+        check(x.view(torch.float16)[..., :8], x, False)
     with pytest.raises(ValueError, match="rows must not overlap"):
-        _check_output("o", torch.zeros(1, 3, 8).expand(4, 3, 8), x, True)
+        check(torch.zeros(1, 3, 8).expand(4, 3, 8), x, True)
     with pytest.raises(ValueError, match="rows must not overlap"):
-        _check_output("o", torch.zeros(100).as_strided((4, 3, 8), (12, 8, 1)), x, True)
+        check(torch.zeros(100).as_strided((4, 3, 8), (12, 8, 1)), x, True)
 
 
 def test_argument_checks():
