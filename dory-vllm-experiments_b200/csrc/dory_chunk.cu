@@ -187,10 +187,13 @@ struct Control {  // shared memory behind the tiles
       item_empty[kQueue], drained;
   Item items[kQueue];
   uint32_t bad[kBadRing];
-  float q_scale[KV8 ? Shape<HD, KV8>::kItemRows : 1];  // what a row's f16 query was divided by
+  // what a row's f16 query was divided by; a set for the item after, which the conversion may
+  // reach while softmax warps are still at the output of the item before
+  float q_scale[2][KV8 ? Shape<HD, KV8>::kItemRows : 1];
   uint32_t tmem;
   int abort;
-  float swap[Shape<HD, KV8>::kTiles][Shape<HD, KV8>::kShares][kM];  // a row's maxima and sums, by share
+  // a row's maxima and sums, by share
+  float swap[Shape<HD, KV8>::kTiles][Shape<HD, KV8>::kShares][Shape<HD, KV8>::kShares > 1 ? kM : 1];
 };
 
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
@@ -583,7 +586,6 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
     const int hi = min(it.pos0 + it.ntok, it.cap);
     if (!wait_warp(c.q_raw, q_phase, &c.abort, a.err)) return;
-    q_phase ^= 1;
 #pragma unroll 1
     for (int t = 0; t < Sh::kTiles; ++t) {  // a row a thread, in place
       const uint32_t row = tiles + t * (HD / 64) * kChunkBytes + thread * 128;
@@ -612,8 +614,9 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
                           __uint_as_float(w[y] & 0xffff0000u) * scale);
         sts128(piece, w);
       }
-      c.q_scale[t * kM + thread] = __uint_as_float(uint32_t(127 - up) << 23);
+      c.q_scale[q_phase][t * kM + thread] = __uint_as_float(uint32_t(127 - up) << 23);
     }
+    q_phase ^= 1;
     fence_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(&c.q_full));
@@ -960,7 +963,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
   const int row_tok = row / a.G, row_head = row - row_tok * a.G;
   const bool row_real = row < a.TB * a.G;
   int queued = 0;
-  uint32_t scored = 0, summed = 0, tiles_seen_before = 0, stage_no = 0;
+  uint32_t scored = 0, summed = 0, tiles_seen_before = 0, stage_no = 0, q_set = 0;
   // The last sum given to the tensor cores is complete.  A parity can only be asked for with one
   // phase of its barrier outstanding.  Two tiles: a phase an item.  256-dim heads: a phase a
   // tile, on two barriers in turn, because scores j only vouch for the sum of tile j - 2.
@@ -999,7 +1002,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
         return;
       tc_fence_after();
       if (KV8 && j == b && live) {  // there since the first scores: they needed the queries
-        sl = a.scale_log2 * a.k_scale * c.q_scale[t * kM + row];
+        sl = a.scale_log2 * a.k_scale * c.q_scale[q_set][t * kM + row];
         slack = kSlack / sl;
       }
       const uint32_t bad = c.bad[(tiles_seen_before + (j - it.kv0)) % kBadRing];
@@ -1149,6 +1152,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       if (!kTwo) ++summed;
     }
     tiles_seen_before += it.kvn;
+    q_set ^= it.kvn > 0;  // the items that have queries
     stage_no += 2 * Sh::kHalves * it.kvn;
 
     // the item's rows

@@ -250,6 +250,24 @@ def test_a_long_prompt_many_times(D):
         assert torch.equal(b.run(attn=attn), first)
 
 
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+@pytest.mark.parametrize("most", [3, 40, 200])
+def test_many_short_sequences(D, fp8, most):
+    """Several items an SM, of one tile or a few: loads and conversions run items ahead of the
+    softmax, whose warps are at the output of the item before."""
+    g = torch.Generator().manual_seed(most)
+    n = torch.randint(1, most + 1, (400,), generator=g)
+    extra = torch.randint(0, 3 * most, (400,), generator=g) * (torch.rand(400, generator=g) < 0.7)
+    b = Batch([(int(x), int(x + y)) for x, y in zip(n, extra)], NH=8, NKV=4, D=D, fp8=fp8, seed=16)
+    # rows of different sizes: a scale that belongs to another item shows
+    b.q *= torch.exp2(torch.randint(-6, 3, (b.T, 1, 1), device=DEV).float()).to(torch.bfloat16)
+    attn = b.attention()
+    first = b.run(attn=attn, gate=b.gate).clone()
+    b.check(first, gate=b.gate)
+    for _ in range(10):
+        assert torch.equal(b.run(attn=attn, gate=b.gate), first)
+
+
 def test_long_cache_offsets_pass_32_bits():
     """Block strides that take element and byte offsets past 2^32."""
     NKV, D, B, blocks = 8, 128, 16, 140_000  # 32,768 elements a block: 4.6e9 elements
