@@ -21,17 +21,24 @@ does that step for a decode batch:
   the cache (`reshape_and_cache`): a negative slot writes nothing; padded requests (seq_len
   0, slot -1 in vLLM's CUDA-graph padding) write nothing and output zero.
 
-Only decode batches (max_query_len == 1) are taken: prefill stays on vLLM's attention, as in
-the reference.  vLLM itself is not imported: the metadata is read by attribute.  Row
-offsets are allocated once per block-table row stride and kept, so calls can be captured in
-CUDA graphs after the first one.
+* `VllmChunkBinding(attention).forward(metadata, kv_cache, q, k, v, positions, ...)`: one layer
+  over a batch of any kind (prompts, parts of prompts, drafted tokens, decodes, mixed) from
+  `query_start_loc` (int32 [num_reqs + 1]), `seq_lens`, `block_table` and `slot_mapping`:
+  dory_rotary_steps.rotary_append for the batch's tokens, then ChunkAttention over the cache.
+  The reference leaves these batches to vLLM's attention.
+
+VllmDecodeBinding takes decode batches (max_query_len == 1) only.  vLLM itself is not imported:
+the metadata is read by attribute.  Row offsets are allocated once per block-table row stride
+and kept, so calls can be captured in CUDA graphs after the first one.
 """
 
 from __future__ import annotations
 
 import torch
 
-from dory_decode_attention import DecodeAttention
+from dory_chunk_attention import ChunkAttention
+from dory_decode_attention import EPS, DecodeAttention
+from dory_rotary_steps import rotary_append
 
 
 def kv_cache_views(kv_cache: torch.Tensor, num_kv_heads: int, head_dim: int):
@@ -93,3 +100,58 @@ class VllmDecodeBinding:
                          table, self._rows(table.stride(0))[:tokens], seq_lens[:tokens], window,
                          softmax_scale, gate, out_nibble_major, out_sumsq=out_sumsq,
                          slot_mapping=slots[:tokens], k_scale=k_scale, v_scale=v_scale)
+
+
+class VllmChunkBinding:
+    """One ChunkAttention instance (its scratch) serving vLLM batches of any kind layer by layer."""
+
+    def __init__(self, attention: ChunkAttention):
+        a = self.attention = attention
+        self._shape = (a.num_kv_heads, a.head_dim)
+
+    @staticmethod
+    def _read(metadata) -> tuple:
+        seq_lens, table, starts = metadata.seq_lens, metadata.block_table, metadata.query_start_loc
+        if starts.numel() < seq_lens.numel() + 1 or table.shape[0] < seq_lens.numel():
+            raise ValueError("metadata needs a query_start_loc entry and a block-table row per "
+                             "request, and the end of the last")
+        return seq_lens, table, starts
+
+    def append(self, metadata, kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+               v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+               q_out: torch.Tensor, *, sqk: torch.Tensor | None = None, sqk_factor: float = 1.0,
+               eps: float = EPS, interleaved: bool = False, k_scale: float = 1.0,
+               v_scale: float = 1.0, error_word: torch.Tensor | None = None) -> None:
+        """The batch's T tokens rotated at `positions`, with `sqk` normalised, their k and v
+        written where the metadata's slot_mapping says (padded tokens: -1), q into q_out (BF16
+        [T, heads, head_dim]).  q, k, v: [T, heads, head_dim], e.g. slices of the layer's fused
+        projection."""
+        key, value = kv_cache_views(kv_cache, *self._shape)
+        rotary_append(q, k, v, positions, cos_sin, metadata.slot_mapping, key, value, q_out,
+                      sqk=sqk, sqk_factor=sqk_factor, eps=eps, interleaved=interleaved,
+                      k_scale=k_scale, v_scale=v_scale, error_word=error_word)
+
+    def attend(self, metadata, kv_cache: torch.Tensor, q: torch.Tensor, window: int,
+               softmax_scale: float, out: torch.Tensor, gate: torch.Tensor | None = None, *,
+               k_scale: float = 1.0, v_scale: float = 1.0) -> None:
+        """Attention of the batch's tokens (q as append left it) over the cache that holds them:
+        out BF16 [T, heads * head_dim], gate as ChunkAttention takes it.  Rows behind the last
+        request (CUDA-graph padding) keep what out held."""
+        seq_lens, table, starts = self._read(metadata)
+        key, value = kv_cache_views(kv_cache, *self._shape)
+        self.attention(q, key, value, table, starts, seq_lens, window, softmax_scale, out, gate,
+                       k_scale=k_scale, v_scale=v_scale)
+
+    def forward(self, metadata, kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                q_out: torch.Tensor, window: int, softmax_scale: float, out: torch.Tensor,
+                gate: torch.Tensor | None = None, *, sqk: torch.Tensor | None = None,
+                sqk_factor: float = 1.0, eps: float = EPS, interleaved: bool = False,
+                k_scale: float = 1.0, v_scale: float = 1.0,
+                error_word: torch.Tensor | None = None) -> None:
+        """append, then attend: one layer's step, three launches and nothing read by the host."""
+        self.append(metadata, kv_cache, q, k, v, positions, cos_sin, q_out, sqk=sqk,
+                    sqk_factor=sqk_factor, eps=eps, interleaved=interleaved, k_scale=k_scale,
+                    v_scale=v_scale, error_word=error_word)
+        self.attend(metadata, kv_cache, q_out, window, softmax_scale, out, gate, k_scale=k_scale,
+                    v_scale=v_scale)
