@@ -154,14 +154,22 @@ struct Shape {
   static constexpr int kParts = kScoreCols > 32 ? 2 : 1;     // the weights are handed over in
   static constexpr int kPartCols = kScoreCols / kParts;
   static constexpr int kSoftmaxWarps = 4 * kShares * kTiles;
-  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1,
-                       kPlanWarp = kSoftmaxWarps + 2;
-  [[maybe_unused]] static constexpr int kConvert = kSoftmaxWarps + 3;  // the first of these
-  static constexpr int kThreads = (kSoftmaxWarps + 3 + kConvertWarps) * 32;
+  // Copying warps: the 256-dim heads' four stages a tile keep one busier than the products
+  // (16-row pages, prompt of 8192: 777 us, 699 with two); elsewhere the second only takes issue
+  // slots (542 us, 565).
+  static constexpr int kLoaders = HD == 256 && !KV8 ? 2 : 1;
+  static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kLoadWarp + kLoaders,
+                       kPlanWarp = kMmaWarp + 1;
+  [[maybe_unused]] static constexpr int kConvert = kPlanWarp + 1;  // the first of these
+  static constexpr int kThreads = (kConvert + kConvertWarps) * 32;
   static constexpr int kItemRows = kTiles * kM;
   // f16 weights are lifted by 2^7, to below 2^15 (kSlack), so that they are exact to 11 bits down
   // to 2^-21 of the row's largest and end at 2^-32 of it
   static constexpr float kLift = KV8 ? 7.0f : 0.0f;
+  // Of four pairs of exponentials, those that go to the FP32 pipe: a piece of 32 columns takes two
+  // warps of a scheduler 486 clocks with one, 562 with none, 532 with two (prompt of 8192: 542
+  // us, 557, 557).  256-dim heads and FP8 caches wait for other things: none (1-2% better).
+  static constexpr int kPolyOf4 = HD == 256 || KV8 ? 0 : 1;
   // tensor memory, in columns: two score buffers (P takes a buffer's first half), then O
   static constexpr int kO = 2 * kN;
   static constexpr int kOStride = HD <= 128 ? 128 : 0;       // between the tiles' O
@@ -436,12 +444,15 @@ __device__ __forceinline__ uint32_t stage_of_v(int i, int n) {
 
 template <int HD, bool KV8>
 __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>& c, uint32_t tiles,
-                          int lane) {
+                          int part, int lane) {
   using Sh = Shape<HD, KV8>;
   // the ring the copies go to: the products' own, or the bytes' that wait for conversion
   constexpr int kRing = KV8 ? Sh::kRawStages : Sh::kStages;
   constexpr int kBytes = KV8 ? Sh::kRawBytes : Sh::kStageBytes;
   constexpr int kBoxes = KV8 ? 1 : Sh::kCols / 64;  // 128-byte boxes across a row
+  // Two warps share a stage's copies: a box each of a row's two.
+  constexpr int kOwnBoxes = kBoxes / Sh::kLoaders;
+  static_assert(kOwnBoxes >= 1, "a box a warp");
   const uint32_t stages = tiles + Sh::kQBytes + (KV8 ? Sh::kStages * Sh::kStageBytes : 0);
   uint64_t* const full = KV8 ? c.raw_full : c.kv_full;
   uint64_t* const empty = KV8 ? c.raw_empty : c.kv_empty;
@@ -479,28 +490,29 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
     };
     bool bad;
     int id = look_up(0, bad);
-    // the queries
-    if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
-    ++q_uses;
-    const int tok0 = uniform(it.tok0);
-    const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
-    if (elect_one()) {
-      const uint32_t bar = smem_u32(KV8 ? &c.q_raw : &c.q_full);
-      mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
+    if (part == 0) {  // the queries
+      if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
+      ++q_uses;
+      const int tok0 = uniform(it.tok0);
+      const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
+      if (elect_one()) {
+        const uint32_t bar = smem_u32(KV8 ? &c.q_raw : &c.q_full);
+        mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
 #pragma unroll 1
-      for (int t = 0; t < filled; ++t)
+        for (int t = 0; t < filled; ++t)
 #pragma unroll 1
-        for (int k = 0; k < HD / 64; ++k)
-          tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
-                      tok0 + t * a.TB, bar);
+          for (int k = 0; k < HD / 64; ++k)
+            tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
+                        tok0 + t * a.TB, bar);
+      }
+      __syncwarp();
     }
-    __syncwarp();
 #pragma unroll 1
     for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
       bool is_v;
       int tile, half;
       stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
-      if (!is_v && half == 0) {
+      if (part == 0 && !is_v && half == 0) {
         const uint32_t mask = __ballot_sync(0xffffffffu, bad);
         if (elect_one()) {
           c.bad[tile_no % kBadRing] = mask;
@@ -529,14 +541,16 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
           row[x] = ((kv0 + tile) * kN + x * a.copy_rows) % a.B;
       }
       if (elect_one()) {
-        mbar_expect(bar, kBytes);
+        mbar_expect(bar, kBytes / Sh::kLoaders);
 #pragma unroll
         for (int x = 0; x < kN / 16; ++x) {
           if (x < copies)
 #pragma unroll
-            for (int k = 0; k < kBoxes; ++k)
-              tma_load_4d(dst + k * kChunkBytes + x * a.copy_rows * 128, map,
-                          half * Sh::kCols + 64 * k, row[x], kvh, block[x], bar);
+            for (int k = 0; k < kOwnBoxes; ++k) {
+              const int box = part * kOwnBoxes + k;
+              tma_load_4d(dst + box * kChunkBytes + x * a.copy_rows * 128, map,
+                          half * Sh::kCols + 64 * box, row[x], kvh, block[x], bar);
+            }
         }
       }
       __syncwarp();
@@ -993,6 +1007,11 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       for (int x = 0; x < Sh::kOutCols * size; x += 128)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(at_gate + x));
     }
+    // the tiles with positions before the first or behind the last that the item sees
+    const int item_lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
+    const int item_hi = min(it.pos0 + it.ntok, it.cap);
+    const int ragged_lo = item_lo % kN ? item_lo / kN : -1;
+    const int ragged_hi = item_hi > 0 && item_hi % kN ? item_hi / kN : -1;
     float sl = a.scale_log2, slack = kSlack / a.scale_log2;
     float m = -INFINITY, l = 0.0f;
     for (int j = b; j < e; ++j) {
@@ -1013,9 +1032,9 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
         if (lane == 0) mbar_arrive(smem_u32(&c.p_full[buffer][part]));
       };
       // V rows of this tile that no row of the item sees, in copies that hold others it does
-      const int z_lo = (a.window ? max(0, it.pos0 - a.window + 1) : 0) - j * kN;
-      const int z_hi = min(it.pos0 + it.ntok, it.cap) - j * kN;
-      if (!KV8 && (z_lo > 0 || z_hi < kN)) {  // (the conversion sees to it)
+      if (!KV8 && (j == ragged_lo || j == ragged_hi)) {  // (FP8: the conversion sees to it)
+        const int z_lo = (a.window ? max(0, it.pos0 - a.window + 1) : 0) - j * kN;
+        const int z_hi = min(it.pos0 + it.ntok, it.cap) - j * kN;
         const int i = j - it.kv0;  // the tile's place in the piece, and so its V stages
         const uint32_t v_no = stage_no + stage_of_v<HD, KV8>(i, it.kvn);
         const int r1 = z_lo > 0 ? (z_lo & ~(a.copy_rows - 1)) : 0, r2 = max(z_lo, 0);
@@ -1129,10 +1148,15 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
           get_scores(x, s);
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
+            const uint64_t z = fma2(pair(s[y], s[y + 1]), sl2, ref2);
             float p0, p1;
-            split(fma2(pair(s[y], s[y + 1]), sl2, ref2), p0, p1);
-            p0 = exp2_approx(p0);
-            p1 = exp2_approx(p1);
+            if (y / 2 % 4 < Sh::kPolyOf4) {
+              exp2_poly2(z, p0, p1);
+            } else {
+              split(z, p0, p1);
+              p0 = exp2_approx(p0);
+              p1 = exp2_approx(p1);
+            }
             sums[y / 2 & 1] = add2(sums[y / 2 & 1], pair(p0, p1));
             p[y / 2] = KV8 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
           }
@@ -1308,7 +1332,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
   grid_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < Sh::kStages; ++i) {
-      mbar_init(smem_u32(&c.kv_full[i]), KV8 ? Sh::kConvertWarps : 1);
+      mbar_init(smem_u32(&c.kv_full[i]), KV8 ? Sh::kConvertWarps : Sh::kLoaders);
       mbar_init(smem_u32(&c.kv_empty[i]), 1);
     }
     for (int i = 0; i < Sh::kRawStages; ++i) {
@@ -1326,7 +1350,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
     }
     for (int i = 0; i < kQueue; ++i) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + 2 + Sh::kConvertWarps);
+      mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + Sh::kLoaders + 1 + Sh::kConvertWarps);
     }
     mbar_init(smem_u32(&c.drained), 1);
     c.abort = 0;
@@ -1345,8 +1369,8 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
   if (warp < Sh::kSoftmaxWarps) {
     softmax_role<HD, KV8>(a, c, tiles, warp, lane);
   } else {
-    if (warp == Sh::kLoadWarp) {
-      load_role<HD, KV8>(a, maps, c, tiles, lane);
+    if (warp < Sh::kLoadWarp + Sh::kLoaders) {
+      load_role<HD, KV8>(a, maps, c, tiles, Sh::kLoaders == 1 ? 0 : warp - Sh::kLoadWarp, lane);
     } else if (warp == Sh::kMmaWarp) {
       mma_items<HD, KV8>(a, c, tiles);
       // one lane issued every product: it is the one elected here too
