@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 #include <limits.h>
 #include <math.h>
+#include <stddef.h>
 #include <string.h>
 
 #include <cudaTypedefs.h>
@@ -218,15 +219,17 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile i
   return true;
 }
 // A whole warp's wait, the same answer in every lane.
-__device__ __forceinline__ bool wait_warp(const uint64_t& bar, uint32_t parity, int* abort,
-                                          uint32_t* err) {
-  const uint32_t b = smem_u32(&bar);
+__device__ __forceinline__ bool wait_bar(uint32_t b, uint32_t parity, int* abort, uint32_t* err) {
   bool ok = mbar_try(b, parity);
   if (!__all_sync(0xffffffffu, ok)) {
     if (!ok) ok = wait_slow(b, parity, abort, err);
     return __all_sync(0xffffffffu, ok);
   }
   return true;
+}
+__device__ __forceinline__ bool wait_warp(const uint64_t& bar, uint32_t parity, int* abort,
+                                          uint32_t* err) {
+  return wait_bar(smem_u32(&bar), parity, abort, err);
 }
 
 // The cache tiles that rows at positions [p0, p0 + n) see: their number and the first.
@@ -695,17 +698,23 @@ __host__ __device__ constexpr int weight_column(int x) {
 }
 
 // ---- products ----
+// One warp, and the path that paces the kernel: each of its instructions delays both tiles (the
+// product loops rolled up, say, cost 17%).  So barriers are plain addresses, descriptors one
+// addition a product, and what needs no wait between shares an elected block.
 template <int HD, bool KV8>
 __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tiles) {
   using Sh = Shape<HD, KV8>;
+  using C = Control<HD, KV8>;
   const uint32_t tmem = uniform(c.tmem), stages = tiles + Sh::kQBytes;
+  const uint32_t control = tiles + Sh::kTileBytes;
   constexpr uint32_t kScores = instruction(!KV8, false, kM, kN);
   constexpr uint32_t kSum = instruction(!KV8, true, kM, Sh::kCols);
   int stage = 0, queued = 0;
   uint32_t phase = 0, q_phase = 0, p_phase = 0, p_count = 0, buffers = 0;
+#define BAR(field, i) (control + uint32_t(offsetof(C, field)) + 8 * (i))
 #define WAIT(bar, parity) \
-  if (!wait_warp(bar, parity, &c.abort, a.err)) return false
-  auto wait_stage = [&]() { return wait_warp(c.kv_full[stage], phase, &c.abort, a.err); };
+  if (!wait_bar(bar, parity, &c.abort, a.err)) return false
+  auto wait_stage = [&]() { return wait_bar(BAR(kv_full, stage), phase, &c.abort, a.err); };
   auto take = [&]() {
     const int was = stage;
     if (++stage == Sh::kStages) {
@@ -714,151 +723,160 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
     }
     return was;
   };
+  // By the elected lane: S (+)= Q K^T over one stage's columns.
   auto scores = [&](int t, int buffer, int st, int half, bool add) {
-    const uint32_t q = tiles + (t * (HD / 64) + half * (Sh::kCols / 64)) * kChunkBytes;
-    const uint32_t k = stages + st * Sh::kStageBytes;
-    const uint64_t q_desc = desc_k_major(q), k_desc = desc_k_major(k);
-    if (elect_one()) {
+    const uint32_t q = desc_k_major(tiles + (t * (HD / 64) + half * (Sh::kCols / 64)) * kChunkBytes);
+    const uint32_t k = desc_k_major(stages + st * Sh::kStageBytes);
 #pragma unroll
-      for (int x = 0; x < Sh::kCols / 64; ++x)
+    for (int x = 0; x < Sh::kCols / 64; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint64_t step = (x * kChunkBytes + 32 * y) >> 4;
-          mma_ss(tmem + buffer * kN, q_desc + step, k_desc + step, kScores, add || x + y > 0);
-        }
-    }
-    __syncwarp();
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t step = (x * kChunkBytes + 32 * y) >> 4;
+        mma_ss(tmem + buffer * kN, q + step, k + step, kScores, x + y > 0 ? 1u : uint32_t(add));
+      }
   };
-  // A part of a tile's positions: the same part of each softmax warpgroup's.
+  // By the elected lane: O += P V for a part of a tile's positions, the same part of each softmax
+  // warpgroup's.
   auto sum = [&](int o_col, int buffer, int st, int part, bool add) {
     constexpr int kSteps = Sh::kPartCols / 16;
     const uint32_t weights = tmem + buffer * kN + 8 * kSteps * part;
-    const uint64_t v_desc = desc_mn_major(stages + st * Sh::kStageBytes, kChunkBytes) +
-                            (part * kSteps * 16 * 128 >> 4);
-    if (elect_one()) {
+    const uint32_t v = desc_mn_major(stages + st * Sh::kStageBytes, kChunkBytes) +
+                       (part * kSteps * 16 * 128 >> 4);
 #pragma unroll
-      for (int i = 0; i < kSteps * Sh::kShares; ++i) {
-        const int x = i / kSteps * (Sh::kScoreCols / 16) + i % kSteps;  // in part 0
-        mma_ts(tmem + o_col, weights + weight_column<HD, KV8>(x), v_desc + (x * 16 * 128 >> 4), kSum,
-               add || part + i > 0);
-      }
+    for (int i = 0; i < kSteps * Sh::kShares; ++i) {
+      const int x = i / kSteps * (Sh::kScoreCols / 16) + i % kSteps;  // in part 0
+      mma_ts(tmem + o_col, weights + weight_column<HD, KV8>(x), v + (x * 16 * 128 >> 4), kSum,
+             part + i > 0 ? 1u : uint32_t(add));
     }
-    __syncwarp();
-  };
-  auto commit = [&](const uint64_t& bar) {
-    if (elect_one()) mma_commit(smem_u32(&bar));
-    __syncwarp();
   };
   for (;;) {
     const int at = queued % kQueue;
-    WAIT(c.item_full[at], (queued / kQueue) & 1);
+    WAIT(BAR(item_full, at), (queued / kQueue) & 1);
     const Item it = c.items[at];
     __syncwarp();
-    if (elect_one()) mbar_arrive(smem_u32(&c.item_empty[at]));
+    if (elect_one()) mbar_arrive(BAR(item_empty, at));
     ++queued;
     if (uniform(it.flags) & kItemEnd) return true;
     const int kvn = uniform(it.kvn);
     if (!kvn) continue;
     const int j0 = uniform(it.kv0), j1 = j0 + kvn;
-    WAIT(c.q_full, q_phase);
+    WAIT(BAR(q_full, 0), q_phase);
     q_phase ^= 1;
     if constexpr (Sh::kTiles == 2) {
-      int b0, b1, e0, e1;
-      tile_range<HD, KV8>(a, it, 0, b0, e0);
-      tile_range<HD, KV8>(a, it, 1, b1, e1);
-      b0 = uniform(b0);
-      b1 = uniform(b1);
-      e0 = uniform(e0);
-      e1 = uniform(e1);
+      int b[2], e[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        tile_range<HD, KV8>(a, it, t, b[t], e[t]);
+        b[t] = uniform(b[t]);
+        e[t] = uniform(e[t]);
+      }
       if (!wait_stage()) return false;
       tc_fence_after();
       int k_st = take();
-#pragma unroll 1
-      for (int t = 0; t < 2; ++t)
-        if ((t ? b1 : b0) <= j0 && j0 < (t ? e1 : e0)) {
-          scores(t, t, k_st, 0, false);
-          commit(c.s_full[t]);
-        }
-      commit(c.kv_empty[k_st]);
-      if (j0 + 1 == j1) commit(c.q_empty);
+      if (elect_one()) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (b[t] <= j0 && j0 < e[t]) {
+            scores(t, t, k_st, 0, false);
+            mma_commit(BAR(s_full, t));
+          }
+        mma_commit(BAR(kv_empty, k_st));
+        if (j0 + 1 == j1) mma_commit(BAR(q_empty, 0));
+      }
       for (int j = j0; j < j1; ++j) {
         if (!wait_stage()) return false;
         const int v_st = take();
         const bool more = j + 1 < j1;
         k_st = -1;
-#pragma unroll 1
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int b = t ? b1 : b0, e = t ? e1 : e0;
-          if (b <= j && j < e) {
-#pragma unroll 1
-            for (int part = 0; part < Sh::kParts; ++part) {
-              WAIT(c.p_full[t][part], p_phase >> t & 1);
+          const bool now = b[t] <= j && j < e[t];
+          const bool next = more && b[t] <= j + 1 && j + 1 < e[t];
+          if (now) {
+#pragma unroll
+            for (int part = 0; part + 1 < Sh::kParts; ++part) {
+              WAIT(BAR(p_full, 2 * t + part), p_phase >> t & 1);
               tc_fence_after();
-              sum(Sh::kO + t * Sh::kOStride, t, v_st, part, j > b);
+              if (elect_one()) sum(Sh::kO + t * Sh::kOStride, t, v_st, part, j > b[t]);
             }
-            p_phase ^= 1u << t;
-            if (j + 1 == e) commit(c.o_full[t]);
           }
-          if (more && b <= j + 1 && j + 1 < e) {
-            if (k_st < 0) {
-              if (!wait_stage()) return false;
-              tc_fence_after();
-              k_st = take();
-            }
-            scores(t, t, k_st, 0, false);
-            commit(c.s_full[t]);
-          }
-        }
-        commit(c.kv_empty[v_st]);
-        if (more) {
-          if (k_st < 0) {  // a tile of positions between the two tiles' windows
+          if (next && k_st < 0) {  // ahead of the wait for the last weights
             if (!wait_stage()) return false;
             k_st = take();
           }
-          commit(c.kv_empty[k_st]);
-          if (j + 2 == j1) commit(c.q_empty);
+          if (now) {
+            WAIT(BAR(p_full, 2 * t + Sh::kParts - 1), p_phase >> t & 1);
+            p_phase ^= 1u << t;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            if (now) {
+              sum(Sh::kO + t * Sh::kOStride, t, v_st, Sh::kParts - 1, j > b[t]);
+              if (j + 1 == e[t]) mma_commit(BAR(o_full, t));
+            }
+            if (next) {
+              scores(t, t, k_st, 0, false);
+              mma_commit(BAR(s_full, t));
+            }
+          }
+        }
+        if (more && k_st < 0) {  // a tile of positions between the two tiles' windows
+          if (!wait_stage()) return false;
+          k_st = take();
+        }
+        if (elect_one()) {
+          mma_commit(BAR(kv_empty, v_st));
+          if (more) mma_commit(BAR(kv_empty, k_st));
+          if (j + 2 == j1) mma_commit(BAR(q_empty, 0));
         }
       }
     } else {
       auto next_scores = [&]() {
+#pragma unroll
         for (int h = 0; h < Sh::kHalves; ++h) {
           if (!wait_stage()) return false;
           tc_fence_after();
           const int st = take();
-          scores(0, buffers & 1, st, h, h > 0);
-          commit(c.kv_empty[st]);
+          if (elect_one()) {
+            scores(0, buffers & 1, st, h, h > 0);
+            mma_commit(BAR(kv_empty, st));
+            if (h + 1 == Sh::kHalves) mma_commit(BAR(s_full, buffers & 1));
+          }
         }
-        commit(c.s_full[buffers & 1]);
         ++buffers;
         return true;
       };
       if (!next_scores()) return false;
       for (int j = j0; j < j1; ++j) {
         if (j + 1 < j1 && !next_scores()) return false;
-        if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1)) commit(c.q_empty);
+        if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1))
+          if (elect_one()) mma_commit(BAR(q_empty, 0));
         const int buffer = p_count & 1;
         const uint32_t parity = (p_count++ >> 1) & 1;
         int v_st[Sh::kHalves];
 #pragma unroll
-        for (int part = 0; part < Sh::kParts; ++part) {
-          WAIT(c.p_full[buffer][part], parity);
-          tc_fence_after();
+        for (int h = 0; h < Sh::kHalves; ++h) {
+          if (!wait_stage()) return false;
+          v_st[h] = take();
+        }
 #pragma unroll
-          for (int h = 0; h < Sh::kHalves; ++h) {
-            if (part == 0) {
-              if (!wait_stage()) return false;
-              tc_fence_after();
-              v_st[h] = take();
+        for (int part = 0; part < Sh::kParts; ++part) {
+          WAIT(BAR(p_full, 2 * buffer + part), parity);
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < Sh::kHalves; ++h) {
+              sum(Sh::kO + h * Sh::kCols, buffer, v_st[h], part, j > j0);
+              if (part + 1 == Sh::kParts) mma_commit(BAR(kv_empty, v_st[h]));
             }
-            sum(Sh::kO + h * Sh::kCols, buffer, v_st[h], part, j > j0);
-            if (part + 1 == Sh::kParts) commit(c.kv_empty[v_st[h]]);
+            if (part + 1 == Sh::kParts) mma_commit(BAR(o_full, buffer));
           }
         }
-        commit(c.o_full[buffer]);
       }
     }
   }
 #undef WAIT
+#undef BAR
 }
 
 // ---- softmax ----
@@ -1370,7 +1388,8 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
     softmax_role<HD, KV8>(a, c, tiles, warp, lane);
   } else {
     if (warp < Sh::kLoadWarp + Sh::kLoaders) {
-      load_role<HD, KV8>(a, maps, c, tiles, Sh::kLoaders == 1 ? 0 : warp - Sh::kLoadWarp, lane);
+      load_role<HD, KV8>(a, maps, c, tiles, Sh::kLoaders == 1 ? 0 : uniform(warp - Sh::kLoadWarp),
+                         lane);
     } else if (warp == Sh::kMmaWarp) {
       mma_items<HD, KV8>(a, c, tiles);
       // one lane issued every product: it is the one elected here too

@@ -184,34 +184,37 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 //     elements further along the contraction are 32 bytes further in the row.
 //   MN-major (the contraction runs down the rows): atoms of eight contraction steps 1,024 bytes
 //     apart, the next 64 columns `next_columns` bytes away.
-constexpr uint64_t kDescBase = (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-  return kDescBase | (uint64_t(1) << 16) | uint64_t(addr >> 4);
-}
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t next_columns) {
-  return kDescBase | (uint64_t(next_columns >> 4) << 16) | uint64_t(addr >> 4);
+// A descriptor's high word is the same for both (eight-row stride, version, swizzle); in the low
+// word, stepping through a tile is an addition.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(uint32_t addr) { return (1u << 16) | (addr >> 4); }
+__device__ __forceinline__ uint32_t desc_mn_major(uint32_t addr, uint32_t next_columns) {
+  return (next_columns >> 4 << 16) | (addr >> 4);
 }
 // FP32 accumulator, A and B both bf16 (or both f16), M x N; B K-major or MN-major.
 __host__ __device__ constexpr uint32_t instruction(bool bf16, bool b_mn_major, int m, int n) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
          ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
-// D [tensor memory] (+)= A [shared memory] B [shared memory]; one thread issues it.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+// D [tensor memory] (+)= A [shared memory] B [shared memory]; one thread issues it.  A constant
+// `add` costs no instruction.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                       uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add)
       : "memory");
 }
 // D [tensor memory] (+)= A [tensor memory: a row a lane, two elements a column] B [shared memory].
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                       uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(add)
       : "memory");
 }
 // One arrival on `bar` when every product this thread has issued is complete.
