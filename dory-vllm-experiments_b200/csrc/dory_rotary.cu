@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
         split(squares, sum, other);
         sum += other;
         for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-        if (!is_v) {
+        if (!is_v && known) {  // zeros stay zeros, whatever eps
           const float inv = rsqrtf(sum + a.eps);
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = mul2(y[j], mul2(weight[j], pair(inv, inv)));
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(128) rotary_any(const RotaryArgs a) {
         sum += y * y;
       }
       for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-      inv = rsqrtf(sum + a.eps);
+      if (inside) inv = rsqrtf(sum + a.eps);
     }
     if (h >= a.NH && slot < 0) return;
     const int g = is_v ? h - a.NH - a.NKV : h - a.NH;

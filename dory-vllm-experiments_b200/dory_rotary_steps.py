@@ -162,8 +162,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                  error_word: torch.Tensor | None = None) -> None:
     """Rotates q [T, NH, D] and k [T, NKV, D] (or None) by the angles of positions [T] (int64
     or int32) into q_out and k_out, same shapes and type (BF16, FP16 or FP32); an output may be
-    its own input itself, otherwise it must lie apart from it.  Any token and head strides,
-    unit last stride.  cos_sin [max_position, rotary_dim]: the first rotary_dim dims turn, pairs
+    its own input itself, otherwise it must lie apart from it; the outputs lie apart from each
+    other and from the other's input.  Any token and head strides, unit last stride.  cos_sin [max_position, rotary_dim]: the first rotary_dim dims turn, pairs
     (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1); the others are copied.  inverse: the
     rotation back.  error_word (optional int32 device tensor) collects
     DORY_DEVERR_POSITION_OOB; such a token's outputs are zero."""

@@ -288,3 +288,19 @@ def test_captured_and_on_another_stream():
     slots.copy_(torch.arange(T, device=DEV).flip(0))
     graph.replay()
     assert torch.equal(out, first.flip(0)) and torch.equal(raw, rows)
+
+
+@pytest.mark.parametrize("D,R", [(128, 128), (64, 24)])  # the wide kernel, and the general one
+def test_an_unknown_position_appends_zeros_whatever_eps(D, R):
+    q, k, v = (torch.randn(1, n, D, device=DEV) for n in (4, 2, 2))
+    key = torch.full((2, 16, 2, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    value = key.clone()
+    q_out = torch.full((1, 4, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    rotary_append(q, k, v, torch.tensor([9], device=DEV), rotary_cos_sin(8, R, device=DEV),
+                  torch.tensor([17], device=DEV), key, value, q_out,
+                  sqk=torch.ones(4 * D, device=DEV), eps=0.0, error_word=word)
+    assert word.item() == _native.DEVERR_POSITION_OOB
+    assert (q_out == 0).all() and (key[1, 1] == 0).all()
+    assert torch.equal(value[1, 1], v[0].to(torch.bfloat16))
+    assert (key[0] == 5.0).all() and (key[1, 2:] == 5.0).all()
