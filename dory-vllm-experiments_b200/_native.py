@@ -29,11 +29,12 @@ QKNORM_WRITE_CACHE = 1
 ROTARY_INTERLEAVED, ROTARY_INVERSE, ROTARY_NORM = 1, 2, 4
 # DORY_DEVERR_*
 DEVERR_BLOCK_OOB, DEVERR_SLOT_OOB, DEVERR_OFFSET_ALIGN, DEVERR_WAIT_TIMEOUT = 1, 2, 4, 8
-DEVERR_POSITION_OOB = 16
+DEVERR_POSITION_OOB, DEVERR_QUERY_START = 16, 32
 DEVERR_NAMES = {DEVERR_BLOCK_OOB: "block id out of range", DEVERR_SLOT_OOB: "slot out of range",
                 DEVERR_OFFSET_ALIGN: "cache offset not 16-byte aligned",
                 DEVERR_WAIT_TIMEOUT: "pipeline wait timed out",
-                DEVERR_POSITION_OOB: "rotary position outside the cos/sin table"}
+                DEVERR_POSITION_OOB: "rotary position outside the cos/sin table",
+                DEVERR_QUERY_START: "query_start decreases or leaves the batch"}
 
 # Every symbol include/dory_decode.h declares (checked by the CPU test suite).
 EXPORTS = ("dory_decode_abi_version", "dory_decode_params_bytes", "dory_decode_scratch_bytes",

@@ -16,11 +16,11 @@
 //   scheduler  derives the SM's piece from query_start / seq_lens on the device (no host read,
 //              so a captured graph follows new lengths) and hands items to the others;
 //   loader     tensor copies: the queries, and K and V tiles page by page through the block
-//              table into a ring; pages outside the item's positions, and bad block ids, load
-//              as zeros without touching memory;
+//              table into a ring (256-dim bf16 heads: two warps); pages outside the item's
+//              positions, and bad block ids, load as zeros without touching memory;
 //   conversion (FP8 caches, four warps) e4m3 tiles to f16 tiles, bf16 queries to scaled f16 ones;
 //   products   tcgen05: S = Q K^T into tensor memory, O += P V with P read from there;
-//   softmax    four warpgroups, a half (256-dim heads: a quarter) of a row per thread: scores to
+//   softmax    two warpgroups, a row (256-dim heads: half a row) per thread: scores to
 //              registers, running maximum, exponentials, P back to tensor memory as 16-bit
 //              floats, and at the end of an item O / sum, gate and store.
 // With 64/128-dim heads an item has two tiles and the products of one overlap the softmax of
@@ -40,6 +40,7 @@
 #include <limits.h>
 #include <math.h>
 #include <stddef.h>
+#include <stdint.h>
 #include <string.h>
 
 #include <cudaTypedefs.h>
@@ -64,7 +65,7 @@ constexpr int kQueue = 4;            // items handed out ahead
 constexpr int kBadRing = 16;         // tiles whose bad-page masks are kept
 constexpr int kMaxPosition = 1 << 30;
 constexpr float kSlack = 8.0f;       // log2 a row's maximum may grow before O is rescaled
-// ~2 s, then give up: above a whole item of redo_row, which the other roles wait for.
+// ~2 s without a row of redo_row done meanwhile (the other roles wait for those), then give up.
 constexpr long long kWaitLimitCycles = 4000000000LL;
 
 struct ChunkArgs {
@@ -200,18 +201,25 @@ struct Control {  // shared memory behind the tiles
   // reach while softmax warps are still at the output of the item before
   float q_scale[2][KV8 ? Shape<HD, KV8>::kItemRows : 1];
   uint32_t tmem;
-  int abort;
+  int abort, redone;  // redone: counts the rows of redo_row
   // a row's maxima and sums, by share
   float swap[Shape<HD, KV8>::kTiles][Shape<HD, KV8>::kShares][Shape<HD, KV8>::kShares > 1 ? kM : 1];
 };
 
+// abort: Control's abort and redone.
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
                                        uint32_t* err) {
-  const long long start = clock64();
+  long long start = clock64();
+  int redone = abort[1];
   while (!mbar_try(bar, parity)) {
-    if (*abort) return false;
+    if (abort[0]) return false;
     if (clock64() - start > kWaitLimitCycles) {
-      *abort = 1;
+      if (redone != abort[1]) {
+        redone = abort[1];
+        start = clock64();
+        continue;
+      }
+      abort[0] = 1;
       atomicOr(err, DORY_DEVERR_WAIT_TIMEOUT);
       return false;
     }
@@ -331,7 +339,17 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
 
   int total = 0, mine = 0;
   for (int base = 0; base < a.S; base += 32) {
-    mine = head_units(a, sequence(a, base + lane), tokens, lane) * a.NKV;
+    const int i = base + lane;
+    // rows that two sequences own, or that are not there: nothing is done (nor do the units, 32
+    // bits for disjoint rows, overflow)
+    const bool broken = i < a.S && (a.query_start[i] < 0 || a.query_start[i + 1] > a.T ||
+                                    a.query_start[i] > a.query_start[i + 1]);
+    if (__any_sync(0xffffffffu, broken)) {
+      if (cta == 0 && lane == 0) atomicOr(a.err, DORY_DEVERR_QUERY_START);
+      total = 0;
+      break;
+    }
+    mine = head_units(a, sequence(a, i), tokens, lane) * a.NKV;
     total += __reduce_add_sync(0xffffffffu, mine);
   }
   const int per = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_units);
@@ -1334,6 +1352,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       __syncwarp();
       redo_row<HD, KV8>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
       __syncwarp();
+      if (lane == 0) atomicAdd(&c.redone, 1);
     }
     done();
   }
@@ -1371,7 +1390,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
       mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + Sh::kLoaders + 1 + Sh::kConvertWarps);
     }
     mbar_init(smem_u32(&c.drained), 1);
-    c.abort = 0;
+    c.abort = c.redone = 0;
     fence_mbar_init();
     fence_async_smem();
   }
@@ -1549,6 +1568,12 @@ bool encode(CUtensorMap* map, const void* base, int esize, int rank, const int64
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whether n elements of `size` bytes from a and m from b share memory.
+bool meet(const void* a, int64_t n, int size, const void* b, int64_t m, int b_size) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + uintptr_t(m * b_size) && y < x + uintptr_t(n * size);
+}
+
 template <int HD, bool KV8>
 int32_t launch(const ChunkArgs& a, const Maps& maps, int device, int ctas, cudaStream_t stream) {
   using Sh = Shape<HD, KV8>;
@@ -1624,19 +1649,32 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   if (!p.q || !p.key_cache || !p.value_cache || !p.block_tables || !p.query_start ||
       !p.seq_lens || !p.out || !p.scratch)
     return fail(DORY_ERR_INVALID_ARGUMENT, "null tensor argument");
+  // The stride of a dimension of one element is not used.
+  const int64_t q_t = p.num_tokens > 1 ? p.q_stride_token : 0;
+  const int64_t out_t = p.num_tokens > 1 ? p.out_stride_token : 0;
+  const int64_t gate_t = p.num_tokens > 1 ? p.gate_stride_token : 0;
+  const int64_t q_h = p.num_heads > 1 ? p.q_stride_head : 0;
+  const int64_t sb = p.num_cache_blocks > 1 ? p.stride_block : 0;
+  const int64_t sh = p.num_kv_heads > 1 ? p.stride_head : 0;
   const int64_t cache_mask = kv8 ? 15 : 7;
-  if (!aligned16(p.q) || !aligned16(p.out) || ((p.q_stride_token | p.q_stride_head) & 7) ||
-      (p.out_stride_token & 7))
+  if (!aligned16(p.q) || !aligned16(p.out) || ((q_t | q_h) & 7) || (out_t & 7))
     return fail(DORY_ERR_ALIGNMENT, "q and out need 16-byte aligned bases and rows");
   if (!aligned16(p.key_cache) || !aligned16(p.value_cache) ||
-      ((p.stride_block | p.stride_offset | p.stride_head) & cache_mask))
+      ((sb | p.stride_offset | sh) & cache_mask))
     return fail(DORY_ERR_ALIGNMENT, "key/value caches need 16-byte aligned bases and strides");
-  if (p.gate && (!aligned16(p.gate) || (p.gate_stride_token & 7)))
+  if (p.gate && (!aligned16(p.gate) || (gate_t & 7)))
     return fail(DORY_ERR_ALIGNMENT, "gate needs a 16-byte aligned base and rows");
   const int64_t need = dory_chunk_scratch_bytes(p.num_heads, p.num_kv_heads, p.head_dim);
   if (p.scratch_bytes < need)
     return fail(DORY_ERR_INVALID_ARGUMENT, "scratch too small (%lld < %lld bytes)",
                 (long long)p.scratch_bytes, (long long)need);
+  // A row may be computed again (redo_row) after others, and a part of itself, have been stored.
+  const int64_t width = int64_t(p.num_heads) * p.head_dim, last = p.num_tokens - 1;
+  const int gate_size = p.gate_dtype == DORY_DTYPE_F32 ? 4 : 2;
+  if (meet(p.out, last * out_t + width, 2, p.q,
+           last * q_t + (p.num_heads - 1) * q_h + p.head_dim, 2) ||
+      (p.gate && meet(p.out, last * out_t + width, 2, p.gate, last * gate_t + width, gate_size)))
+    return fail(DORY_ERR_INVALID_ARGUMENT, "out must lie apart from q and gate");
 
   ChunkArgs a;
   memset(&a, 0, sizeof(a));
@@ -1649,14 +1687,14 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   a.gate = p.gate;
   a.out = static_cast<__nv_bfloat16*>(p.out);
   a.err = static_cast<uint32_t*>(p.scratch);
-  a.q_t = p.q_stride_token;
-  a.q_h = p.q_stride_head;
-  a.out_t = p.out_stride_token;
-  a.gate_t = p.gate_stride_token;
+  a.q_t = q_t;
+  a.q_h = q_h;
+  a.out_t = out_t;
+  a.gate_t = gate_t;
   a.table_stride = p.table_stride;
-  a.sb = p.stride_block;
+  a.sb = sb;
   a.so = p.stride_offset;
-  a.sh = p.stride_head;
+  a.sh = sh;
   a.blocks = p.num_cache_blocks;
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.k_scale = p.k_scale;
@@ -1693,10 +1731,10 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   a.part_o = reinterpret_cast<float*>(scratch + layout.o);
   Maps maps;
   const int64_t q_dims[3] = {p.head_dim, p.num_heads, p.num_tokens};
-  const int64_t q_strides[3] = {1, p.q_stride_head, p.q_stride_token};
+  const int64_t q_strides[3] = {1, q_h, q_t};
   const int q_box[3] = {64, G, a.TB};
   const int64_t c_dims[4] = {p.head_dim, p.block_size, p.num_kv_heads, p.num_cache_blocks};
-  const int64_t c_strides[4] = {1, p.stride_offset, p.stride_head, p.stride_block};
+  const int64_t c_strides[4] = {1, p.stride_offset, sh, sb};
   const int esize = kv8 ? 1 : 2;
   const int c_box[4] = {128 / esize, a.copy_rows, 1, 1};
   if (!encode(&maps.q, p.q, 2, 3, q_dims, q_strides, q_box) ||

@@ -73,7 +73,9 @@ class ChunkAttention:
         query_start[i + 1] - 1 of q; seq_lens: int32 [S], positions including those rows (0:
         a padded request, zero rows); window: 0 for all earlier positions; gate: FP32, BF16 or
         FP16 [T, heads * head_dim] (e.g. post-sigmoid) or None; out: BF16 [T, heads *
-        head_dim].  Rows that no sequence owns keep what out held."""
+        head_dim], whose span of memory lies apart from those of q and gate.  Rows that no
+        sequence owns keep what out held.  A query_start that decreases or leaves [0, T] is
+        reported (check_errors) and nothing is written."""
         heads, dim, dev = self.num_heads, self.head_dim, self._dev_index
         if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
             raise ValueError("q and out must be bfloat16")

@@ -81,8 +81,10 @@ enum {
   DORY_DEVERR_SLOT_OOB = 2u,      /* an append slot outside the cache                     */
   DORY_DEVERR_OFFSET_ALIGN = 4u,  /* a cache offset not a multiple of 8 elements          */
   DORY_DEVERR_WAIT_TIMEOUT = 8u,  /* a pipeline wait gave up after its iteration limit    */
-  DORY_DEVERR_POSITION_OOB = 16u  /* a rotary position outside [0, max_position); that token's
+  DORY_DEVERR_POSITION_OOB = 16u, /* a rotary position outside [0, max_position); that token's
                                    * q and k are zero                                       */
+  DORY_DEVERR_QUERY_START = 32u   /* a chunk call's query_start decreases or leaves [0, T]:
+                                   * the call wrote nothing                                 */
 };
 
 /*
@@ -452,7 +454,8 @@ typedef struct DoryChunkParams {
   const int32_t* query_start;     /* int32 [S + 1], not decreasing, within [0, T]            */
   const int32_t* seq_lens;        /* int32 [S]: positions including the chunk's own          */
   const void* gate;               /* optional [T, NH * HD] of gate_dtype                     */
-  void* out;                      /* BF16 [T, NH * HD], 16-byte aligned rows                 */
+  void* out;                      /* BF16 [T, NH * HD], 16-byte aligned rows; apart from q and
+                                   * gate                                                    */
   void* scratch;                  /* dory_chunk_scratch_bytes(), zeroed once by
                                    * dory_decode_scratch_init(); word 0 is the error word
                                    * (dory_decode_fetch_errors); calls that can overlap on the

@@ -76,6 +76,8 @@ FP8 = _native.DTYPE_FP8_E4M3
     (dict(stride_block=4), _native.ERR_ALIGNMENT, "16-byte"),
     (dict(gate=0x1004), _native.ERR_ALIGNMENT, "16-byte"),
     (dict(scratch_bytes=16), _native.ERR_INVALID_ARGUMENT, "scratch too small"),
+    (dict(out=0x1000 + 2 * 3 * 4096), _native.ERR_INVALID_ARGUMENT, "apart"),  # q's last row
+    (dict(out=0x1000000, gate=0x1000000 + 2 * 3 * 4096 + 16), _native.ERR_INVALID_ARGUMENT, "apart"),
 ])
 def test_host_validation(lib, kw, status, message):
     p = params(**kw)

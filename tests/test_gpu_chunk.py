@@ -220,8 +220,44 @@ def test_hidden_rows_may_hold_anything(bad, D, window):
     assert out[clean].isfinite().all()
     off, tol = (out - want)[clean].abs(), (2.0 ** -6 * size + 1e-6)[clean]
     assert (off <= tol).all()
-    assert not out[~clean].isfinite().any() or bad != bad or True
     assert (out[want.isnan()].isnan()).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(20, 200)], [(1, 3000)]])  # whole items, and parts joined
+def test_a_visible_nan_key_reaches_its_rows(D, lens):
+    """Wherever in a tile the position lies."""
+    b = Batch(lens, D=D, seed=31)
+    clean = b.run().clone().view(b.T, b.NH, D)
+    groups = b.NH // b.NKV
+    for pos in list(range(100, 117)) + [0, 33, 63, 64, 127, 128]:
+        row = b.key[b.tables[0, pos // 16].long(), pos % 16, 1]
+        kept = row.clone()
+        row[5] = float("nan")
+        out = b.run().view(b.T, b.NH, D)
+        assert out[:, groups:].isnan().all(), pos
+        assert torch.equal(out[:, :groups], clean[:, :groups])
+        row.copy_(kept)
+
+
+def test_a_single_token_of_any_stride():
+    b = Batch([(1, 90)], NH=4, NKV=1, seed=32)
+    want = b.run(gate=b.gate).clone()
+    q = b.q.as_strided((1, 4, 128), (4 * 128 + 1, 128, 1))
+    gate, out = (x.as_strided(x.shape, (x.shape[1] + 3, 1)) for x in (b.gate, b.out))
+    b.out.fill_(5.0)
+    b.key, b.value = (c.as_strided(c.shape, (c.stride(0), c.stride(1), 1, 1))
+                      for c in (b.key, b.value))
+    assert torch.equal(b.run(gate=gate, q=q, out=out), want)
+
+
+@pytest.mark.parametrize("starts", [[0, 30, 20, 40], [-1, 10, 20, 40], [0, 10, 20, 41],
+                                    [0, 40, 0, 40]])
+def test_a_broken_query_start_is_reported_and_nothing_written(starts):
+    b = Batch([(10, 50), (10, 20), (20, 20)], seed=33)
+    b.query_start.copy_(torch.tensor(starts, dtype=torch.int32))
+    out = b.run(errors=_native.DEVERR_QUERY_START)
+    assert (out == 5.0).all()
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -337,6 +373,11 @@ def test_refusals():
                dict(out=b.out.float()), dict(out=b.out[:2]), dict(gate=b.gate[:, :5]),
                dict(gate=b.gate.double()), dict(lens=b.seq_lens.cpu()), dict(gate=b.gate.cpu())):
         with pytest.raises(ValueError):
+            call(**kw)
+    flat = b.q.view(b.T, -1)
+    for kw in (dict(out=flat), dict(q=b.q[:3], out=flat[1:], gate=b.gate[:3]),
+               dict(gate=b.out)):  # rows may be read again after others have been written
+        with pytest.raises(ValueError, match="apart"):
             call(**kw)
     with pytest.raises(ValueError):  # an FP8 instance over a bf16 cache
         ChunkAttention(b.NH, b.NKV, b.D, DEV, kv_cache_dtype="fp8")(
