@@ -186,19 +186,21 @@ struct Item {
   int kvh, seq;
   int cap;           // positions of the sequence that the table names
   int slot;          // partial-result slot, -1: the whole item is here
-  int pad[6];
+  int tile;          // the tensor-core tile of its first rows: 1 only if they fill one at most
+  int pad[5];
+  __device__ int tiles(const ChunkArgs& a) const { return ntok > a.TB ? 2 : 1; }
 };
 
 template <int HD, bool KV8>
 struct Control {  // shared memory behind the tiles
   alignas(8) uint64_t kv_full[Shape<HD, KV8>::kStages], kv_empty[Shape<HD, KV8>::kStages];
-  uint64_t raw_full[4], raw_empty[4], q_raw;  // FP8 caches only
-  uint64_t q_full, q_empty, s_full[2], p_full[2][2], o_full[2], item_full[kQueue],
+  uint64_t raw_full[4], raw_empty[4], q_raw[2];  // FP8 caches only
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], item_full[kQueue],
       item_empty[kQueue], drained;
   Item items[kQueue];
   uint32_t bad[kBadRing];
-  // what a row's f16 query was divided by; a set for the item after, which the conversion may
-  // reach while softmax warps are still at the output of the item before
+  // what a row's f16 query was divided by; a second set for the tile's next item, which the
+  // conversion may reach while softmax warps are still at the output of the item before
   float q_scale[2][KV8 ? Shape<HD, KV8>::kItemRows : 1];
   uint32_t tmem;
   int abort, redone;  // redone: counts the rows of redo_row
@@ -251,8 +253,9 @@ __device__ __forceinline__ int tiles_seen(int p0, int n, int cap, int window, in
 // Those of tile t of an item within this CTA's piece: [b, e).
 template <int HD, bool KV8>
 __device__ __forceinline__ void tile_range(const ChunkArgs& a, const Item& it, int t, int& b, int& e) {
-  const int skip = t * a.TB;
-  const int n = tiles_seen(it.pos0 + skip, min(it.ntok - skip, a.TB), it.cap, a.window, b);
+  const int skip = (t - it.tile) * a.TB;
+  const int n = tiles_seen(it.pos0 + skip, skip < 0 ? 0 : min(it.ntok - skip, a.TB), it.cap,
+                           a.window, b);
   e = b + n;
   b = max(b, it.kv0);
   e = min(e, it.kv0 + it.kvn);
@@ -319,7 +322,7 @@ template <int HD, bool KV8>
 __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
   const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
   int32_t* join = a.joins + cta * 8;
-  int queued = 0;
+  int queued = 0, turn = 0;
   auto push = [&](const Item& it) {
     const int at = queued % kQueue;
     if (queued >= kQueue &&
@@ -410,6 +413,8 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
         it.seq = seq;
         it.cap = s.cap;
         it.slot = whole ? -1 : (off == 0 ? 2 * cta + 1 : 2 * cta);
+        // items of one tile's rows take the two in turn: one's output overlaps the next one
+        it.tile = Shape<HD, KV8>::kTiles == 2 && it.ntok <= a.TB ? turn ^= 1 : 0;
         if (!whole && off == 0) {
           cut = 1;
           if (lane == 0) {
@@ -478,7 +483,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
   uint64_t* const full = KV8 ? c.raw_full : c.kv_full;
   uint64_t* const empty = KV8 ? c.raw_empty : c.kv_empty;
   const int copies = kN / a.copy_rows;
-  int stage = 0, queued = 0, q_uses = 0;
+  int stage = 0, queued = 0, q_uses[2] = {0, 0};
   uint32_t phase = 1, tile_no = 0, issued = 0;  // phase of the stage's empty barrier: free at first
   bool ok = true;
   for (;;) {
@@ -512,21 +517,24 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
     bool bad;
     int id = look_up(0, bad);
     if (part == 0) {  // the queries
-      if (!(ok = wait_warp(c.q_empty, (q_uses & 1) ^ 1, &c.abort, a.err))) break;
-      ++q_uses;
-      const int tok0 = uniform(it.tok0);
-      const int filled = uniform(min(Sh::kTiles, (it.ntok + a.TB - 1) / a.TB));
-      if (elect_one()) {
-        const uint32_t bar = smem_u32(KV8 ? &c.q_raw : &c.q_full);
-        mbar_expect(bar, filled * (HD / 64) * a.TB * a.G * 128);
-#pragma unroll 1
-        for (int t = 0; t < filled; ++t)
+      const int tok0 = uniform(it.tok0), first = uniform(it.tile);
+      const int end = first + uniform(it.tiles(a));
+#pragma unroll
+      for (int t = 0; t < Sh::kTiles; ++t) {
+        if (t < first || t >= end) continue;
+        if (!(ok = wait_warp(c.q_empty[t], (q_uses[t] & 1) ^ 1, &c.abort, a.err))) break;
+        ++q_uses[t];
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(KV8 ? &c.q_raw[t] : &c.q_full[t]);
+          mbar_expect(bar, (HD / 64) * a.TB * a.G * 128);
 #pragma unroll 1
           for (int k = 0; k < HD / 64; ++k)
             tma_load_3d(tiles + (t * (HD / 64) + k) * kChunkBytes, &maps.q, 64 * k, kvh * a.G,
-                        tok0 + t * a.TB, bar);
+                        tok0 + (t - first) * a.TB, bar);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      if (!ok) break;
     }
 #pragma unroll 1
     for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
@@ -590,9 +598,11 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
       while (!mbar_try(smem_u32(&full[i % kRing]), (i / kRing) & 1) &&
              clock64() - start < 200000000LL) {
       }
-    while (q_uses && !mbar_try(smem_u32(KV8 ? &c.q_raw : &c.q_full), (q_uses - 1) & 1) &&
-           clock64() - start < 300000000LL) {
-    }
+    for (int t = 0; t < Sh::kTiles; ++t)
+      while (q_uses[t] &&
+             !mbar_try(smem_u32(KV8 ? &c.q_raw[t] : &c.q_full[t]), (q_uses[t] - 1) & 1) &&
+             clock64() - start < 300000000LL) {
+      }
   }
 }
 
@@ -620,9 +630,9 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     if (!kvn) continue;
     const int lo = a.window ? max(0, it.pos0 - a.window + 1) : 0;
     const int hi = min(it.pos0 + it.ntok, it.cap);
-    if (!wait_warp(c.q_raw, q_phase, &c.abort, a.err)) return;
 #pragma unroll 1
-    for (int t = 0; t < Sh::kTiles; ++t) {  // a row a thread, in place
+    for (int t = it.tile; t < it.tile + it.tiles(a); ++t) {  // a row a thread, in place
+      if (!wait_warp(c.q_raw[t], q_phase >> t & 1, &c.abort, a.err)) return;
       const uint32_t row = tiles + t * (HD / 64) * kChunkBytes + thread * 128;
       float top = 0.0f;
 #pragma unroll 1
@@ -649,12 +659,12 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
                           __uint_as_float(w[y] & 0xffff0000u) * scale);
         sts128(piece, w);
       }
-      c.q_scale[q_phase][t * kM + thread] = __uint_as_float(uint32_t(127 - up) << 23);
+      c.q_scale[q_phase >> t & 1][t * kM + thread] = __uint_as_float(uint32_t(127 - up) << 23);
+      q_phase ^= 1u << t;
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c.q_full[t]));
     }
-    q_phase ^= 1;
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&c.q_full));
 #pragma unroll 1
     for (int q = 0; q < 2 * Sh::kHalves * kvn; ++q) {
       if (!wait_warp(c.raw_full[raw], raw_phase, &c.abort, a.err)) return;
@@ -778,8 +788,16 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
     const int kvn = uniform(it.kvn);
     if (!kvn) continue;
     const int j0 = uniform(it.kv0), j1 = j0 + kvn;
-    WAIT(BAR(q_full, 0), q_phase);
-    q_phase ^= 1;
+    const int filled = uniform(((1 << it.tiles(a)) - 1) << it.tile);
+#pragma unroll
+    for (int t = 0; t < Sh::kTiles; ++t)
+      if (filled >> t & 1) WAIT(BAR(q_full, t), q_phase >> t & 1);
+    q_phase ^= filled;
+    auto free_queries = [&]() {  // by the elected lane, behind the item's last scores
+#pragma unroll
+      for (int t = 0; t < Sh::kTiles; ++t)
+        if (filled >> t & 1) mma_commit(BAR(q_empty, t));
+    };
     if constexpr (Sh::kTiles == 2) {
       int b[2], e[2];
 #pragma unroll
@@ -799,7 +817,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
             mma_commit(BAR(s_full, t));
           }
         mma_commit(BAR(kv_empty, k_st));
-        if (j0 + 1 == j1) mma_commit(BAR(q_empty, 0));
+        if (j0 + 1 == j1) free_queries();
       }
       for (int j = j0; j < j1; ++j) {
         if (!wait_stage()) return false;
@@ -845,7 +863,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
         if (elect_one()) {
           mma_commit(BAR(kv_empty, v_st));
           if (more) mma_commit(BAR(kv_empty, k_st));
-          if (j + 2 == j1) mma_commit(BAR(q_empty, 0));
+          if (j + 2 == j1) free_queries();
         }
       }
     } else {
@@ -868,7 +886,7 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
       for (int j = j0; j < j1; ++j) {
         if (j + 1 < j1 && !next_scores()) return false;
         if (j + 2 >= j1 && (j + 2 == j1 || j0 + 1 == j1))
-          if (elect_one()) mma_commit(BAR(q_empty, 0));
+          if (elect_one()) free_queries();
         const int buffer = p_count & 1;
         const uint32_t parity = (p_count++ >> 1) & 1;
         int v_st[Sh::kHalves];
@@ -1030,8 +1048,8 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     if (it.flags & kItemEnd) return;
     int b, e;
     tile_range<HD, KV8>(a, it, t, b, e);
-    const int tok = t * a.TB + row_tok;
-    const bool live = row_real && tok < it.ntok;
+    const int tok = (t - it.tile) * a.TB + row_tok;
+    const bool live = row_real && tok >= 0 && tok < it.ntok;
     const bool warp_live = __any_sync(0xffffffffu, live);
     const int pos = it.pos0 + tok;
     const int see_hi = min(pos, it.cap - 1), see_lo = a.window ? max(0, pos - a.window + 1) : 0;
@@ -1212,7 +1230,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       if (!kTwo) ++summed;
     }
     tiles_seen_before += it.kvn;
-    q_set ^= it.kvn > 0;  // the items that have queries
+    q_set ^= it.kvn > 0 && t >= it.tile && t < it.tile + it.tiles(a);  // the tile had queries
     stage_no += 2 * Sh::kHalves * it.kvn;
 
     // the item's rows
@@ -1241,7 +1259,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     }
     // Opaque here, or the compiler computes everything below that depends on them alone once,
     // ahead of the items, and spills it across the loop over the tiles.
-    int own_lane = lane, own_row = t * kM + row, col0 = share * Sh::kOutCols;
+    int own_lane = lane, own_row = (t - it.tile) * kM + row, col0 = share * Sh::kOutCols;
     asm volatile("" : "+r"(own_lane), "+r"(own_row), "+r"(col0));
     const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;
     const bool whole = it.slot < 0, gated = whole && a.gate;
@@ -1376,10 +1394,10 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
       mbar_init(smem_u32(&c.raw_full[i]), 1);
       mbar_init(smem_u32(&c.raw_empty[i]), Sh::kConvertWarps);
     }
-    mbar_init(smem_u32(&c.q_raw), 1);
-    mbar_init(smem_u32(&c.q_full), KV8 ? Sh::kConvertWarps : 1);
-    mbar_init(smem_u32(&c.q_empty), 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&c.q_raw[i]), 1);
+      mbar_init(smem_u32(&c.q_full[i]), KV8 ? Sh::kConvertWarps : 1);
+      mbar_init(smem_u32(&c.q_empty[i]), 1);
       mbar_init(smem_u32(&c.s_full[i]), 1);
       for (int part = 0; part < 2; ++part)
         mbar_init(smem_u32(&c.p_full[i][part]), 4 * Sh::kShares);
