@@ -84,7 +84,7 @@ class VllmDecodeBinding:
         (uint8 e4m3 bytes, the same shape) and k_scale / v_scale the layer's float scales."""
         if int(metadata.max_query_len) != 1:
             raise NotImplementedError("only decode batches (one query token per request); "
-                                      "prefill stays on vLLM's attention")
+                                      "VllmChunkBinding takes the others")
         tokens = qk.shape[0]
         seq_lens, table = metadata.seq_lens, metadata.block_table
         if seq_lens.numel() < tokens or table.shape[0] < tokens:
