@@ -21,6 +21,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "dory_common.h"
 #include "dory_sm100.cuh"
 
@@ -93,6 +95,14 @@ __device__ __forceinline__ void unpack(const Piece<T>& p, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
 }
+__device__ __forceinline__ void unpack(const Piece<__nv_bfloat16>& p, float (&x)[8]) {
+  const uint32_t w[4] = {p.w[0].x, p.w[0].y, p.w[0].z, p.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
 template <typename T>
 __device__ __forceinline__ void store_piece(T* p, const float (&x)[8]) {
   T e[8];
@@ -128,11 +138,10 @@ __device__ __forceinline__ int64_t position_of(const RotaryArgs& a, int t) {
 __device__ __forceinline__ void report(const RotaryArgs& a, uint32_t bit) {
   if (a.err) atomicOr(a.err, bit);
 }
-// Byte address of a cache row (K or V head g) of `slot`; elements of `esize` bytes.
-__device__ __forceinline__ uint8_t* cache_row(const RotaryArgs& a, uint8_t* base, int64_t slot,
-                                              int g, int esize) {
+// Offset of a slot's row (head 0) in a cache, in elements.
+__device__ __forceinline__ int64_t slot_offset(const RotaryArgs& a, int64_t slot) {
   const int64_t block = slot < INT32_MAX ? uint32_t(slot) / uint32_t(a.B) : slot / a.B;
-  return base + (block * a.sb + (slot - block * a.B) * a.so + int64_t(g) * a.sh) * esize;
+  return block * a.sb + (slot - block * a.B) * a.so;
 }
 
 // Row h of a token: 0 .. NH-1 q, then k heads, then (append) v heads.
@@ -171,6 +180,7 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
   const T* in = here ? static_cast<const T*>(rows.in) + g * rows.in_h : nullptr;
   const int64_t in_t = rows.in_t;
 
+  const float sign = APPEND ? 1.0f : a.sign;  // the append rotates forwards only
   uint64_t weight[8];  // with the norm, pairs: (sqk * sqk_factor)^2 of the lane's dims, 1 for k
   if constexpr (APPEND) {
 #pragma unroll
@@ -187,58 +197,93 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
   }
 
   const int first = blockIdx.x * a.run, last = min(first + a.run, a.T);  // this block's tokens
-  const int warps = blockDim.x >> 5;
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   const int angle_quads = a.R * (a.cs_dtype == DORY_DTYPE_F32 ? 4 : 2) / 16;
-  const uint4* const angle_ring = ring + kAhead * kQuads * blockDim.x;
+  // Everything that steps with the token or the place in the ring is kept and added to: address
+  // arithmetic was half of the instructions, which bound the append (8192 tokens: 40 us, 53 before).
+  const uint32_t place_bytes = kQuads * blockDim.x * 16, angle_bytes = warps * angle_quads * 16;
   const uint32_t own = uint32_t(__cvta_generic_to_shared(ring + threadIdx.x));
-  auto angles_of = [&](int place) {  // this warp's copy of a token's angles
-    return angle_ring + (place * warps + (threadIdx.x >> 5)) * angle_quads;
+  const uint32_t own_angles = uint32_t(__cvta_generic_to_shared(ring)) + kAhead * place_bytes +
+                              (threadIdx.x >> 5) * angle_quads * 16;
+  const uint32_t piece = blockDim.x * 16;  // between a thread's 16-byte words
+  // Positions and slots: a lane reads those of one token in 32 and the warp hands them round, so
+  // that they cost a token one shuffle each and the division by the block size nothing.  A
+  // position outside the table is -1, a slot that is not written an offset of -1.
+  int positions = -1;
+  int64_t offsets = -1, offsets_next = -1;
+  auto read_ahead = [&](int t) {  // tokens t .. t + 31
+    t += lane;
+    const bool reports = blockIdx.y == 0 && threadIdx.x < 32 && t < last;
+    int64_t slot = 0;
+    if constexpr (APPEND) {
+      slot = t < last ? a.slots[t] : -1;
+      const bool fits = slot >= 0 && slot < a.cache_slots;
+      offsets_next = fits ? slot_offset(a, slot) : -1;
+      if (reports && slot >= a.cache_slots) report(a, DORY_DEVERR_SLOT_OOB);
+    }
+    positions = 0;
+    if (a.R > 0) {
+      const int64_t pos = t < last ? position_of(a, t) : 0;
+      const bool inside = uint64_t(pos) < uint64_t(a.max_position);
+      positions = inside ? int(pos) : -1;
+      if (reports && !inside && slot >= 0) report(a, DORY_DEVERR_POSITION_OOB);
+    }
   };
-  auto position = [&](int t) { return a.R > 0 && t < last ? position_of(a, t) : int64_t(0); };
-  auto inside = [&](int64_t pos) { return a.R == 0 || (pos >= 0 && pos < a.max_position); };
-  // Starts the loads of token t, at position pos: elements and angles by asynchronous copies,
-  // since registers for as many tokens would leave too few threads.
-  auto ask = [&](int t, int64_t pos, int place) {
+  // Starts the loads of the next token, t, into the ring's place `to`: elements and angles by
+  // asynchronous copies, since registers for as many tokens would leave too few threads.
+  const T* next_in = in + (here ? first * in_t : 0);
+  uint32_t known_bits = 0;  // whether the angles of the tokens asked for last exist
+  auto ask = [&](int t, int to) {
+    if (((t - first) & 31) == 0) read_ahead(t);
+    const int pos = __shfl_sync(0xffffffffu, positions, (t - first) & 31);
+    known_bits = 2 * known_bits + (pos >= 0);
     if (t < last) {
       if (here) {
-        const T* p = in + t * in_t;
+        const uint32_t dst = own + to * place_bytes;
 #pragma unroll
         for (int i = 0; i < kQuads / 2; ++i) {
-          copy_async(own + (place * kQuads + i) * blockDim.x * 16, p + oa + i * (16 / sizeof(T)));
-          copy_async(own + (place * kQuads + kQuads / 2 + i) * blockDim.x * 16,
-                     p + ob + i * (16 / sizeof(T)));
+          copy_async(dst + i * piece, next_in + oa + i * (16 / sizeof(T)));
+          copy_async(dst + (kQuads / 2 + i) * piece, next_in + ob + i * (16 / sizeof(T)));
         }
+        next_in += in_t;
       }
-      if (a.R > 0 && inside(pos)) {
-        const uint4* row = static_cast<const uint4*>(a.cos_sin) + pos * angle_quads;
-        const uint32_t to = uint32_t(__cvta_generic_to_shared(angles_of(place)));
-        for (int i = threadIdx.x & 31; i < angle_quads; i += 32) copy_async(to + i * 16, row + i);
+      if (a.R > 0 && pos >= 0) {
+        const uint4* row = static_cast<const uint4*>(a.cos_sin) + int64_t(pos) * angle_quads + lane;
+        const uint32_t dst = own_angles + to * angle_bytes + lane * 16;
+        if (lane < angle_quads) copy_async(dst, row);
+        if (lane + 32 < angle_quads) copy_async(dst + 512, row + 32);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
 #pragma unroll 1
-  for (int i = 0; i < kAhead - 1; ++i) ask(first + i, position(first + i), i);
-  int64_t pos = position(first), pos_ask = position(first + kAhead - 1);
-  int64_t slot = APPEND && first < last ? a.slots[first] : 0;
+  for (int i = 0; i < kAhead - 1; ++i) ask(first + i, i);
   int place = 0;
+  uint8_t* out = nullptr;  // of q (append), or of any row
+  int64_t out_step = 0;
+  uint8_t* const cache_head = (is_v ? a.vc : a.kc) + g * a.sh * (KV8 ? 1 : 2);  // of k and v
+  if (here && (!APPEND || is_q)) {
+    constexpr int kOut = APPEND ? 2 : int(sizeof(T));
+    out = static_cast<uint8_t*>(rows.out) + (g * rows.out_h + first * rows.out_t) * kOut;
+    out_step = rows.out_t * kOut;
+  }
 #pragma unroll 1
   for (int t = first; t < last; ++t) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
     __syncwarp();  // the warp's angles are there, and its reads of the token before are done
-    ask(t + kAhead - 1, pos_ask, place == 0 ? kAhead - 1 : place - 1);
-    const int64_t pos_next = position(t + 1);
-    pos_ask = position(t + kAhead);
-    const int64_t slot_next = APPEND && t + 1 < last ? a.slots[t + 1] : 0;
-    const bool known = inside(pos);
+    if (APPEND && ((t - first) & 31) == 0) offsets = offsets_next;
+    ask(t + kAhead - 1, place == 0 ? kAhead - 1 : place - 1);
+    const bool known = known_bits >> (kAhead - 1) & 1;
+    const int64_t offset = APPEND ? __shfl_sync(0xffffffffu, offsets, (t - first) & 31) : 0;
+    const uint4* const mine = ring + place * (kQuads * blockDim.x) + threadIdx.x;
     uint64_t y[8];  // the lane's elements in pairs: four of the first piece, four of the second
     {
       Piece<T> xa, xb;
 #pragma unroll
       for (int i = 0; i < kQuads / 2; ++i) {
-        xa.w[i] = ring[(place * kQuads + i) * blockDim.x + threadIdx.x];
-        xb.w[i] = ring[(place * kQuads + kQuads / 2 + i) * blockDim.x + threadIdx.x];
+        xa.w[i] = mine[i * blockDim.x];
+        xb.w[i] = mine[(kQuads / 2 + i) * blockDim.x];
       }
       float ya[8], yb[8];
       unpack(xa, ya);
@@ -254,21 +299,23 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
       for (int j = 0; j < 8; ++j) y[j] = 0;
     } else if (turn) {
       float c[8], s[8];
-      load8(angles_of(place), 8 * l, a.cs_dtype, c);
-      load8(angles_of(place), a.R / 2 + 8 * l, a.cs_dtype, s);
+      const uint4* const angles = ring + kAhead * kQuads * blockDim.x +
+                                  (place * warps + (threadIdx.x >> 5)) * angle_quads;
+      load8(angles, 8 * l, a.cs_dtype, c);
+      load8(angles, a.R / 2 + 8 * l, a.cs_dtype, s);
       if (a.inter) {  // a pair is one rotation: (u, w) c + (w, u) (-s, s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float u, w;
           split(y[j], u, w);
-          const float turn_by = a.sign * s[j];
+          const float turn_by = sign * s[j];
           y[j] = fma2(pair(w, u), pair(-turn_by, turn_by), mul2(y[j], pair(c[j], c[j])));
         }
       } else {  // two rotations at once
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint64_t u = y[j], w = y[4 + j], c2 = pair(c[2 * j], c[2 * j + 1]);
-          const uint64_t s2 = pair(a.sign * s[2 * j], a.sign * s[2 * j + 1]);
+          const uint64_t s2 = pair(sign * s[2 * j], sign * s[2 * j + 1]);
           y[j] = fma2(mul2(w, pair(-1.0f, -1.0f)), s2, mul2(u, c2));
           y[4 + j] = fma2(u, s2, mul2(w, c2));
         }
@@ -282,17 +329,16 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
         float sum, other;
         split(squares, sum, other);
         sum += other;
-        for (int m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+        if (lanes > 8) sum += __shfl_xor_sync(0xffffffffu, sum, 8);  // 4, 8 or 16 lanes a row
+        if (lanes > 4) sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         if (!is_v && known) {  // zeros stay zeros, whatever eps
           const float inv = rsqrtf(sum + a.eps);
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = mul2(y[j], mul2(weight[j], pair(inv, inv)));
         }
       }
-    }
-    if (h == 0 && l == 0) {
-      if (!known && !(APPEND && slot < 0)) report(a, DORY_DEVERR_POSITION_OOB);
-      if (APPEND && slot >= a.cache_slots) report(a, DORY_DEVERR_SLOT_OOB);
     }
     if (here) {
       float ya[8], yb[8];
@@ -302,17 +348,12 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
         split(y[4 + j], yb[2 * j], yb[2 * j + 1]);
       }
       if (!APPEND || is_q) {
-        if constexpr (APPEND) {
-          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.q.out) + t * a.q.out_t + g * a.q.out_h;
-          store_piece(o + oa, ya);
-          store_piece(o + ob, yb);
-        } else {
-          T* o = static_cast<T*>(rows.out) + t * rows.out_t + g * rows.out_h;
-          store_piece(o + oa, ya);
-          store_piece(o + ob, yb);
-        }
-      } else if (slot >= 0 && slot < a.cache_slots) {
-        uint8_t* o = cache_row(a, is_v ? a.vc : a.kc, slot, g, KV8 ? 1 : 2);
+        using Out = std::conditional_t<APPEND, __nv_bfloat16, T>;
+        store_piece(reinterpret_cast<Out*>(out) + oa, ya);
+        store_piece(reinterpret_cast<Out*>(out) + ob, yb);
+        out += out_step;
+      } else if (offset >= 0) {
+        uint8_t* o = cache_head + offset * (KV8 ? 1 : 2);
         if constexpr (KV8) {
           const float scale = is_v ? a.v_scale : a.k_scale;
 #pragma unroll
@@ -330,8 +371,6 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
         }
       }
     }
-    pos = pos_next;
-    slot = slot_next;
     if (++place == kAhead) place = 0;
   }
 }
@@ -397,7 +436,9 @@ __global__ void __launch_bounds__(128) rotary_any(const RotaryArgs a) {
     }
     if (h >= a.NH && slot < 0) return;
     const int g = is_v ? h - a.NH - a.NKV : h - a.NH;
-    uint8_t* row_out = h < a.NH ? nullptr : cache_row(a, is_v ? a.vc : a.kc, slot, g, KV8 ? 1 : 2);
+    uint8_t* row_out = h < a.NH ? nullptr
+                                : (is_v ? a.vc : a.kc) +
+                                      (slot_offset(a, slot) + g * a.sh) * (KV8 ? 1 : 2);
     for (int i = lane; i < a.D; i += 32) {
       float y = is_v ? to_f32(x[i]) : inside ? turned(a, x, i, pos) : 0.0f;
       if (a.norm && !is_v) {
@@ -562,11 +603,12 @@ int32_t rotary(const DoryRotaryParams* P, bool append, void* stream) {
   if (append) {
     fits(a.v, false);
     pieces = pieces && aligned16(p.key_cache) && aligned16(p.value_cache) &&
-             !((a.sb | a.so | a.sh) & 7);
+             !((a.sb | a.so | a.sh) & 7) && a.sb >= 0 && a.so >= 0;
   }
   // A block's ring is then at most 3 x (384 threads x 64 bytes + 12 warps x 1 KB) = 108 KB.
   const int angle_bytes = p.rotary_dim * (p.cos_sin_dtype == DORY_DTYPE_F32 ? 4 : 2);
-  pieces = pieces && aligned16(p.cos_sin) && aligned16(p.sqk) && angle_bytes <= 1024;
+  pieces = pieces && aligned16(p.cos_sin) && aligned16(p.sqk) && angle_bytes <= 1024 &&
+           p.max_position <= INT32_MAX;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!append) return run_type<false, false>(a, p.io_dtype, pieces, s);
   return kv8 ? run_type<true, true>(a, p.io_dtype, pieces, s)

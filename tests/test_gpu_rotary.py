@@ -304,3 +304,56 @@ def test_an_unknown_position_appends_zeros_whatever_eps(D, R):
     assert (q_out == 0).all() and (key[1, 1] == 0).all()
     assert torch.equal(value[1, 1], v[0].to(torch.bfloat16))
     assert (key[0] == 5.0).all() and (key[1, 2:] == 5.0).all()
+
+
+def test_a_block_walks_many_tokens():
+    """More tokens than 32 a block, which the kernels read positions and slots of at a time, with
+    positions and slots out of range everywhere."""
+    T, D = 3552 * 70 + 5, 64
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(T, 4, D, generator=g, device=DEV).to(torch.bfloat16)
+    q, k, v = x.split([2, 1, 1], dim=1)
+    pos = torch.randint(-1, 4100, (T,), generator=g, device=DEV)
+    blocks = T // 16 + 1
+    slots = torch.randperm(T, generator=g, device=DEV)
+    slots[pos % 7 == 1] = -1
+    slots[pos % 7 == 2] += blocks * 16
+    table = rotary_cos_sin(4096, D, device=DEV)
+    key = torch.full((blocks, 16, 1, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    value = key.clone()
+    q_out = torch.empty(T, 2, D, dtype=torch.bfloat16, device=DEV)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    rotary_append(q, k, v, pos, table, slots, key, value, q_out, error_word=word)
+    assert word.item() == _native.DEVERR_POSITION_OOB | _native.DEVERR_SLOT_OOB
+    inside = (pos >= 0) & (pos < 4096)
+    c, s = (t[:, None] for t in table[pos.clamp(0, 4095)].double().chunk(2, dim=1))
+    a, b = x[:, :3].double().chunk(2, dim=2)
+    want = torch.cat([a * c - b * s, b * c + a * s], dim=2) * inside[:, None, None]
+    size = torch.cat([(a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()], dim=2)
+    # each product and the sum rounded to FP32, then to bf16
+    tol = 3 * 2.0 ** -24 * size + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -20) + 1e-30
+    assert ((q_out.double() - want[:, :2]).abs() <= tol[:, :2]).all()
+    kept = (slots >= 0) & (slots < blocks * 16)
+    at = slots[kept]
+    flat_k, flat_v = key.view(-1, D), value.view(-1, D)
+    assert ((flat_k[at].double() - want[kept, 2]).abs() <= tol[kept, 2]).all()
+    assert torch.equal(flat_v[at], v[kept, 0])
+    free = torch.ones(blocks * 16, dtype=torch.bool, device=DEV)
+    free[at] = False
+    assert (flat_k[free] == 5.0).all() and (flat_v[free] == 5.0).all()
+    rotary_embed(q, k, pos, table, q_out, k_out := torch.empty_like(k))
+    assert ((q_out.double() - want[:, :2]).abs() <= tol[:, :2]).all()
+    assert ((k_out.double() - want[:, 2:]).abs() <= tol[:, 2:]).all()
+
+
+@pytest.mark.parametrize("D,R", [(64, 64), (128, 64), (256, 256)])
+def test_a_padding_token_of_unknown_position_is_not_reported(D, R):
+    x = torch.randn(3, 4, D, device=DEV).to(torch.bfloat16)
+    key = torch.full((2, 16, 1, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    value, word = key.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    q_out = torch.empty(3, 2, D, dtype=torch.bfloat16, device=DEV)
+    rotary_append(x[:, :2], x[:, 2:3], x[:, 3:], torch.tensor([0, 99, -4], device=DEV),
+                  rotary_cos_sin(8, R, device=DEV), torch.tensor([3, -1, -1], device=DEV), key,
+                  value, q_out, error_word=word)
+    assert word.item() == 0 and (q_out[1:] == 0).all()
+    assert torch.equal(value[0, 3], x[0, 3:]) and (value.view(-1, D)[4:] == 5.0).all()
