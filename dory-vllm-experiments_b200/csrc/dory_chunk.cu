@@ -318,28 +318,14 @@ __device__ __forceinline__ int scan_add(int x, int lane) {  // inclusive
   return x;
 }
 
+// A CTA's units [u0, u1), of `per` a CTA: its first item is number m of KV head kvh of sequence
+// seq, from its unit off on.
+struct Piece {
+  int u0, u1, per, seq, kvh, m, off;
+};
 template <int HD, bool KV8>
-__device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
+__device__ Piece find_piece(const ChunkArgs& a, int lane) {
   const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
-  int32_t* join = a.joins + cta * 8;
-  int queued = 0, turn = 0;
-  auto push = [&](const Item& it) {
-    const int at = queued % kQueue;
-    if (queued >= kQueue &&
-        !wait_warp(c.item_empty[at], (queued / kQueue - 1) & 1, &c.abort, a.err))
-      return false;
-    if (lane == 0) {
-      c.items[at] = it;
-      mbar_arrive(smem_u32(&c.item_full[at]));
-    }
-    __syncwarp();
-    ++queued;
-    return true;
-  };
-  Item end;
-  memset(&end, 0, sizeof(end));
-  end.flags = kItemEnd;
-
   int total = 0, mine = 0;
   for (int base = 0; base < a.S; base += 32) {
     const int i = base + lane;
@@ -357,7 +343,7 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
   }
   const int per = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_units);
   const int u0 = min(cta * per, total), u1 = min(u0 + per, total);
-  int cut = 0;  // whether this CTA holds the first part of a cut item
+  Piece p{u0, u1, per, 0, 0, 0, 0};
   if (u0 < u1) {
     // the sequence, KV head and item that hold unit u0
     int before = 0, seq = 0;
@@ -373,7 +359,7 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
       }
       before = __shfl_sync(0xffffffffu, upto, 31);
     }
-    Seq s = sequence(a, seq);
+    const Seq s = sequence(a, seq);
     const int per_head =
         __shfl_sync(0xffffffffu, head_units(a, lane ? Seq{0, 0, 0, 0} : s, tokens, lane), 0);
     int rest = u0 - before;
@@ -394,9 +380,43 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, int lane) {
       rest -= __shfl_sync(0xffffffffu, upto, 31);
       if ((base + 32) * tokens >= s.n) break;  // not reached: rest lies within the head
     }
-    int off = rest;
+    p.seq = seq;
+    p.kvh = kvh;
+    p.m = m;
+    p.off = rest;
+  }
+  return p;
+}
+
+template <int HD, bool KV8>
+__device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& p, int lane) {
+  const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
+  int32_t* join = a.joins + cta * 8;
+  int queued = 0, turn = 0;
+  auto push = [&](const Item& it) {
+    const int at = queued % kQueue;
+    if (queued >= kQueue &&
+        !wait_warp(c.item_empty[at], (queued / kQueue - 1) & 1, &c.abort, a.err))
+      return false;
+    if (lane == 0) {
+      c.items[at] = it;
+      mbar_arrive(smem_u32(&c.item_full[at]));
+    }
+    __syncwarp();
+    ++queued;
+    return true;
+  };
+  Item end;
+  memset(&end, 0, sizeof(end));
+  end.flags = kItemEnd;
+
+  int cut = 0;  // whether this CTA holds the first part of a cut item
+  if (p.u0 < p.u1) {
+    const int u1 = p.u1, per = p.per;
+    int seq = p.seq, kvh = p.kvh, m = p.m, off = p.off, first, tiles;
+    Seq s = sequence(a, seq);
 #pragma unroll 1
-    for (int at = u0; at < u1;) {
+    for (int at = p.u0; at < u1;) {
       const int units = item_units(a, s, m, tokens, first, tiles);
       const int take = min(units - off, u1 - at);
       const int work = units - kItemUnits;  // cache tiles, or 1
@@ -1413,6 +1433,9 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
     fence_async_smem();
   }
   if (warp == Sh::kMmaWarp) tmem_alloc(smem_u32(&c.tmem), 512);
+  Piece piece;  // the others have nothing to do before it is known
+  memset(&piece, 0, sizeof(piece));
+  if (warp == Sh::kPlanWarp) piece = find_piece<HD, KV8>(a, lane);
   if (warp == Sh::kLoadWarp && lane == 0) {
     prefetch_map(&maps.q);
     prefetch_map(&maps.k);
@@ -1436,7 +1459,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
       while (!mbar_try(smem_u32(&c.drained), 0) && clock64() - start < 1000000000LL) {
       }
     } else if (warp == Sh::kPlanWarp) {
-      plan_role<HD, KV8>(a, c, lane);
+      plan_role<HD, KV8>(a, c, piece, lane);
     } else if constexpr (KV8) {
       convert_role<HD, KV8>(a, c, tiles, threadIdx.x - Sh::kConvert * 32);
     }
@@ -1474,8 +1497,8 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
   using Sh = Shape<HD, KV8>;
   constexpr int kPer = HD / 32;  // columns of a lane
   grid_wait();
-  const int32_t* join = a.joins + blockIdx.x * 8;
-  const int parts = join[0], tok0 = join[1], ntok = join[2], kvh = join[3];
+  const int4 join = *reinterpret_cast<const int4*>(a.joins + blockIdx.x * 8);
+  const int parts = join.x, tok0 = join.y, ntok = join.z, kvh = join.w;
   if (!parts) return;
   const int lane = threadIdx.x & 31;
   for (int r = blockIdx.y * 16 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 16 * kJoinSlices) {
@@ -1485,9 +1508,14 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
     auto slot = [&](int i) {
       return int64_t(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * Sh::kItemRows + r;
     };
-    float m = -INFINITY, l = 0.0f, acc[kPer];
+    const int token = tok0 + tok;
+    const int64_t column = int64_t(kvh * a.G + in_tile - row_tok * a.G) * HD + lane * kPer;
+    float m = -INFINITY, l = 0.0f, acc[kPer], gate[kPer];
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) acc[x] = 0.0f;
+    for (int x = 0; x < kPer; ++x) {  // the gate on its way with the parts
+      acc[x] = 0.0f;
+      gate[x] = a.gate ? load_gate(a, token * a.gate_t + column + x) : 1.0f;
+    }
     for (int i = 0; i < parts; i += 4) {  // four parts on their way at once
       float2 ml[4];
       float o[4][kPer];
@@ -1511,15 +1539,9 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
       }
     }
     const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;
-    const int token = tok0 + tok;
-    const int64_t column = int64_t(kvh * a.G + in_tile - row_tok * a.G) * HD + lane * kPer;
 #pragma unroll
     for (int x = 0; x < kPer; x += 2) {
-      float y0 = acc[x] * inv, y1 = acc[x + 1] * inv;
-      if (a.gate) {
-        y0 *= load_gate(a, token * a.gate_t + column + x);
-        y1 *= load_gate(a, token * a.gate_t + column + x + 1);
-      }
+      const float y0 = acc[x] * inv * gate[x], y1 = acc[x + 1] * inv * gate[x + 1];
       *reinterpret_cast<uint32_t*>(a.out + token * a.out_t + column + x) = pack_bf16(y0, y1);
     }
   }
