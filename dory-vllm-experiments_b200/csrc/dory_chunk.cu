@@ -46,6 +46,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "dory_common.h"
 #include "dory_sm100.cuh"
@@ -1006,23 +1007,12 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
   if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
 }
 
-// Two consecutive gate values: their bits (16-bit types: the first word), and their product.
-__device__ __forceinline__ uint2 load_gate2(const ChunkArgs& a, int64_t at) {
-  if (a.gate_dtype == DORY_DTYPE_F32)
-    return *reinterpret_cast<const uint2*>(static_cast<const float*>(a.gate) + at);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.gate) + at), 0);
-}
-__device__ __forceinline__ void apply_gate2(int dtype, const uint2& w, float* v) {
-  if (dtype == DORY_DTYPE_F32) {
-    v[0] *= __uint_as_float(w.x);
-    v[1] *= __uint_as_float(w.y);
-  } else if (dtype == DORY_DTYPE_BF16) {
-    v[0] *= __uint_as_float(w.x << 16);
-    v[1] *= __uint_as_float(w.x & 0xffff0000u);
-  } else {
-    v[0] *= __half2float(__ushort_as_half(w.x & 0xffff));
-    v[1] *= __half2float(__ushort_as_half(w.x >> 16));
-  }
+// Two 16-bit gate values, in g.x, as FP32.
+__device__ __forceinline__ void widen2(bool bf16, uint2& g) {
+  const uint32_t w = g.x;
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  g.x = bf16 ? w << 16 : __float_as_uint(h.x);
+  g.y = bf16 ? w & 0xffff0000u : __float_as_uint(h.y);
 }
 
 // A bit for each of 32 columns that lies above `last` or below `first`.
@@ -1289,77 +1279,107 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     // 32 lines an instruction: 20,500 clocks an item with an FP32 gate.
     const int quarter = own_lane & 3;
     const int where = row_head << 16 | tok;  // tok < 256
-    float row_inv[4], odd[4];                // odd: NaN once a value of the row is not finite
-    int64_t out_at[4], gate_at[4];
+    uint64_t row_inv[4], odd[4];             // odd: NaN once a value of the row is not finite
+    int64_t out_at[4];
+    const char* gate_at[4];
     uint32_t alive = 0;
+    const uint32_t lives = __ballot_sync(0xffffffffu, live);
+    const int gate_size = a.gate_dtype == DORY_DTYPE_F32 ? 4 : 2;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {  // rows 8 r + lane / 4
-      const int src = 8 * r + (own_lane >> 2);
+      const int own = 8 * r + (own_lane >> 2);
+      const bool there = lives >> own & 1;
+      const int src = there ? own : __ffs(lives) - 1;  // any row's gate may be read in its place
       const int w = __shfl_sync(0xffffffffu, where, src);
-      row_inv[r] = whole ? __shfl_sync(0xffffffffu, inv, src) : 1.0f;
-      alive |= uint32_t(__shfl_sync(0xffffffffu, int(live), src)) << r;
+      const float f = whole ? __shfl_sync(0xffffffffu, inv, src) : 1.0f;
+      row_inv[r] = pair(f, f);
+      alive |= uint32_t(there) << r;
       const int64_t token = it.tok0 + (w & 0xffff);
       const int64_t column = int64_t(it.kvh * a.G + (w >> 16)) * HD + col0;
       out_at[r] = whole ? token * a.out_t + column
                         : (int64_t(it.slot) * Sh::kItemRows + own_row - own_lane + src) * HD + col0;
-      gate_at[r] = token * a.gate_t + column + 2 * quarter;
-      odd[r] = 0.0f;
+      gate_at[r] = static_cast<const char*>(a.gate) +
+                   (token * a.gate_t + column + 2 * quarter) * gate_size;
+      odd[r] = 0;
     }
-    uint2 g[4][4];  // the gate's bits, asked for a piece ahead
-    auto ask_gate = [&](int x) {
+    // Code of its own for each type of gate (its elements' bytes; 0: none), without a test or a
+    // branch in it.  The gate is asked for a piece ahead.
+    auto output = [&](auto bytes) {
+      constexpr int kBytes = bytes.value;
+      uint2 g[4][4];
+      auto ask_gate = [&]() {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[r][i] = make_uint2(0, 0);  // defined on every path, or it lives from the start on
-          if (gated && (alive >> r & 1)) g[r][i] = load_gate2(a, gate_at[r] + x + 8 * i);
+          for (int i = 0; i < 4; ++i) {
+            if (kBytes == 4) g[r][i] = *reinterpret_cast<const uint2*>(gate_at[r] + 32 * i);
+            if (kBytes == 2) g[r][i].x = *reinterpret_cast<const uint32_t*>(gate_at[r] + 16 * i);
+          }
+          gate_at[r] += 32 * kBytes;
         }
-    };
-    ask_gate(0);
+      };
+      if (kBytes) ask_gate();
 #pragma unroll 1
-    for (int x = 0; x < Sh::kOutCols; x += 32) {
-      float o[32];  // row r's columns 8 i + 2 quarter + y at 16 (r / 2) + 4 i + 2 (r % 2) + y
+      for (int x = 0; x < Sh::kOutCols; x += 32) {
+        float o[32];  // row r's columns 8 i + 2 quarter + y at 16 (r / 2) + 4 i + 2 (r % 2) + y
 #pragma unroll
-      for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-      if (e > b) {
-        tmem_ld_fragment(o_addr + x, reinterpret_cast<uint32_t*>(o));
-        tmem_ld_fragment(o_addr + (16u << 16) + x, reinterpret_cast<uint32_t*>(o + 16));
-      }
-      tmem_wait_ld32(reinterpret_cast<uint32_t*>(o));
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* v = o + 16 * (r / 2) + 4 * i + 2 * (r % 2);
-          odd[r] = fmaf(v[0], 0.0f, fmaf(v[1], 0.0f, odd[r]));
-          v[0] *= row_inv[r];
-          v[1] *= row_inv[r];
-          if (gated) apply_gate2(a.gate_dtype, g[r][i], v);
+        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+        if (e > b) {
+          tmem_ld_fragment(o_addr + x, reinterpret_cast<uint32_t*>(o));
+          tmem_ld_fragment(o_addr + (16u << 16) + x, reinterpret_cast<uint32_t*>(o + 16));
         }
-      if (x + 32 < Sh::kOutCols) ask_gate(x + 32);
+        tmem_wait_ld32(reinterpret_cast<uint32_t*>(o));
+        uint64_t v[4][4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t w[4];
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float* v = o + 16 * (r / 2) + 4 * i + 2 * (r % 2);
-          w[i] = pack_bf16(v[0], v[1]);
-          if (!whole && (alive >> r & 1))
-            *reinterpret_cast<float2*>(a.part_o + out_at[r] + x + 8 * i + 2 * quarter) =
-                make_float2(v[0], v[1]);
-        }
-        if (whole) {
+          for (int i = 0; i < 4; ++i) {
+            const float* at_o = o + 16 * (r / 2) + 4 * i + 2 * (r % 2);
+            v[r][i] = pair(at_o[0], at_o[1]);
+            odd[r] = fma2(v[r][i], 0, odd[r]);
+            if (whole) v[r][i] = mul2(v[r][i], row_inv[r]);
+            if (kBytes == 2) widen2(a.gate_dtype == DORY_DTYPE_BF16, g[r][i]);
+            if (kBytes)
+              v[r][i] = mul2(v[r][i], pair(__uint_as_float(g[r][i].x), __uint_as_float(g[r][i].y)));
+          }
+        if (kBytes && x + 32 < Sh::kOutCols) ask_gate();
+        if (kBytes || whole) {
           const bool second = quarter & 1;  // of two neighbours: takes the odd eights
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? w[i] : w[i + 1], 1);
-            if (alive >> r & 1)
-              *reinterpret_cast<uint2*>(a.out + out_at[r] + x + 8 * (i + second) + 4 * (quarter >> 1)) =
-                  second ? make_uint2(got, w[i + 1]) : make_uint2(w[i], got);
+          for (int r = 0; r < 4; ++r) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v0, v1;
+              split(v[r][i], v0, v1);
+              w[i] = pack_bf16(v0, v1);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? w[i] : w[i + 1], 1);
+              if (alive >> r & 1)
+                *reinterpret_cast<uint2*>(a.out + out_at[r] + x + 8 * (i + second) +
+                                          4 * (quarter >> 1)) =
+                    second ? make_uint2(got, w[i + 1]) : make_uint2(w[i], got);
+            }
           }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v0, v1;
+              split(v[r][i], v0, v1);
+              if (alive >> r & 1)
+                *reinterpret_cast<float2*>(a.part_o + out_at[r] + x + 8 * i + 2 * quarter) =
+                    make_float2(v0, v1);
+            }
         }
       }
-    }
+    };
+    if (!gated) output(std::integral_constant<int, 0>());
+    else if (gate_size == 4) output(std::integral_constant<int, 4>());
+    else output(std::integral_constant<int, 2>());
     __syncwarp();
     const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
     if (live && !whole && share == 0)
@@ -1367,7 +1387,9 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     uint32_t again = 0;  // rows, as lanes
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t lanes = __ballot_sync(0xffffffffu, isnan(odd[r]));
+      float odd0, odd1;
+      split(odd[r], odd0, odd1);
+      const uint32_t lanes = __ballot_sync(0xffffffffu, isnan(odd0) || isnan(odd1));
       if (lanes)
         for (int y = 0; y < 8; ++y)
           if (lanes >> (4 * y) & 15) again |= 1u << (8 * r + y);
