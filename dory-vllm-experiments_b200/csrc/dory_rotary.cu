@@ -3,16 +3,17 @@
 // include/dory_decode.h.
 //
 // Both read every input once and write every output once, with a handful of operations per
-// element: HBM bounds a long prompt, the launch and two dependent loads (position, then
-// table row) a single token.
+// element: HBM bounds a long rotation (8192 tokens of 32 + 8 heads of 128 bf16 dims: 30.9 us, 85%
+// of the measured copy rate), instruction issue and then HBM a long append (40.4 us, 78%), the
+// launch and two dependent loads (position, then table row) a single token (4.3 us).
 //
 // rotary_vec: a head's row belongs to head_dim / 16 neighbouring lanes.  Lane l holds two
 // 8-element pieces that contain both members of its pairs: dims 8l and rotary_dim / 2 + 8l of
 // the half layout, 16l and 16l + 8 of the interleaved one, so in both it needs the angles 8l ..
 // 8l + 7 and no exchange between lanes (the norm alone takes log2(head_dim / 16) shuffles).  A
 // block takes the heads of one token, then of the next: a lane keeps its head, so its share of
-// sqk stays in registers, the heads of a token share its angles in L1, and the next token's loads
-// (position, then angles) are on their way while this one is worked on.
+// sqk stays in registers, the heads of a token share its angles in L1, and the loads of the next
+// two tokens are on their way while this one is worked on.
 // rotary_any: one warp per row, a pair per lane, for every size, stride and alignment.
 
 #include <cuda_bf16.h>
