@@ -593,9 +593,13 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
         row[x] = 0;
       }
       if (a.copy_rows != a.B) {
+        int r = (kv0 + tile) * kN % a.B;
 #pragma unroll
-        for (int x = 0; x < kN / 16; ++x)
-          row[x] = ((kv0 + tile) * kN + x * a.copy_rows) % a.B;
+        for (int x = 0; x < kN / 16; ++x) {
+          row[x] = r;
+          r += a.copy_rows;  // which divides both the tile and the page
+          if (r == a.B) r = 0;
+        }
       }
       if (elect_one()) {
         mbar_expect(bar, kBytes / Sh::kLoaders);

@@ -10,6 +10,9 @@ for v's rounding and 2^-8 of the result.
 
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
@@ -243,3 +246,40 @@ def test_refusals():
     meta.query_start_loc = torch.tensor([0, 4], dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="KV-cache shape"):
         binding.attend(meta, layer.cache[:, 0], q, 0, 1.0, out)
+
+
+FIRST = """
+import sys, torch
+sys.path[:0] = [{package!r}]
+from dory_chunk_attention import ChunkAttention
+from dory_rotary_steps import rotary_append, rotary_cos_sin
+dev, T = torch.device("cuda"), 40
+q, k, v = torch.randn(T, 12, 128, device=dev).bfloat16().split([8, 2, 2], 1)
+key = torch.zeros(8, 16, 2, 128, device=dev, dtype=torch.bfloat16)
+value, at = key.clone(), torch.arange(T, device=dev)
+table = rotary_cos_sin(64, 128, device=dev)
+q_out = torch.empty(T, 8, 128, device=dev, dtype=torch.bfloat16)
+blocks = torch.arange(8, device=dev, dtype=torch.int32)[None]
+start = torch.tensor([0, T], device=dev, dtype=torch.int32)
+out = torch.zeros(T, 1024, device=dev, dtype=torch.bfloat16)
+attn = ChunkAttention(8, 2, 128, dev)
+def step():
+    rotary_append(q, k, v, at, table, at, key, value, q_out)
+    attn(q_out, key, value, blocks, start, start[1:], 0, 0.09, out)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+attn.check_errors()
+first = out.clone()
+for x in (out, key, value):
+    x.zero_()
+step()
+assert torch.equal(out, first) and out.any()
+"""
+
+
+def test_the_first_call_may_be_a_captured_one():
+    package = str(Path(__file__).resolve().parents[1] / "dory-vllm-experiments_b200")
+    subprocess.run([sys.executable, "-c", FIRST.format(package=package)], check=True, timeout=300)

@@ -357,3 +357,23 @@ def test_a_padding_token_of_unknown_position_is_not_reported(D, R):
                   value, q_out, error_word=word)
     assert word.item() == 0 and (q_out[1:] == 0).all()
     assert torch.equal(value[0, 3], x[0, 3:]) and (value.view(-1, D)[4:] == 5.0).all()
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("dim_step", [1, 3])  # the wide kernel, and (odd strides) the general one
+def test_append_offsets_pass_32_bits(D, dim_step):
+    stride = 2 ** 25 + (dim_step - 1)
+    buf = torch.empty(70 * stride, dtype=torch.bfloat16, device=DEV)
+    key = buf.as_strided((70, 16, 2, D), (stride, 2 * D, D, 1))
+    value = buf.as_strided((70, 16, 2, D), (stride, 2 * D, D, 1), 2 ** 24)
+    for c in (key, value):
+        c[[0, 5, 69]] = 5.0
+    x = torch.randn(3, 6, D, device=DEV).to(torch.bfloat16)
+    slots = torch.tensor([69 * 16 + 15, 3, 5 * 16], device=DEV)
+    q_out = torch.empty(3, 2, D, dtype=torch.bfloat16, device=DEV)
+    rotary_append(x[:, :2], x[:, 2:4], x[:, 4:], None, None, slots, key, value, q_out)
+    assert torch.equal(q_out, x[:, :2])
+    for c, rows in ((key, x[:, 2:4]), (value, x[:, 4:])):
+        assert torch.equal(c[69, 15], rows[0]) and torch.equal(c[0, 3], rows[1])
+        assert torch.equal(c[5, 0], rows[2])
+        assert (c[69, :15] == 5.0).all() and (c[5, 1:] == 5.0).all() and (c[0, 4:] == 5.0).all()
