@@ -38,7 +38,7 @@
 // between softmax and product warps, tile by tile (prompt of 8192, 32 query heads on 8, 128 dims:
 // 545 us, 1,010 TFLOP/s, 63% of the library GEMM's rate; no exponentials, or half of the
 // products, would save 5-13%); 256-dim heads the page copies as well (16 heads on 4: 690 us, 580
-// with 128-row pages); FP8 caches the conversion (626 us); short items their latency, 4-5 us
+// with 128-row pages); FP8 caches the conversion (598 us); short items their latency, 4-5 us
 // each, and a call of few tokens the chain from launch to join (4 tokens over 640: 16 us).
 
 #include <cuda_bf16.h>
@@ -648,6 +648,13 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
   using Sh = Shape<HD, KV8>;
   const int lane = thread & 31;
   const uint32_t stages = tiles + Sh::kQBytes, raws = stages + Sh::kStages * Sh::kStageBytes;
+  // A thread converts 16 dims at a time, one 16-byte piece of bytes to two of f16, of every 16th
+  // row.  Of eight lanes four take half of a row and four the other half of its neighbour, so
+  // that no two of them share a bank.
+  const int piece = thread & 7, own_row = (thread >> 3) ^ (piece >> 2);
+  const uint32_t own_src = own_row * 128 + ((piece ^ own_row) & 7) * 16;
+  const uint32_t own_dst = (piece >> 2) * kChunkBytes + own_row * 128 +
+                           (((piece & 3) * 2) ^ (own_row & 7)) * 16;
   int queued = 0, raw = 0, stage = 0;
   uint32_t raw_phase = 0, phase = 1, q_phase = 0;
   for (;;) {
@@ -706,30 +713,24 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       int tile, half;
       stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
       const int seen_lo = lo - (it.kv0 + tile) * kN, seen_hi = hi - (it.kv0 + tile) * kN;
-      // 16 dims at a time: one 16-byte piece of bytes, two of f16.  Eight lanes take a row; the
-      // upper four write their second piece first, so that no two lanes share a bank.
-#pragma unroll 2
-      for (int x = thread; x < kN * 8; x += 128) {
-        const int row = x >> 3, piece = x & 7;
+      // Rows 16 apart have the same swizzle, so a step is an addition to three addresses (FP8
+      // prompt of 8192: 598 us; 618 with the addresses formed row by row, 256-dim heads 796, 872).
+      const uint32_t src = from + own_src, dst = to + own_dst;
+      const int own_seen = own_row - seen_lo, n_seen = max(seen_hi - seen_lo, 0);
+      constexpr int kAtOnce = HD == 256 ? 4 : 2;
+#pragma unroll kAtOnce
+      for (int k = 0; k < kN / 16; ++k) {
         uint32_t w[4], f[8];
-        lds128(from + row * 128 + ((piece ^ row) & 7) * 16, w);
-        const bool seen = row >= seen_lo && row < seen_hi;  // by some row of the item
+        lds128(src + k * 16 * 128, w);
+        const bool seen = uint32_t(own_seen + 16 * k) < uint32_t(n_seen);  // by a row of the item
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          f[2 * y] = seen ? e4m3x2_to_f16x2(w[y]) : 0;
-          f[2 * y + 1] = seen ? e4m3x2_to_f16x2(w[y] >> 16) : 0;
+          if (!seen) w[y] = 0;
+          f[2 * y] = e4m3x2_to_f16x2(w[y]);
+          f[2 * y + 1] = e4m3x2_to_f16x2(w[y] >> 16);
         }
-        const uint32_t chunk = to + (piece >> 2) * kChunkBytes + row * 128;
-        const int first = (piece & 3) * 2;
-        const bool upper = piece & 4;
-        uint32_t early[4], late[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          early[y] = upper ? f[4 + y] : f[y];
-          late[y] = upper ? f[y] : f[4 + y];
-        }
-        sts128(chunk + ((first + upper) ^ (row & 7)) * 16, early);
-        sts128(chunk + ((first + !upper) ^ (row & 7)) * 16, late);
+        sts128(dst + k * 16 * 128, f);
+        sts128((dst ^ 16) + k * 16 * 128, f + 4);
       }
       fence_async_smem();
       __syncwarp();
