@@ -38,7 +38,7 @@
 // between softmax and product warps, tile by tile (prompt of 8192, 32 query heads on 8, 128 dims:
 // 545 us, 1,010 TFLOP/s, 63% of the library GEMM's rate; no exponentials, or half of the
 // products, would save 5-13%); 256-dim heads the page copies as well (16 heads on 4: 690 us, 580
-// with 128-row pages); FP8 caches the conversion (598 us); short items their latency, 4-5 us
+// with 128-row pages); FP8 caches the conversion (586 us); short items their latency, 4-5 us
 // each, and a call of few tokens the chain from launch to join (4 tokens over 640: 16 us).
 
 #include <cuda_bf16.h>
@@ -714,7 +714,7 @@ __device__ void convert_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       stage_holds<HD, KV8>(q, kvn, is_v, tile, half);
       const int seen_lo = lo - (it.kv0 + tile) * kN, seen_hi = hi - (it.kv0 + tile) * kN;
       // Rows 16 apart have the same swizzle, so a step is an addition to three addresses (FP8
-      // prompt of 8192: 598 us; 618 with the addresses formed row by row, 256-dim heads 796, 872).
+      // prompt of 8192: 598 us then; 618 with the addresses formed row by row, 256-dim heads 796, 872).
       const uint32_t src = from + own_src, dst = to + own_dst;
       const int own_seen = own_row - seen_lo, n_seen = max(seen_hi - seen_lo, 0);
       constexpr int kAtOnce = HD == 256 ? 4 : 2;
@@ -1157,7 +1157,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
           }
         };
         float mt = -INFINITY;
-        if (!KV8 && !edge) {  // FP8: fewer registers a thread
+        if (!edge) {  // all columns on their way at once
           float s[Sh::kScoreCols], top[4];
 #pragma unroll
           for (int x = 0; x < Sh::kScoreCols; x += 32)
