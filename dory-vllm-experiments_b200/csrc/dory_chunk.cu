@@ -580,7 +580,6 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
       }
       const int own = id;
       id = look_up(q + 1, bad);  // in flight while this stage's copies are issued
-      if (!(ok = wait_warp(empty[stage], phase, &c.abort, a.err))) break;
       const uint32_t bar = smem_u32(&full[stage]);
       const uint32_t dst = stages + stage * kBytes;
       const CUtensorMap* map = is_v ? &maps.v : &maps.k;
@@ -601,6 +600,7 @@ __device__ void load_role(const ChunkArgs& a, const Maps& maps, Control<HD, KV8>
           if (r == a.B) r = 0;
         }
       }
+      if (!(ok = wait_warp(empty[stage], phase, &c.abort, a.err))) break;
       if (elect_one()) {
         mbar_expect(bar, kBytes / Sh::kLoaders);
 #pragma unroll
