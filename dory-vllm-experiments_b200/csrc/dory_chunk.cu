@@ -36,9 +36,9 @@
 //
 // What bounds it, measured (CUDA graph, 16-row pages, FP32 gate): long chunks the hand-over
 // between softmax and product warps, tile by tile (prompt of 8192, 32 query heads on 8, 128 dims:
-// 545 us, 1,010 TFLOP/s, 63% of the library GEMM's rate; no exponentials, or half of the
-// products, would save 5-13%); 256-dim heads the page copies as well (16 heads on 4: 690 us, 580
-// with 128-row pages); FP8 caches the conversion (586 us); short items their latency, 4-5 us
+// 535 us, 1,025 TFLOP/s, 64% of the library GEMM's rate; no exponentials, or half of the
+// products, would save 5-13%); 256-dim heads the page copies as well (16 heads on 4: 674 us, 575
+// with 128-row pages); FP8 caches the conversion (589 us); short items their latency, 4-5 us
 // each, and a call of few tokens the chain from launch to join (4 tokens over 640: 16 us).
 
 #include <cuda_bf16.h>
@@ -165,8 +165,8 @@ struct Shape {
   static constexpr int kPartCols = kScoreCols / kParts;
   static constexpr int kSoftmaxWarps = 4 * kShares * kTiles;
   // Copying warps: the 256-dim heads' four stages a tile keep one busier than the products
-  // (16-row pages, prompt of 8192: 777 us, 699 with two); elsewhere the second only takes issue
-  // slots (542 us, 565).
+  // (16-row pages, prompt of 8192: 786 us, 692 with two; four: 662, but 640 in place of 587 with
+  // 128-row pages); elsewhere the second only takes issue slots (542 us, 565).
   static constexpr int kLoaders = HD == 256 && !KV8 ? 2 : 1;
   static constexpr int kLoadWarp = kSoftmaxWarps, kMmaWarp = kLoadWarp + kLoaders,
                        kPlanWarp = kMmaWarp + 1;
