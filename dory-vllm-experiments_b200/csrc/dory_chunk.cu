@@ -93,7 +93,6 @@ struct ChunkArgs {
   int copy_rows;      // rows of a tensor copy: the largest power of two dividing B, up to 128
   int copy_shift;     // its logarithm
   int table_span;     // positions the table names, at most kMaxPosition
-  int min_units;      // cache tiles an SM takes at least
   int32_t* joins;     // [CTAs][8]: the item cut at the end of each CTA's piece
   float2* part_ml;    // [2 CTAs][rows]: (maximum in log2 units, sum of weights)
   float* part_o;      // [2 CTAs][rows][HD]
@@ -349,7 +348,7 @@ __device__ Piece find_piece(const ChunkArgs& a, int lane) {
     mine = head_units(a, sequence(a, i), tokens, lane) * a.NKV;
     total += __reduce_add_sync(0xffffffffu, mine);
   }
-  const int per = max((total + int(gridDim.x) - 1) / int(gridDim.x), a.min_units);
+  const int per = max((total + int(gridDim.x) - 1) / int(gridDim.x), 1);
   const int u0 = min(cta * per, total), u1 = min(u0 + per, total);
   Piece p{u0, u1, per, 0, 0, 0, 0};
   if (u0 < u1) {
@@ -1190,7 +1189,8 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
         }
         if (j == b) {
           m = mt;
-        } else if (__any_sync(0xffffffffu, !(mt <= m + slack))) {  // NaN too
+        } else if (__any_sync(0xffffffffu, live && !(mt <= m + slack))) {  // NaN too
+          // (a row that is none holds whatever was in shared memory: it must not decide)
           const float grown = max2(m, mt);
           const float f = m == -INFINITY ? 0.0f : exp2_approx((m - grown) * sl);
           l *= f;
@@ -1789,7 +1789,6 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   while ((1 << a.copy_shift) < a.copy_rows) ++a.copy_shift;
   const int64_t span = int64_t(p.max_blocks) * p.block_size;
   a.table_span = span < kMaxPosition ? int(span) : kMaxPosition;
-  a.min_units = 1;
   // The device counts units in 32 bits.
   const int64_t most = (int64_t(p.num_tokens) / (a.TB * (p.head_dim == 256 ? 1 : 2)) + p.num_seqs + 1) *
                        (a.table_span / kN + 2 + kItemUnits);

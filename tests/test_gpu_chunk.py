@@ -327,6 +327,24 @@ def test_same_results_every_time_and_per_split():
         assert torch.equal(b.run(), first)
 
 
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+@pytest.mark.parametrize("NH,NKV", [(6, 2), (33, 1), (7, 1)])
+def test_same_results_whatever_ran_before(D, fp8, NH, NKV):
+    """Groups that do not fill a tile's 128 rows: the others hold what shared memory held."""
+    g = torch.Generator().manual_seed(D + NH)
+    lens = [(n, int(n + torch.randint(0, 900, (), generator=g)))
+            for n in torch.randint(1, 90, (40,), generator=g).tolist()]
+    b = Batch(lens, NH=NH, NKV=NKV, D=D, fp8=fp8, seed=40)
+    b.scale *= 4  # maxima that grow past the rescaling's slack here and there
+    attn = b.attention()
+    first = b.run(window=300, gate=b.gate, attn=attn).clone()
+    b.check(first, 300, b.gate)
+    other = Batch([(600, 900)], NH=8, NKV=8, D=D, seed=41, spread=30.0, fp8=fp8)
+    for size in (1.0, 1e3, float("nan"), 1e-3):
+        other.run(q=other.q * size)
+        assert torch.equal(b.run(window=300, gate=b.gate, attn=attn), first), size
+
+
 def test_captured_with_changing_lengths_and_two_instances():
     b = Batch([(40, 500), (8, 700)], NH=16, NKV=4, seed=13)
     attn = b.attention()
