@@ -94,7 +94,9 @@ struct ChunkArgs {
   int copy_shift;     // its logarithm
   int table_span;     // positions the table names, at most kMaxPosition
   int32_t* joins;     // [CTAs][8]: the item cut at the end of each CTA's piece
-  float2* part_ml;    // [2 CTAs][rows]: (maximum in log2 units, sum of weights)
+  // [2 CTAs][rows][shares]: (maximum in log2 units, sum of weights).  One for each softmax
+  // warpgroup of a row: either may compute its columns again (redo_row), against another maximum.
+  float2* part_ml;
   float* part_o;      // [2 CTAs][rows][HD]
 };
 struct Maps {
@@ -954,7 +956,7 @@ struct RowOut {
   __nv_bfloat16* out;  // whole rows
   int64_t gate_at;     // -1: no gate
   float* part_o;       // partial rows
-  float2* part_ml;     // may be null: another warp writes it
+  float2* part_ml;
 };
 template <int HD, bool KV8>
 __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, int head, int lo,
@@ -1015,7 +1017,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
       o.part_o[d] = acc[i];
     }
   }
-  if (o.part_ml && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
+  if (!o.out && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
 }
 
 // Two 16-bit gate values, in g.x, as FP32.
@@ -1395,8 +1397,8 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     else output(std::integral_constant<int, 2>());
     __syncwarp();
     const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
-    if (live && !whole && share == 0)
-      a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl - Sh::kLift, l);
+    if (live && !whole)
+      a.part_ml[slot_row * Sh::kShares + share] = make_float2(m == -INFINITY ? 0.0f : m * sl - Sh::kLift, l);
     uint32_t again = 0;  // rows, as lanes
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1421,7 +1423,7 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       r.out = whole ? a.out + r_token * a.out_t + column : nullptr;
       r.gate_at = a.gate ? r_token * a.gate_t + column : -1;
       r.part_o = a.part_o + r_slot * HD + col0;
-      r.part_ml = !whole && share == 0 ? a.part_ml + r_slot : nullptr;
+      r.part_ml = a.part_ml + r_slot * Sh::kShares + share;
       __syncwarp();
       redo_row<HD, KV8>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
       __syncwarp();
@@ -1558,7 +1560,7 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
       for (int y = 0; y < 4; ++y) {
         ml[y] = make_float2(0.0f, 0.0f);
         if (i + y < parts) {
-          ml[y] = a.part_ml[slot(i + y)];
+          ml[y] = a.part_ml[slot(i + y) * Sh::kShares + lane * Sh::kShares / 32];
           load_row<kPer>(a.part_o + slot(i + y) * HD + lane * kPer, o[y]);
         }
       }
@@ -1590,10 +1592,11 @@ struct ScratchLayout {
 };
 ScratchLayout scratch_layout(int ctas, int head_dim) {
   const int64_t rows = head_dim == 256 ? kM : 2 * kM;
+  const int64_t shares = head_dim == 256 ? kWide256 : kWide128;
   ScratchLayout s;
   s.joins = 256;  // [0, 256): header; word 0 = device error flags
   s.ml = s.joins + (int64_t(ctas) * 32 + 255) / 256 * 256;
-  s.o = s.ml + 2 * ctas * rows * 8;
+  s.o = s.ml + 2 * ctas * rows * shares * 8;
   s.total = s.o + 2 * ctas * rows * head_dim * 4;
   return s;
 }

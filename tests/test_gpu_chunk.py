@@ -404,3 +404,39 @@ def test_refusals():
         ChunkAttention(8, 2, 96, DEV)
     assert (b.out == 5.0).all()
     call(q=b.q[:0], out=b.out[:0])  # nothing to do
+
+
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+@pytest.mark.parametrize("column", [7, 0.75])
+@pytest.mark.parametrize("hidden", [False, True])
+def test_one_bad_value_in_a_cut_item_spoils_its_column_alone(D, fp8, column, hidden):
+    """An item cut between SMs into parts of several tiles, whose maxima keep growing by less than
+    makes O be rescaled, and one NaN in V, in either half of the columns: the rows that see it
+    have that column NaN, and everything else is right, wherever it was computed again."""
+    column = column if isinstance(column, int) else int(column * D)
+    n, length = 20, 40000
+    b = Batch([(n, length)], D=D, fp8=fp8, seed=51)
+    b.q[:, :, 0] = 4.0
+    pos = torch.arange(length, device=DEV)
+    ids = b.tables[0, pos // 16].long()
+    # 1.2 more in log2 units from a tile to the next, six tiles long
+    step = 1.2 / 1.4427 / (4.0 * b.scale * b.scales[0])
+    b.key[ids, pos % 16, :, 0] = (pos // 128 % 6 * step)[:, None].expand(-1, b.NKV).to(b.key.dtype)
+    at = length - 3 if hidden else length // 2
+    row = b.value[ids[at], at % 16]
+    row[1, column] = float("nan")
+    out = b.run().double()
+    k = b.key.float().nan_to_num(0, 0, 0).norm(dim=-1).max().item() * b.scales[0]
+    score = (D + 4) * F32 * b.scale * b.q.float().norm(dim=-1).max().item() * k
+    rel = 2.0 ** -8 + 2 * score + 6e-6 + (8 + length) * F32
+    want, size = b.oracle()
+    tol = rel * size + 2.0 ** -8 * want.abs() * (1 + rel) + 2.0 ** -130
+    if fp8:
+        v = b.value.float().nan_to_num(0, 0, 0).abs().max().item() * b.scales[1]
+        tol = tol + 2.0 ** -32 * length * v
+    spoilt = torch.zeros(b.T, b.NH, D, dtype=torch.bool, device=DEV)
+    spoilt[n - 3 if hidden else 0:, b.NH // b.NKV:, column] = True
+    spoilt = spoilt.view(b.T, -1)
+    assert torch.equal(want.isnan(), spoilt) and torch.equal(out.isnan(), spoilt)
+    off = (out - want).abs()
+    assert (off <= tol)[~spoilt].all(), (off / tol)[~spoilt].max().item()
