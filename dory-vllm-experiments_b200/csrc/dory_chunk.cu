@@ -1005,7 +1005,7 @@ __device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, in
     }
   }
   for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-  const float inv = (KV8 ? a.v_scale : 1.0f) / l;
+  const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;  // 0: it sees nothing
   for (int i = 0; i < HD / 32; ++i) {
     const int d = lane + 32 * i;
     if (d >= cols) break;

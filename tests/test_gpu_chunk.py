@@ -440,3 +440,23 @@ def test_one_bad_value_in_a_cut_item_spoils_its_column_alone(D, fp8, column, hid
     assert torch.equal(want.isnan(), spoilt) and torch.equal(out.isnan(), spoilt)
     off = (out - want).abs()
     assert (off <= tol)[~spoilt].all(), (off / tol)[~spoilt].max().item()
+
+
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+@pytest.mark.parametrize("why", ["short", "blocks"])
+def test_rows_that_see_nothing_are_zero_beside_rows_that_see_a_bad_value(D, fp8, why):
+    b = Batch([(40, 40), (3, 9)], D=D, fp8=fp8, seed=52, poison=False)
+    if why == "short":
+        b.seq_lens[0] = 30  # ten rows before the first position
+        seen = torch.arange(40, device=DEV) - 10
+        errors = 0
+    else:
+        b.tables[0, 0] = b.blocks
+        seen = torch.arange(40, device=DEV) - 16
+        errors = _native.DEVERR_BLOCK_OOB
+    b.value[b.tables[0, 1].long(), 4] = float("nan")  # position 20
+    out = b.run(errors=errors)[:40]
+    assert (out[seen < 0] == 0).all()
+    sees_it = torch.arange(40, device=DEV) - (10 if why == "short" else 0) >= 20
+    assert out[sees_it].isnan().all() and out[~sees_it].isfinite().all()
+    assert (out[(seen >= 0) & ~sees_it] != 0).any()
