@@ -401,6 +401,8 @@ template <int HD, bool KV8>
 __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& p, int lane) {
   const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
   int32_t* join = a.joins + cta * 8;
+  // Before anything can give up: the join must not find an earlier call's record.
+  if (lane == 0) join[0] = 0;
   int queued = 0, turn = 0;
   auto push = [&](const Item& it) {
     const int at = queued % kQueue;
@@ -419,7 +421,6 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& 
   memset(&end, 0, sizeof(end));
   end.flags = kItemEnd;
 
-  int cut = 0;  // whether this CTA holds the first part of a cut item
   if (p.u0 < p.u1) {
     const int u1 = p.u1, per = p.per;
     int seq = p.seq, kvh = p.kvh, m = p.m, off = p.off, first, tiles;
@@ -445,7 +446,6 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& 
         // items of one tile's rows take the two in turn: one's output overlaps the next one
         it.tile = Shape<HD, KV8>::kTiles == 2 && it.ntok <= a.TB ? turn ^= 1 : 0;
         if (!whole && off == 0) {
-          cut = 1;
           if (lane == 0) {
             join[0] = (at + work - 1) / per - cta + 1;  // CTAs that hold a part
             join[1] = it.tok0;
@@ -466,7 +466,6 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& 
       }
     }
   }
-  if (!cut && lane == 0) join[0] = 0;
   if (cta == 0)  // lengths beyond the block table
     for (int i = lane; i < a.S; i += 32)
       if (a.seq_lens[i] > a.table_span && sequence(a, i).n) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
@@ -1541,7 +1540,7 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
   for (int r = blockIdx.y * 16 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 16 * kJoinSlices) {
     const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
     const int tok = t * a.TB + row_tok;
-    if (in_tile >= a.TB * a.G || tok >= ntok) continue;
+    if (in_tile >= a.TB * a.G || tok >= ntok || tok0 + tok >= a.T) continue;
     auto slot = [&](int i) {
       return int64_t(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * Sh::kItemRows + r;
     };
