@@ -205,7 +205,7 @@ struct Control {  // shared memory behind the tiles
   alignas(8) uint64_t kv_full[Shape<HD, KV8>::kStages], kv_empty[Shape<HD, KV8>::kStages];
   uint64_t raw_full[4], raw_empty[4], q_raw[2];  // FP8 caches only
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], item_full[kQueue],
-      item_empty[kQueue], drained;
+      item_empty[kQueue], met[4 * Shape<HD, KV8>::kTiles], drained;
   Item items[kQueue];
   uint32_t bad[kBadRing];
   // what a row's f16 query was divided by; a second set for the tile's next item, which the
@@ -1045,8 +1045,15 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
   constexpr bool kTwo = Sh::kTiles == 2;
   const int quad = warp & 3, row = quad * 32 + lane;
   const int t = (warp >> 2) / Sh::kShares, share = (warp >> 2) % Sh::kShares;
-  // the warps that share rows, of one tile
-  auto meet = [&]() { named_barrier(1 + t * 4 + quad, Sh::kShares * 32); };
+  // The warps that share rows, of one tile: a wait like any other, so that one of them can give up
+  // (a block barrier would keep the other for good).
+  uint32_t met = 0;
+  auto meet = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&c.met[t * 4 + quad]));
+    met ^= 1;
+    return wait_warp(c.met[t * 4 + quad], met ^ 1, &c.abort, a.err);
+  };
   const uint32_t tmem = c.tmem + (uint32_t(quad * 32) << 16);
   const uint32_t o_addr = tmem + Sh::kO + t * Sh::kOStride + share * Sh::kOutCols;
   const uint32_t stages = tiles + Sh::kQBytes;
@@ -1183,10 +1190,10 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
         }
         if constexpr (Sh::kShares > 1) {  // the rest of the row's columns
           c.swap[t][share][row] = mt;
-          meet();
+          if (!meet()) return;
 #pragma unroll
           for (int x = 1; x < Sh::kShares; ++x) mt = max2(mt, c.swap[t][(share + x) % Sh::kShares][row]);
-          if (!kTwo) meet();  // a warp may go on to the next tile while another still reads
+          if (!kTwo && !meet()) return;  // a warp may go on to the next tile while another still reads
         }
         if (j == b) {
           m = mt;
@@ -1275,10 +1282,10 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
       // the sums of the shares; each warp is past its last tile's maxima: the sum just waited for
       // needed every share's weights
       c.swap[t][share][row] = l;
-      meet();
+      if (!meet()) return;
 #pragma unroll
       for (int x = 1; x < Sh::kShares; ++x) l += c.swap[t][(share + x) % Sh::kShares][row];
-      meet();
+      if (!meet()) return;
     }
     // Opaque here, or the compiler computes everything below that depends on them alone once,
     // ahead of the items, and spills it across the loop over the tiles.
@@ -1463,6 +1470,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
       mbar_init(smem_u32(&c.item_full[i]), 1);
       mbar_init(smem_u32(&c.item_empty[i]), Sh::kSoftmaxWarps + Sh::kLoaders + 1 + Sh::kConvertWarps);
     }
+    for (int i = 0; i < 4 * Sh::kTiles; ++i) mbar_init(smem_u32(&c.met[i]), Sh::kShares);
     mbar_init(smem_u32(&c.drained), 1);
     c.abort = c.redone = 0;
     fence_mbar_init();

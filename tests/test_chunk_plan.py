@@ -173,3 +173,23 @@ def test_an_empty_batch_leaves_no_record(plan):
     for seqs in ([(0, 0)], [(0, 100), (0, 5)]):
         T, joins = plan(128, 9, 100, 2, 32, 0, seqs)
         assert T == 0 and all(parts == 0 for parts, *_ in joins)
+
+
+def test_no_role_waits_without_a_limit():
+    """A role that gives up leaves its loop, so nothing inside the roles may wait for another warp
+    except through an mbarrier with a limit: the only block barriers are the kernel's own, before
+    the roles and after them."""
+    text = SOURCE.read_text()
+    header = (SOURCE.parent / "dory_sm100.cuh").read_text()
+    for name in ("bar.sync", "barrier.sync", "barrier.cta", "named_barrier", "cooperative_groups"):
+        assert name not in text and name not in header, name
+    kernel = between(text, "    chunk_kernel(const __grid_constant__", "template <int N>")
+    assert text.count("__syncthreads()") == kernel.count("__syncthreads()") == 2
+    # a failed wait is never ignored: every call of these is tested
+    for line in text.split("\n"):
+        code = line.split("//")[0].strip()
+        if code.startswith(("meet()", "wait_warp(", "wait_bar(", "wait_sum(", "wait_stage(")):
+            assert False, line
+    # and every spin on a barrier has the clock in its condition or body
+    for at in [i for i in range(len(text)) if text.startswith("while (!mbar_try", i)]:
+        assert "clock64()" in text[at:at + 260], text[at:at + 80]
