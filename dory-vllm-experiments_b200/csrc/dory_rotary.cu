@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
 }
 
 // ------------------------------------------------------------------------------------
-// The rotated element i of a row.
+// The rotated element i of a row: the product and the fused sum that rotary_vec forms, so that a
+// row's bits do not depend on its strides.
 template <typename T>
 __device__ __forceinline__ float turned(const RotaryArgs& a, const T* x, int i, int64_t pos) {
   if (i >= a.R) return to_f32(x[i]);
@@ -387,7 +388,8 @@ __device__ __forceinline__ float turned(const RotaryArgs& a, const T* x, int i, 
   const int i0 = a.inter ? 2 * pair : pair, i1 = a.inter ? 2 * pair + 1 : pair + half;
   const float c = load_as_f32(a.cos_sin, pos * a.R + pair, a.cs_dtype);
   const float s = a.sign * load_as_f32(a.cos_sin, pos * a.R + half + pair, a.cs_dtype);
-  return first ? to_f32(x[i0]) * c - to_f32(x[i1]) * s : to_f32(x[i1]) * c + to_f32(x[i0]) * s;
+  return first ? __fmaf_rn(-to_f32(x[i1]), s, __fmul_rn(to_f32(x[i0]), c))
+               : __fmaf_rn(to_f32(x[i0]), s, __fmul_rn(to_f32(x[i1]), c));
 }
 
 template <typename T, bool APPEND, bool KV8>

@@ -377,3 +377,26 @@ def test_append_offsets_pass_32_bits(D, dim_step):
         assert torch.equal(c[69, 15], rows[0]) and torch.equal(c[0, 3], rows[1])
         assert torch.equal(c[5, 0], rows[2])
         assert (c[69, :15] == 5.0).all() and (c[5, 1:] == 5.0).all() and (c[0, 4:] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_off_the_16_byte_grid_give_the_same_bits(dtype, interleaved):
+    T, NH, NKV, D, R = 1500, 4, 2, 128, 96
+    qkv, pos, table = inputs(T, NH, NKV, D, R, dtype, seed=24)
+    d, p, cs = qkv.to(DEV), pos.to(DEV), table.to(DEV)
+    odd = torch.zeros(T, (NH + 2 * NKV) * D + 1, dtype=d.dtype, device=DEV)[:, 1:].unflatten(1, (-1, D))
+    odd.copy_(d)
+    outs = []
+    for x in (d, odd):
+        q, k, v = x.split([NH, NKV, NKV], dim=1)
+        qo, ko = torch.empty_like(q, memory_format=torch.contiguous_format), \
+            torch.empty_like(k, memory_format=torch.contiguous_format)
+        rotary_embed(q, k, p, cs, qo, ko, interleaved=interleaved)
+        key = torch.zeros(T // 16 + 1, 16, NKV, D, dtype=torch.bfloat16, device=DEV)
+        value, qb = key.clone(), torch.empty(T, NH, D, dtype=torch.bfloat16, device=DEV)
+        rotary_append(q, k, v, p, cs, torch.arange(T, device=DEV), key, value, qb,
+                      interleaved=interleaved)
+        outs.append((qo, ko, key, value, qb))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
