@@ -145,6 +145,19 @@ __device__ __forceinline__ int64_t slot_offset(const RotaryArgs& a, int64_t slot
   return block * a.sb + (slot - block * a.B) * a.so;
 }
 
+// The factor that the decode calls and qk_norm_cache normalise a row with, so that a row's bits do
+// not depend on the call that appends it: the FP64 sum of squares rounded to FP32, eps added there,
+// and 1 / sqrt of that, correctly rounded.  With y near 1 / sqrt(t) and e = 1 - t y^2, 1 / sqrt(t) =
+// y / sqrt(1 - e) = y (1 + e / 2 + 3 e^2 / 8 + ..); |e| < 2^-21, so what is left out is below 2^-64.
+// A sum beyond FP32 gives 0.  The wider sum and root cost a long append issue slots (8192 tokens: 46
+// us; 40 with both in FP32, whose rows differed in their last bits from those of the other calls).
+__device__ __forceinline__ float inv_norm(double sum, float eps) {
+  const float t = __fadd_rn(__double2float_rn(sum), eps);
+  const double y = double(rsqrtf(t)), e = fma(-double(t), y * y, 1.0);
+  const float inv = __double2float_rn(fma(y, e * fma(e, 0.375, 0.5), y));
+  return isinf(t) ? 0.0f : inv;
+}
+
 // Row h of a token: 0 .. NH-1 q, then k heads, then (append) v heads.
 template <typename T>
 __device__ __forceinline__ const T* row_in(const RotaryArgs& a, int t, int h) {
@@ -324,20 +337,23 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
     }
     if constexpr (APPEND) {
       if (a.norm) {  // every lane of the warp takes part: rows never straddle a warp
-        uint64_t squares = mul2(y[0], y[0]);
+        double sum = 0.0, other = 0.0;
 #pragma unroll
-        for (int j = 1; j < 8; ++j) squares = fma2(y[j], y[j], squares);
-        float sum, other;
-        split(squares, sum, other);
+        for (int j = 0; j < 8; ++j) {
+          float u, w;
+          split(y[j], u, w);
+          sum += double(u) * double(u);
+          other += double(w) * double(w);
+        }
         sum += other;
         if (lanes > 8) sum += __shfl_xor_sync(0xffffffffu, sum, 8);  // 4, 8 or 16 lanes a row
         if (lanes > 4) sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         if (!is_v && known) {  // zeros stay zeros, whatever eps
-          const float inv = rsqrtf(sum + a.eps);
+          const float inv = inv_norm(sum, a.eps);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = mul2(y[j], mul2(weight[j], pair(inv, inv)));
+          for (int j = 0; j < 8; ++j) y[j] = mul2(weight[j], mul2(y[j], pair(inv, inv)));
         }
       }
     }
@@ -429,13 +445,13 @@ __global__ void __launch_bounds__(128) rotary_any(const RotaryArgs a) {
     }
     float inv = 1.0f;
     if (a.norm && !is_v) {
-      float sum = 0.0f;
+      double sum = 0.0;
       for (int i = lane; i < a.D; i += 32) {
-        const float y = inside ? turned(a, x, i, pos) : 0.0f;
+        const double y = inside ? turned(a, x, i, pos) : 0.0f;
         sum += y * y;
       }
       for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-      if (inside) inv = rsqrtf(sum + a.eps);
+      if (inside) inv = inv_norm(sum, a.eps);
     }
     if (h >= a.NH && slot < 0) return;
     const int g = is_v ? h - a.NH - a.NKV : h - a.NH;
@@ -445,12 +461,11 @@ __global__ void __launch_bounds__(128) rotary_any(const RotaryArgs a) {
     for (int i = lane; i < a.D; i += 32) {
       float y = is_v ? to_f32(x[i]) : inside ? turned(a, x, i, pos) : 0.0f;
       if (a.norm && !is_v) {
-        float f = inv;
+        y *= inv;
         if (h < a.NH) {
           const float u = load_as_f32(a.sqk, int64_t(h) * a.D + i, a.sqk_dtype) * a.sqk_factor;
-          f *= u * u;
+          y = u * u * y;
         }
-        y *= f;
       }
       if (h < a.NH)
         (static_cast<__nv_bfloat16*>(a.q.out) + t * a.q.out_t + h * a.q.out_h)[i] =

@@ -368,7 +368,8 @@ int32_t dory_residual_update(const DoryResidualParams* params, void* stream);
  * dory_rotary_append writes q_out (BF16; q and q_out may be NULL) and the cache rows of k and
  * v at slot_mapping[t] (negative: a padding token, no row is written; outside the cache:
  * reported as DORY_DEVERR_SLOT_OOB and skipped).  With DORY_ROTARY_NORM the rotated q and k
- * are brought to unit length first, as the raw decode calls do:
+ * are brought to unit length first, to the bits of the raw decode calls and dory_qk_norm_cache (the
+ * sum of squares in FP64, rounded to FP32 before eps, and its inverse root correctly rounded):
  *   q_out = bf16((float(sqk[h]) * sqk_factor)^2 * q * rsqrt(sum q^2 + eps)),
  *   k     = bf16(k * rsqrt(sum k^2 + eps)).
  * BF16 caches take bf16(k), bf16(v); FP8 caches e4m3(bf16(k) / k_scale), e4m3(bf16(v) /

@@ -283,3 +283,39 @@ assert torch.equal(out, first) and out.any()
 def test_the_first_call_may_be_a_captured_one():
     package = str(Path(__file__).resolve().parents[1] / "dory-vllm-experiments_b200")
     subprocess.run([sys.executable, "-c", FIRST.format(package=package)], check=True, timeout=300)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_the_decode_call_appends_the_prompt_paths_row(D, fp8):
+    """DecodeAttention.from_raw on the FP32 rows that rotary_embed turned, and rotary_append on the
+    rows themselves, leave the same bytes in the cache, everywhere."""
+    from dory_rotary_steps import rotary_append, rotary_embed
+    if fp8 and D == 64:
+        pytest.skip("no FP8 caches of 64-dim heads")
+    g = torch.Generator(device=DEV).manual_seed(12)
+    n, steps = 16, 64
+    cos_sin = rotary_cos_sin(n + 1, D, device=DEV)
+    sqk = (torch.rand(NH * D, generator=g, device=DEV) + 0.5).to(torch.bfloat16)
+    attn = DecodeAttention(NH, NKV, D, DEV, kv_cache_dtype="fp8" if fp8 else "auto")
+    ks, vs = (0.02, 0.03) if fp8 else (1.0, 1.0)
+    kind = torch.uint8 if fp8 else torch.bfloat16
+    table = torch.tensor([1, 0], dtype=torch.int32, device=DEV)
+    at, slot = torch.tensor([n], device=DEV), torch.tensor([0], device=DEV)
+    for _ in range(steps):
+        x = torch.randn(1, NH + 2 * NKV, D, generator=g, device=DEV) * 3
+        q, k, v = x.split([NH, NKV, NKV], dim=1)
+        caches = [torch.randint(0, 100, (2, 16, NKV, D), generator=g, device=DEV).to(kind)
+                  for _ in range(2)]
+        mine = [c.clone() for c in caches]
+        rotary_append(q, k, v, at, cos_sin, slot, *mine, torch.empty(1, NH, D, dtype=torch.bfloat16,
+                                                                     device=DEV),
+                      sqk=sqk, sqk_factor=FACTOR, k_scale=ks, v_scale=vs)
+        turned = x[:, :NH + NKV].contiguous()
+        rotary_embed(q, k, at, cos_sin, turned[:, :NH], turned[:, NH:])
+        attn.from_raw(turned.view(-1), v.reshape(-1), sqk, FACTOR, EPS, slot, *caches, table,
+                      torch.tensor([n + 1], dtype=torch.int32, device=DEV), 0, 0.1,
+                      torch.ones(NH * D, device=DEV), torch.empty(8, NH * D // 8, device=DEV),
+                      k_scale=ks, v_scale=vs)
+        attn.check_errors()
+        assert all(torch.equal(a, b) for a, b in zip(mine, caches))

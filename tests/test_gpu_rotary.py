@@ -400,3 +400,62 @@ def test_rows_off_the_16_byte_grid_give_the_same_bits(dtype, interleaved):
         outs.append((qo, ko, key, value, qb))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,R", [(64, 64), (128, 128), (128, 0), (256, 64), (128, 34)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_leaves_the_bits_of_the_other_normalising_calls(D, R, interleaved):
+    """The rotated FP32 rows through qk_norm_cache give the query and the cache rows bit for bit."""
+    from dory_sublayer_steps import qk_norm_cache
+    T, NH, NKV = 1500, 4, 2
+    qkv, pos, table = inputs(T, NH, NKV, D, R or 2, "f32", seed=21)
+    d = qkv.to(DEV)
+    # rows of many sizes, so that sums of squares come near every kind of rounding
+    d[:, :NH + NKV] *= torch.exp2(torch.randint(-9, 9, (T, NH + NKV, 1), device=DEV).float())
+    cs, p = table.to(DEV), pos.to(DEV)
+    sqk = (torch.rand(NH * D, generator=torch.Generator().manual_seed(22)) + 0.5).to(DEV)
+    slots = torch.randperm(T, generator=torch.Generator().manual_seed(23)).to(DEV)
+    turned = d[:, :NH + NKV].contiguous()
+    if R:
+        rotary_embed(d[:, :NH], d[:, NH:NH + NKV], p, cs, turned[:, :NH], turned[:, NH:],
+                     interleaved=interleaved)
+    caches = [torch.zeros(T // 16 + 1, 16, NKV, D, dtype=torch.bfloat16, device=DEV) for _ in range(4)]
+    q_out = [torch.empty(T, NH * D, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    qk_norm_cache(turned.view(T, -1), d[:, NH + NKV:].reshape(T, -1).contiguous(), sqk, 0.7, 1e-6, q_out[0], NH, D,
+                  key_cache=caches[0], value_cache=caches[1], slot_mapping=slots)
+    rotary_append(d[:, :NH], d[:, NH:NH + NKV], d[:, NH + NKV:], p, cs if R else None, slots,
+                  caches[2], caches[3], q_out[1], sqk=sqk, sqk_factor=0.7, eps=1e-6,
+                  interleaved=interleaved)
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+    assert torch.equal(q_out[0], q_out[1])
+
+
+@pytest.mark.parametrize("D,R", [(128, 128), (64, 24)])  # the wide kernel, and the general one
+def test_a_norm_beyond_fp32_gives_zeros(D, R):
+    """The sum of squares is an FP32 value: infinite from rows of 1e20 on."""
+    x = torch.full((1, 3, D), 1e20, device=DEV)
+    key = torch.full((1, 16, 1, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    value, q_out = key.clone(), torch.empty(1, 1, D, dtype=torch.bfloat16, device=DEV)
+    rotary_append(x[:, :1], x[:, 1:2], x[:, 2:], torch.tensor([0], device=DEV),
+                  rotary_cos_sin(8, R, device=DEV), torch.tensor([0], device=DEV), key, value, q_out,
+                  sqk=torch.ones(D, device=DEV))
+    assert (q_out == 0).all() and (key[0, 0] == 0).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_normalised_rows_off_the_16_byte_grid_give_the_same_bits(interleaved):
+    T, NH, NKV, D, R = 1500, 4, 2, 128, 96
+    qkv, pos, table = inputs(T, NH, NKV, D, R, "f32", seed=25)
+    d, p, cs = qkv.to(DEV), pos.to(DEV), table.to(DEV)
+    odd = torch.zeros(T, (NH + 2 * NKV) * D + 1, device=DEV)[:, 1:].unflatten(1, (-1, D))
+    odd.copy_(d)
+    outs = []
+    for x in (d, odd):
+        key = torch.zeros(T // 16 + 1, 16, NKV, D, dtype=torch.bfloat16, device=DEV)
+        value, q_out = key.clone(), torch.empty(T, NH, D, dtype=torch.bfloat16, device=DEV)
+        rotary_append(*x.split([NH, NKV, NKV], dim=1), p, cs, torch.arange(T, device=DEV), key, value,
+                      q_out, sqk=torch.full((NH * D,), 1.3, device=DEV), sqk_factor=0.7,
+                      interleaved=interleaved)
+        outs.append((key, value, q_out))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
