@@ -31,8 +31,9 @@
 //
 // Positions no row of the item sees (behind the sequence, before the window) may hold anything,
 // so their V rows are zeroed in shared memory (0 x NaN would reach the sum).  A position that
-// some rows see and others do not can still hold Inf or NaN: a row whose O comes out
-// non-finite from finite weights is recomputed from its own positions alone (redo_row).
+// some rows see and others do not can still hold Inf or NaN: a row whose O comes out non-finite
+// from finite weights is looked at by the join kernel, which computes it again from its own
+// positions alone if it took part in a product with such a position without seeing it.
 //
 // What bounds it, measured (CUDA graph, 16-row pages, FP32 gate): long chunks the hand-over
 // between softmax and product warps, tile by tile (prompt of 8192, 32 query heads on 8, 128 dims:
@@ -73,7 +74,7 @@ constexpr int kQueue = 4;            // items handed out ahead
 constexpr int kBadRing = 16;         // tiles whose bad-page masks are kept
 constexpr int kMaxPosition = 1 << 30;
 constexpr float kSlack = 8.0f;       // log2 a row's maximum may grow before O is rescaled
-// ~2 s without a row of redo_row done meanwhile (the other roles wait for those), then give up.
+// ~2 s, then give up.
 constexpr long long kWaitLimitCycles = 4000000000LL;
 
 struct ChunkArgs {
@@ -93,10 +94,8 @@ struct ChunkArgs {
   int copy_rows;      // rows of a tensor copy: the largest power of two dividing B, up to 128
   int copy_shift;     // its logarithm
   int table_span;     // positions the table names, at most kMaxPosition
-  int32_t* joins;     // [CTAs][8]: the item cut at the end of each CTA's piece
-  // [2 CTAs][rows][shares]: (maximum in log2 units, sum of weights).  One for each softmax
-  // warpgroup of a row: either may compute its columns again (redo_row), against another maximum.
-  float2* part_ml;
+  int32_t* joins;     // [CTAs][8] (Join): what each CTA leaves to the join kernel
+  float2* part_ml;    // [2 CTAs][rows]: (maximum in log2 units, sum of weights)
   float* part_o;      // [2 CTAs][rows][HD]
 };
 struct Maps {
@@ -116,13 +115,21 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(two_bytes)));
   return r;
 }
-__device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(e4m3x2_to_f16x2(b))));
-}
-template <bool KV8>
-__device__ __forceinline__ float cache_value(const void* p, int64_t i) {
-  if (KV8) return e4m3_to_f32(static_cast<const uint8_t*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// The first N values of a cache row's words.
+template <bool KV8, int N>
+__device__ __forceinline__ void unpack(const uint32_t* words, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    if (KV8) {
+      const uint32_t h = e4m3x2_to_f16x2(words[i / 4] >> (8 * (i % 4)) & 0xffffu);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      x[i] = f.x;
+      x[i + 1] = f.y;
+    } else {
+      x[i] = __uint_as_float(words[i / 2] << 16);
+      x[i + 1] = __uint_as_float(words[i / 2] & 0xffff0000u);
+    }
+  }
 }
 
 // Rows [t0, t1) of sequence i, whatever the arrays hold: always within [0, T].
@@ -212,25 +219,18 @@ struct Control {  // shared memory behind the tiles
   // conversion may reach while softmax warps are still at the output of the item before
   float q_scale[2][KV8 ? Shape<HD, KV8>::kItemRows : 1];
   uint32_t tmem;
-  int abort, redone;  // redone: counts the rows of redo_row
+  int abort;
   // a row's maxima and sums, by share
   float swap[Shape<HD, KV8>::kTiles][Shape<HD, KV8>::kShares][Shape<HD, KV8>::kShares > 1 ? kM : 1];
 };
 
-// abort: Control's abort and redone.
 __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort,
                                        uint32_t* err) {
-  long long start = clock64();
-  int redone = abort[1];
+  const long long start = clock64();
   while (!mbar_try(bar, parity)) {
-    if (abort[0]) return false;
+    if (*abort) return false;
     if (clock64() - start > kWaitLimitCycles) {
-      if (redone != abort[1]) {
-        redone = abort[1];
-        start = clock64();
-        continue;
-      }
-      abort[0] = 1;
+      *abort = 1;
       atomicOr(err, DORY_DEVERR_WAIT_TIMEOUT);
       return false;
     }
@@ -397,13 +397,62 @@ __device__ Piece find_piece(const ChunkArgs& a, int lane) {
   return p;
 }
 
+// The parts of items that make up a piece, in order: f(item, its cache tiles or 1, its first unit's
+// number), until it returns false.
+template <int HD, bool KV8, class F>
+__device__ __forceinline__ void walk(const ChunkArgs& a, const Piece& p, F f) {
+  const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
+  if (p.u0 >= p.u1) return;
+  const int u1 = p.u1;
+  int seq = p.seq, kvh = p.kvh, m = p.m, off = p.off, turn = 0, first, tiles;
+  Seq s = sequence(a, seq);
+#pragma unroll 1
+  for (int at = p.u0; at < u1;) {
+    const int units = item_units(a, s, m, tokens, first, tiles);
+    const int take = min(units - off, u1 - at);
+    const int work = units - kItemUnits;  // cache tiles, or 1
+    if (off < work) {
+      Item it;
+      it.flags = 0;
+      it.kv0 = first + off;
+      it.kvn = tiles ? min(take, work - off) : 0;
+      it.tok0 = s.t0 + m * tokens;
+      it.ntok = min(tokens, s.n - m * tokens);
+      it.pos0 = s.pos + m * tokens;
+      it.kvh = kvh;
+      it.seq = seq;
+      it.cap = s.cap;
+      it.slot = off == 0 ? (take >= work ? -1 : 2 * cta + 1) : 2 * cta;
+      // items of one tile's rows take the two in turn: one's output overlaps the next one
+      it.tile = Shape<HD, KV8>::kTiles == 2 && it.ntok <= a.TB ? turn ^= 1 : 0;
+      if (!f(it, work, at)) return;
+    }
+    at += take;
+    off = 0;
+    if (++m * tokens >= s.n) {
+      m = 0;
+      if (++kvh == a.NKV) {
+        kvh = 0;
+        if (at < u1) do s = sequence(a, ++seq); while (s.n == 0 && seq < a.S);
+      }
+    }
+  }
+}
+
+// What a CTA leaves to the join kernel: the item whose first part ends its piece, and whether a
+// row of an item that it holds whole came out non-finite from finite weights.
+struct Join {
+  int32_t parts, tok0, ntok, kvh;  // parts: CTAs that hold one; 0: no item
+  int32_t odd, seq, pos0, cap;
+};
+
 template <int HD, bool KV8>
 __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& p, int lane) {
-  const int tokens = Shape<HD, KV8>::kTiles * a.TB, cta = blockIdx.x;
-  int32_t* join = a.joins + cta * 8;
+  const int cta = blockIdx.x;
+  Join* const join = reinterpret_cast<Join*>(a.joins) + cta;
   // Before anything can give up: the join must not find an earlier call's record.
-  if (lane == 0) join[0] = 0;
-  int queued = 0, turn = 0;
+  if (lane == 0) join->parts = join->odd = 0;
+  int queued = 0;
   auto push = [&](const Item& it) {
     const int at = queued % kQueue;
     if (queued >= kQueue &&
@@ -417,58 +466,26 @@ __device__ void plan_role(const ChunkArgs& a, Control<HD, KV8>& c, const Piece& 
     ++queued;
     return true;
   };
-  Item end;
-  memset(&end, 0, sizeof(end));
-  end.flags = kItemEnd;
-
-  if (p.u0 < p.u1) {
-    const int u1 = p.u1, per = p.per;
-    int seq = p.seq, kvh = p.kvh, m = p.m, off = p.off, first, tiles;
-    Seq s = sequence(a, seq);
-#pragma unroll 1
-    for (int at = p.u0; at < u1;) {
-      const int units = item_units(a, s, m, tokens, first, tiles);
-      const int take = min(units - off, u1 - at);
-      const int work = units - kItemUnits;  // cache tiles, or 1
-      if (off < work) {
-        const bool whole = off == 0 && take >= work;
-        Item it;
-        it.flags = 0;
-        it.kv0 = first + off;
-        it.kvn = tiles ? min(take, work - off) : 0;
-        it.tok0 = s.t0 + m * tokens;
-        it.ntok = min(tokens, s.n - m * tokens);
-        it.pos0 = s.pos + m * tokens;
-        it.kvh = kvh;
-        it.seq = seq;
-        it.cap = s.cap;
-        it.slot = whole ? -1 : (off == 0 ? 2 * cta + 1 : 2 * cta);
-        // items of one tile's rows take the two in turn: one's output overlaps the next one
-        it.tile = Shape<HD, KV8>::kTiles == 2 && it.ntok <= a.TB ? turn ^= 1 : 0;
-        if (!whole && off == 0) {
-          if (lane == 0) {
-            join[0] = (at + work - 1) / per - cta + 1;  // CTAs that hold a part
-            join[1] = it.tok0;
-            join[2] = it.ntok;
-            join[3] = kvh;
-          }
-        }
-        if (!push(it)) return;
-      }
-      at += take;
-      off = 0;
-      if (++m * tokens >= s.n) {
-        m = 0;
-        if (++kvh == a.NKV) {
-          kvh = 0;
-          if (at < u1) do s = sequence(a, ++seq); while (s.n == 0 && seq < a.S);
-        }
-      }
+  bool ok = true;
+  walk<HD, KV8>(a, p, [&](const Item& it, int work, int at) {
+    if (it.slot == 2 * cta + 1 && lane == 0) {
+      join->parts = (at + work - 1) / p.per - cta + 1;
+      join->tok0 = it.tok0;
+      join->ntok = it.ntok;
+      join->kvh = it.kvh;
+      join->seq = it.seq;
+      join->pos0 = it.pos0;
+      join->cap = it.cap;
     }
-  }
+    return ok = push(it);
+  });
+  if (!ok) return;
   if (cta == 0)  // lengths beyond the block table
     for (int i = lane; i < a.S; i += 32)
       if (a.seq_lens[i] > a.table_span && sequence(a, i).n) atomicOr(a.err, DORY_DEVERR_BLOCK_OOB);
+  Item end;
+  memset(&end, 0, sizeof(end));
+  end.flags = kItemEnd;
   push(end);
 }
 
@@ -949,76 +966,6 @@ __device__ bool mma_items(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t tile
 }
 
 // ---- softmax ----
-// One row from its own positions [lo, hi) alone, by the warp: the row's partial result, or
-// its output.  Slow; for rows whose sum came out non-finite.
-struct RowOut {
-  __nv_bfloat16* out;  // whole rows
-  int64_t gate_at;     // -1: no gate
-  float* part_o;       // partial rows
-  float2* part_ml;
-};
-template <int HD, bool KV8>
-__device__ __noinline__ void redo_row(const ChunkArgs& a, int seq, int token, int head, int lo,
-                                      int hi, int col0, int cols, RowOut o) {
-  const int lane = threadIdx.x & 31;
-  const __nv_bfloat16* q = a.q + token * a.q_t + head * a.q_h;
-  const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
-  const int64_t kv = int64_t(head / a.G) * a.sh;
-  const float qk = a.scale_log2 * (KV8 ? a.k_scale : 1.0f);
-  float m = -INFINITY, l = 0.0f, acc[HD / 32];
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) acc[i] = 0.0f;
-#pragma unroll 1
-  for (int c0 = lo; c0 < hi; c0 += 32) {
-    const int c = c0 + lane;
-    float s = -INFINITY;
-    int64_t at = -1;
-    if (c < hi) {
-      const int64_t id = block_of(a, table, c);
-      if (id >= 0) {
-        at = id * a.sb + int64_t(c % a.B) * a.so + kv;
-        float dot = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < HD; ++i) dot += __bfloat162float(q[i]) * cache_value<KV8>(a.kc, at + i);
-        s = dot * qk;
-      }
-    }
-    float top = s;
-    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
-    const float w = exp2f(s - base), shrink = exp2f(m - base);
-    m = m_new;
-    l = l * shrink + w;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] *= shrink;
-#pragma unroll 1
-    for (int k = 0; k < 32; ++k) {
-      const int64_t row = __shfl_sync(0xffffffffu, at, k);
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      if (row < 0) continue;
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        const int d = lane + 32 * i;
-        if (d < cols) acc[i] += wk * cache_value<KV8>(a.vc, row + col0 + d);
-      }
-    }
-  }
-  for (int k = 16; k; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-  const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;  // 0: it sees nothing
-  for (int i = 0; i < HD / 32; ++i) {
-    const int d = lane + 32 * i;
-    if (d >= cols) break;
-    if (o.out) {
-      float y = acc[i] * inv;
-      if (o.gate_at >= 0) y *= load_gate(a, o.gate_at + d);
-      o.out[d] = __float2bfloat16_rn(y);
-    } else {
-      o.part_o[d] = acc[i];
-    }
-  }
-  if (!o.out && lane == 0) *o.part_ml = make_float2(m == -INFINITY ? 0.0f : m, l);
-}
-
 // Two 16-bit gate values, in g.x, as FP32.
 __device__ __forceinline__ void widen2(bool bf16, uint2& g) {
   const uint32_t w = g.x;
@@ -1403,37 +1350,19 @@ __device__ void softmax_role(const ChunkArgs& a, Control<HD, KV8>& c, uint32_t t
     else output(std::integral_constant<int, 2>());
     __syncwarp();
     const int64_t slot_row = int64_t(max(it.slot, 0)) * Sh::kItemRows + own_row;
-    if (live && !whole)
-      a.part_ml[slot_row * Sh::kShares + share] = make_float2(m == -INFINITY ? 0.0f : m * sl - Sh::kLift, l);
-    uint32_t again = 0;  // rows, as lanes
+    if (live && !whole && share == 0)
+      a.part_ml[slot_row] = make_float2(m == -INFINITY ? 0.0f : m * sl - Sh::kLift, l);
+    if (whole) {  // (parts: the join kernel sees for itself)
+      bool again = false;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float odd0, odd1;
-      split(odd[r], odd0, odd1);
-      const uint32_t lanes = __ballot_sync(0xffffffffu, isnan(odd0) || isnan(odd1));
-      if (lanes)
-        for (int y = 0; y < 8; ++y)
-          if (lanes >> (4 * y) & 15) again |= 1u << (8 * r + y);
-    }
-    again &= __ballot_sync(0xffffffffu, live && isfinite(l));
-    while (again) {
-      const int src = __ffs(again) - 1;
-      again &= again - 1;
-      const int r_token = it.tok0 + __shfl_sync(0xffffffffu, tok, src);
-      const int r_head = it.kvh * a.G + __shfl_sync(0xffffffffu, row_head, src);
-      const int lo = max(__shfl_sync(0xffffffffu, see_lo, src), it.kv0 * kN);
-      const int hi = min(__shfl_sync(0xffffffffu, see_hi, src) + 1, (it.kv0 + it.kvn) * kN);
-      const int64_t r_slot = __shfl_sync(0xffffffffu, slot_row, src);
-      const int64_t column = int64_t(r_head) * HD + col0;
-      RowOut r;
-      r.out = whole ? a.out + r_token * a.out_t + column : nullptr;
-      r.gate_at = a.gate ? r_token * a.gate_t + column : -1;
-      r.part_o = a.part_o + r_slot * HD + col0;
-      r.part_ml = a.part_ml + r_slot * Sh::kShares + share;
-      __syncwarp();
-      redo_row<HD, KV8>(a, it.seq, r_token, r_head, lo, hi, col0, Sh::kOutCols, r);
-      __syncwarp();
-      if (lane == 0) atomicAdd(&c.redone, 1);
+      for (int r = 0; r < 4; ++r) {
+        float odd0, odd1;
+        split(odd[r], odd0, odd1);
+        const float sum = __shfl_sync(0xffffffffu, l, 8 * r + (own_lane >> 2));
+        again |= (isnan(odd0) || isnan(odd1)) && (alive >> r & 1) && isfinite(sum);
+      }
+      if (__any_sync(0xffffffffu, again) && lane == 0)
+        reinterpret_cast<Join*>(a.joins)[blockIdx.x].odd = 1;
     }
     done();
   }
@@ -1472,7 +1401,7 @@ __global__ void __launch_bounds__(Shape<HD, KV8>::kThreads, 1)
     }
     for (int i = 0; i < 4 * Sh::kTiles; ++i) mbar_init(smem_u32(&c.met[i]), Sh::kShares);
     mbar_init(smem_u32(&c.drained), 1);
-    c.abort = c.redone = 0;
+    c.abort = 0;
     fence_mbar_init();
     fence_async_smem();
   }
@@ -1533,19 +1462,244 @@ __device__ __forceinline__ void load_row(const float* p, float* v) {
   }
 }
 
-// Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
-// starts at the end of CTA c's piece, a warp a row.
-constexpr int kJoinSlices = 8;
+// ---- rows computed again ----
+// A product takes 0 x NaN for a position that a row does not see, so a row can come out non-finite
+// through a position of its tiles that only other rows see.  Such a row is computed from its own
+// positions alone; one that sees a non-finite V itself, and took part in a product with no other,
+// is as the formula has it and stays.
+
+// 16 bytes of a V row: whether a value among them is Inf or NaN.
+template <bool KV8>
+__device__ __forceinline__ bool non_finite(const uint4& w) {
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    any |= KV8 ? __vcmpeq4(x[i] & 0x7f7f7f7fu, 0x7f7f7f7fu)
+               : __vcmpeq2(x[i] & 0x7f807f80u, 0x7f807f80u);
+  return any;
+}
+
+// The first position of [from, to) whose V holds Inf or NaN, or -1; by the warp.
 template <int HD, bool KV8>
-__global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
+__device__ __noinline__ int find_bad(const ChunkArgs& a, int seq, int kvh, int from, int to) {
+  constexpr int kSize = KV8 ? 1 : 2, kLanes = HD * kSize / 16;
+  constexpr int kAt = 32 / kLanes, kAhead = 8;  // positions at once, loads in flight
+  const int lane = threadIdx.x & 31;
+  const int32_t* table = a.tables + int64_t(seq) * a.table_stride;
+  const char* v = static_cast<const char*>(a.vc) + int64_t(kvh) * a.sh * kSize + lane % kLanes * 16;
+#pragma unroll 1
+  for (int c0 = from; c0 < to; c0 += kAhead * kAt) {
+    uint4 w[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int c = c0 + u * kAt + lane / kLanes;
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (c < to) {
+        const int64_t id = table[c / a.B];  // c lies within the table; bad blocks count as zeros
+        if (id >= 0 && id < a.blocks)
+          w[u] = *reinterpret_cast<const uint4*>(v + (id * a.sb + int64_t(c % a.B) * a.so) * kSize);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t hits = __ballot_sync(0xffffffffu, non_finite<KV8>(w[u]));
+      if (hits) return c0 + u * kAt + (__ffs(hits) - 1) / kLanes;
+    }
+  }
+  return -1;
+}
+
+// Row (token tok of the item, query head) from positions [lo, hi) alone, by the warp.
+template <int HD, bool KV8>
+__device__ __noinline__ void redo_row(const ChunkArgs& a, const Item& it, int tok, int head, int lo,
+                                      int hi) {
+  constexpr int kSize = KV8 ? 1 : 2;
+  constexpr int kPiece = 16 / kSize, kLanes = HD / kPiece;  // elements a lane, lanes a K row
+  constexpr int kCols = HD / 32;                            // columns of O a lane
+  constexpr int kAhead = 8;                                 // rows of K, of V in flight
+  using Words = std::conditional_t<kCols * kSize == 16, uint4,
+                                   std::conditional_t<kCols * kSize == 8, uint2, uint32_t>>;
+  const int lane = threadIdx.x & 31, sub = lane % kLanes, column = lane * kCols;
+  const int32_t* table = a.tables + int64_t(it.seq) * a.table_stride;
+  const char* const keys =
+      static_cast<const char*>(a.kc) + (int64_t(it.kvh) * a.sh + sub * kPiece) * kSize;
+  const char* const values =
+      static_cast<const char*>(a.vc) + (int64_t(it.kvh) * a.sh + column) * kSize;
+  const float qk = a.scale_log2 * (KV8 ? a.k_scale : 1.0f);
+  const int64_t token = it.tok0 + tok;
+  float q[kPiece], m = -INFINITY, l = 0.0f, acc[kCols];
+#pragma unroll
+  for (int i = 0; i < kPiece; ++i)
+    q[i] = __bfloat162float(a.q[token * a.q_t + head * a.q_h + sub * kPiece + i]);
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+  auto place = [&](int c) -> int64_t {  // bytes to position c's rows; -1: there are none
+    if (c >= hi) return -1;
+    const int64_t id = block_of(a, table, c);
+    return id < 0 ? -1 : (id * a.sb + int64_t(c % a.B) * a.so) * kSize;
+  };
+  int64_t next = place(lo + lane);
+#pragma unroll 1
+  for (int c0 = lo; c0 < hi; c0 += 32) {
+    const int64_t at = next;
+    next = place(c0 + 32 + lane);  // on its way while this one is worked on
+    // kLanes lanes take kLanes positions one after the other: lane x's own at step x % kLanes
+    float s = -INFINITY;
+#pragma unroll 1
+    for (int step0 = 0; step0 < kLanes; step0 += kAhead) {
+      uint4 w[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int64_t row = __shfl_sync(0xffffffffu, at, lane - sub + step0 + x);
+        w[x] = *reinterpret_cast<const uint4*>(keys + (row < 0 ? 0 : row));
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const uint32_t words[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+        float k[kPiece], dot = 0.0f;
+        unpack<KV8, kPiece>(words, k);
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) dot += q[i] * k[i];
+#pragma unroll
+        for (int y = kLanes / 2; y; y >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, y);
+        if (sub == step0 + x && at >= 0) s = dot * qk;
+      }
+    }
+    if (__any_sync(0xffffffffu, isnan(s))) {  // and so is every weight
+      l = s = NAN;
+      break;
+    }
+    float top = s;
+#pragma unroll
+    for (int y = 16; y; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
+    const float w = exp2f(s - base), shrink = exp2f(m - base);
+    m = m_new;
+    l = l * shrink + w;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] *= shrink;
+#pragma unroll 1
+    for (int k0 = 0; k0 < 32; k0 += kAhead) {
+      Words words[kAhead];
+      bool there[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const int64_t row = __shfl_sync(0xffffffffu, at, k0 + x);
+        there[x] = row >= 0;
+        words[x] = *reinterpret_cast<const Words*>(values + (row < 0 ? 0 : row));
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        const float wk = __shfl_sync(0xffffffffu, w, k0 + x);
+        float v[kCols];
+        unpack<KV8, kCols>(reinterpret_cast<const uint32_t*>(&words[x]), v);
+        if (there[x])  // whatever the caches' first row, read in its place, holds
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) acc[i] += wk * v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int y = 16; y; y >>= 1) l += __shfl_xor_sync(0xffffffffu, l, y);
+  const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;  // 0: it sees nothing
+  const int64_t to = int64_t(head) * HD + column;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    float y = acc[i] * inv;
+    if (a.gate) y *= load_gate(a, token * a.gate_t + to + i);
+    a.out[token * a.out_t + to + i] = __float2bfloat16_rn(y);
+  }
+}
+
+// Looks at row r of an item, which came out non-finite, and computes it again if it has to be;
+// false: it stays.  `guess`: a position that may be non-finite, for the block's warps.
+template <int HD, bool KV8>
+__device__ __noinline__ bool mend_row(const ChunkArgs& a, const Item& it, int r, volatile int* guess) {
+  const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
+  const int tok = t * a.TB + row_tok, head = it.kvh * a.G + in_tile - row_tok * a.G;
+  const int pos = it.pos0 + tok;
+  // the positions whose products the row's tile took part in, and those that the row sees
+  int first;
+  const int tiles =
+      tiles_seen(it.pos0 + t * a.TB, min(it.ntok - t * a.TB, a.TB), it.cap, a.window, first);
+  const int p0 = max(first * kN, a.window ? it.pos0 - a.window + 1 : 0);
+  const int p1 = max(min((first + tiles) * kN, min(it.pos0 + it.ntok, it.cap)), p0);
+  const int lo = min(max(a.window ? pos - a.window + 1 : 0, p0), p1);
+  const int hi = max(min(pos + 1, p1), lo);
+  if (find_bad<HD, KV8>(a, it.seq, it.kvh, p0, lo) < 0 &&
+      find_bad<HD, KV8>(a, it.seq, it.kvh, hi, p1) < 0) {
+    // The warps of a block look for it in different places; what one finds serves all.
+    const int step = (hi - lo + 15) / 16;
+    for (int i = 0; i < 16; ++i) {
+      const int g = *guess;  // never set, perhaps
+      if (g >= lo && g < hi && find_bad<HD, KV8>(a, it.seq, it.kvh, g, g + 1) >= 0) return false;
+      const int from = lo + (i + (threadIdx.x >> 5)) % 16 * step;
+      const int found = find_bad<HD, KV8>(a, it.seq, it.kvh, from, min(from + step, hi));
+      if (found < 0) continue;
+      *guess = found;
+      return false;
+    }
+    // neither: a sum that overflowed FP32 against a reference below the row's maximum
+  }
+  redo_row<HD, KV8>(a, it, tok, head, lo, hi);
+  return true;
+}
+
+constexpr int kJoinSlices = 8;
+// What a warp of join_kernel does where rows came out non-finite: it looks at its rows of the item
+// that was joined (`cut`), and of the items that CTA blockIdx.x held whole (`whole`).
+template <int HD, bool KV8>
+__device__ __noinline__ void look_through(const ChunkArgs& a, int row0, bool cut, bool whole) {
+  __shared__ int guess;
+  const int lane = threadIdx.x & 31;
+  auto rows = [&](const Item& it) {
+#pragma unroll 1
+    for (int r = row0; r < Shape<HD, KV8>::kItemRows; r += 16 * kJoinSlices) {
+      const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
+      const int tok = t * a.TB + row_tok;
+      if (in_tile >= a.TB * a.G || tok >= it.ntok || it.tok0 + tok >= a.T) continue;
+      const int64_t column = int64_t(it.kvh * a.G + in_tile - row_tok * a.G) * HD + lane * (HD / 32);
+      bool bad = false;
+#pragma unroll
+      for (int x = 0; x < HD / 32; ++x)
+        bad |= !isfinite(__bfloat162float(a.out[(it.tok0 + tok) * a.out_t + column + x]));
+      if (__any_sync(0xffffffffu, bad)) mend_row<HD, KV8>(a, it, r, &guess);
+    }
+  };
+  if (cut) {
+    const Join& j = reinterpret_cast<const Join*>(a.joins)[blockIdx.x];
+    Item it;
+    it.tok0 = j.tok0;
+    it.ntok = j.ntok;
+    it.kvh = j.kvh;
+    it.seq = j.seq;
+    it.pos0 = j.pos0;
+    it.cap = j.cap;
+    rows(it);
+  }
+  if (whole)
+    walk<HD, KV8>(a, find_piece<HD, KV8>(a, lane), [&](const Item& it, int, int) {
+      if (it.slot < 0) rows(it);
+      return true;
+    });
+}
+
+// Joins the parts of the items that were cut between CTAs: block (c, s) takes the item that
+// starts at the end of CTA c's piece, a warp a row.  Then, where one of them, or of the rows of CTA
+// c's whole items, is not finite, it looks through those.
+template <int HD, bool KV8>
+__global__ void __launch_bounds__(512, HD == 256 ? 1 : 2) join_kernel(const __grid_constant__ ChunkArgs a) {
   using Sh = Shape<HD, KV8>;
   constexpr int kPer = HD / 32;  // columns of a lane
   grid_wait();
   const int4 join = *reinterpret_cast<const int4*>(a.joins + blockIdx.x * 8);
+  const int odd = a.joins[blockIdx.x * 8 + 4];
   const int parts = join.x, tok0 = join.y, ntok = join.z, kvh = join.w;
-  if (!parts) return;
-  const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 16 + (threadIdx.x >> 5); r < Sh::kItemRows; r += 16 * kJoinSlices) {
+  if (!parts && !odd) return;
+  const int lane = threadIdx.x & 31, row0 = blockIdx.y * 16 + (threadIdx.x >> 5);
+  bool cut_odd = false;
+  for (int r = row0; parts && r < Sh::kItemRows; r += 16 * kJoinSlices) {
     const int t = r / kM, in_tile = r % kM, row_tok = in_tile / a.G;
     const int tok = t * a.TB + row_tok;
     if (in_tile >= a.TB * a.G || tok >= ntok || tok0 + tok >= a.T) continue;
@@ -1567,7 +1721,7 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
       for (int y = 0; y < 4; ++y) {
         ml[y] = make_float2(0.0f, 0.0f);
         if (i + y < parts) {
-          ml[y] = a.part_ml[slot(i + y) * Sh::kShares + lane * Sh::kShares / 32];
+          ml[y] = a.part_ml[slot(i + y)];
           load_row<kPer>(a.part_o + slot(i + y) * HD + lane * kPer, o[y]);
         }
       }
@@ -1582,12 +1736,21 @@ __global__ void __launch_bounds__(512) join_kernel(const ChunkArgs a) {
         for (int x = 0; x < kPer; ++x) acc[x] = acc[x] * keep + w * o[y][x];
       }
     }
+    float zero = 0.0f;  // NaN if a sum is not finite
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) zero = fmaf(acc[x], 0.0f, zero);
+    cut_odd |= isnan(zero) && isfinite(l);
     const float inv = l == 0.0f ? 0.0f : (KV8 ? a.v_scale : 1.0f) / l;
 #pragma unroll
     for (int x = 0; x < kPer; x += 2) {
       const float y0 = acc[x] * inv * gate[x], y1 = acc[x + 1] * inv * gate[x + 1];
       *reinterpret_cast<uint32_t*>(a.out + token * a.out_t + column + x) = pack_bf16(y0, y1);
     }
+  }
+  cut_odd = __any_sync(0xffffffffu, cut_odd);
+  if (cut_odd || odd) {
+    __syncwarp();  // the warp's stores come first
+    look_through<HD, KV8>(a, row0, cut_odd, odd);
   }
 }
 
@@ -1599,11 +1762,10 @@ struct ScratchLayout {
 };
 ScratchLayout scratch_layout(int ctas, int head_dim) {
   const int64_t rows = head_dim == 256 ? kM : 2 * kM;
-  const int64_t shares = head_dim == 256 ? kWide256 : kWide128;
   ScratchLayout s;
   s.joins = 256;  // [0, 256): header; word 0 = device error flags
   s.ml = s.joins + (int64_t(ctas) * 32 + 255) / 256 * 256;
-  s.o = s.ml + 2 * ctas * rows * shares * 8;
+  s.o = s.ml + 2 * ctas * rows * 8;
   s.total = s.o + 2 * ctas * rows * head_dim * 4;
   return s;
 }
@@ -1753,7 +1915,7 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
   if (p.scratch_bytes < need)
     return fail(DORY_ERR_INVALID_ARGUMENT, "scratch too small (%lld < %lld bytes)",
                 (long long)p.scratch_bytes, (long long)need);
-  // A row may be computed again (redo_row) after others, and a part of itself, have been stored.
+  // A row may be computed again (redo_row) after others, and itself, have been stored.
   const int64_t width = int64_t(p.num_heads) * p.head_dim, last = p.num_tokens - 1;
   const int gate_size = p.gate_dtype == DORY_DTYPE_F32 ? 4 : 2;
   if (meet(p.out, last * out_t + width, 2, p.q,

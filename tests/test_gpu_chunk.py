@@ -460,3 +460,66 @@ def test_rows_that_see_nothing_are_zero_beside_rows_that_see_a_bad_value(D, fp8,
     sees_it = torch.arange(40, device=DEV) - (10 if why == "short" else 0) >= 20
     assert out[sees_it].isnan().all() and out[~sees_it].isfinite().all()
     assert (out[(seen >= 0) & ~sees_it] != 0).any()
+
+
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+def test_one_bad_value_does_not_slow_a_prompt_down(D, fp8):
+    """Rows that see a NaN are NaN by the formula itself; only rows that share a tile with it and
+    do not see it have to be computed again."""
+    b = Batch([(2048, 2048)], NH=16, NKV=2, D=D, fp8=fp8, seed=53)
+    attn = b.attention()
+
+    def milliseconds():
+        times = []
+        for _ in range(4):
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            e[0].record()
+            b.run(attn=attn)
+            e[1].record()
+            torch.cuda.synchronize()
+            times.append(e[0].elapsed_time(e[1]))
+        return min(times[1:])
+    clean, want = milliseconds(), b.out.clone().view(b.T, b.NH, D)
+    b.value[b.tables[0, 20].long(), 5, 1, 9] = float("nan")  # position 325
+    bad, out = milliseconds(), b.out.view(b.T, b.NH, D)
+    assert out[325:, 8:, 9].isnan().all() and out[:325].isfinite().all() and out[:, :8].isfinite().all()
+    out[325:, 8:, 9] = want[325:, 8:, 9]
+    # rows computed again differ by the rounding of their weights and of the result
+    assert ((out - want).float().abs() <= 2.0 ** -6 * (want.float().abs() + 1)).all()
+    assert bad < 8 * clean, (bad, clean)
+
+
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_scattered_bad_values(D, fp8, window, seed):
+    """NaN and Inf all over V, whole items and cut ones, bad blocks and rows before the sequence:
+    every element is what the formula gives from the positions that its row sees."""
+    g = torch.Generator().manual_seed(60 + seed)
+    b = Batch([(70, 90), (3, 3), (33, 2500), (20, 12), (1, 40), (90, 300)], NH=6, NKV=2, D=D, fp8=fp8,
+              seed=60 + seed)
+    b.tables[2, 7] = b.blocks  # positions 112 to 127: with the window, none of the last rows sees them
+    for _ in range(25):
+        i = int(torch.randint(0, 6, (), generator=g))
+        n = max(int(b.seq_lens[i]) - int(torch.randint(0, 100, (), generator=g)), 1)
+        at = int(torch.randint(max(0, n - 60), n, (), generator=g))
+        block = int(b.tables[i, at // 16])
+        if 0 <= block < b.blocks:
+            bad = [float("nan"), float("inf"), -float("inf")][int(torch.randint(0, 3, (), generator=g))]
+            columns = torch.randint(0, D, (int(torch.randint(1, 4, (), generator=g)),), generator=g)
+            b.value[block, at % 16, int(torch.randint(0, 2, (), generator=g)), columns.to(DEV)] = \
+                torch.tensor(bad, device=DEV).to(b.value.dtype)
+    out = b.run(window=window, gate=b.gate, errors=0 if window else _native.DEVERR_BLOCK_OOB)
+    want, size = b.oracle(window, b.gate)
+    assert torch.equal(out.isnan(), want.isnan())
+    infinite = want.isinf()
+    assert torch.equal(out.double()[infinite], want[infinite])
+    clean = want.isfinite()
+    k = b.key.float().nan_to_num(0, 0, 0).norm(dim=-1).max().item() * b.scales[0]
+    score = (D + 4) * F32 * b.scale * b.q.float().norm(dim=-1).max().item() * k
+    rel = 2.0 ** -8 + 2 * score + 6e-6 + (8 + 2500) * F32
+    tol = rel * size + 2.0 ** -8 * want.abs() * (1 + rel) + 2.0 ** -130
+    if fp8:
+        v = b.value.float().nan_to_num(0, 0, 0).abs().max().item() * b.scales[1]
+        tol = tol + 2.0 ** -32 * 2500 * v
+    assert ((out.double() - want).abs() <= tol)[clean].all()
