@@ -86,6 +86,12 @@ def _heads(name: str, x: torch.Tensor, tokens: int, head_dim: int) -> tuple:
     return x.data_ptr(), stride[0], stride[1], shape[1]
 
 
+def _end(rows: tuple, size: int, tokens: int, dim: int) -> int:
+    """The address behind the last of `rows`, as _heads returns them."""
+    ptr, token, head, heads = rows
+    return ptr + ((tokens - 1) * token + (heads - 1) * head + dim) * size
+
+
 def _check_output(name: str, out: tuple, out_size: int, x: tuple, x_size: int, tokens: int,
                   dim: int, in_place: bool) -> None:
     """ValueError if rows of an output lie on one another, or the output over its input `x`
@@ -105,11 +111,41 @@ def _check_output(name: str, out: tuple, out_size: int, x: tuple, x_size: int, t
         if in_place:
             return
         raise ValueError(f"{name} must not be its input")
-    end = ptr + ((tokens - 1) * token + (heads - 1) * head + dim) * out_size
-    x_end = x[0] + ((tokens - 1) * x[1] + (heads - 1) * x[2] + dim) * x_size
-    if ptr < x_end and x[0] < end:
+    if ptr < _end(x, x_size, tokens, dim) and x[0] < _end(out, out_size, tokens, dim):
         raise ValueError(f"{name} must lie apart from its input" +
                          (" or be that tensor itself" if in_place else ""))
+
+
+def _meet(a: tuple, a_size: int, b: tuple, b_size: int, tokens: int, dim: int) -> bool:
+    """Whether rows of a and b, as _heads returns them, share memory; a_size, b_size: bytes of an
+    element.  Slices of one fused projection lie between one another and do not."""
+    a_ptr, a_token, a_head, a_heads = a
+    b_ptr, b_token, b_head, b_heads = b
+    if not tokens or not a_heads or not b_heads:
+        return False
+    if _end(a, a_size, tokens, dim) <= b_ptr or _end(b, b_size, tokens, dim) <= a_ptr:
+        return False
+    a_width = ((a_heads - 1) * a_head + dim) * a_size
+    b_width = ((b_heads - 1) * b_head + dim) * b_size
+    step = a_token * a_size
+    if step and step == b_token * b_size and a_width <= (b_ptr - a_ptr) % step <= step - b_width:
+        return False  # side by side in every token
+    # heads between heads, or anything else: row by row
+    starts, sizes = [], []
+    for ptr, token, head, heads, size in ((a_ptr, a_token, a_head, a_heads, a_size),
+                                          (b_ptr, b_token, b_head, b_heads, b_size)):
+        rows = (torch.arange(tokens)[:, None] * token + torch.arange(heads) * head).flatten() * size
+        starts.append(rows + ptr)
+        sizes.append(torch.full_like(rows, dim * size))
+    owner = torch.cat([torch.zeros_like(starts[0]), torch.ones_like(starts[1])])
+    start, order = torch.cat(starts).sort()
+    end, owner = start + torch.cat(sizes)[order], owner[order]
+    # the furthest that rows of either have reached before each row of the other
+    for mine in (0, 1):
+        reached = torch.where(owner == mine, end, 0).cummax(0).values
+        if ((owner[1:] != mine) & (reached[:-1] > start[1:])).any():
+            return True
+    return False
 
 
 def _table(cos_sin, positions, tokens: int, head_dim: int) -> tuple:
@@ -163,8 +199,9 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     """Rotates q [T, NH, D] and k [T, NKV, D] (or None) by the angles of positions [T] (int64
     or int32) into q_out and k_out, same shapes and type (BF16, FP16 or FP32); an output may be
     its own input itself, otherwise it must lie apart from it; the outputs lie apart from each
-    other and from the other's input.  Any token and head strides, unit last stride.  cos_sin [max_position, rotary_dim]: the first rotary_dim dims turn, pairs
-    (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1); the others are copied.  inverse: the
+    other and from the other's input.  Any token and head strides, unit last stride.  cos_sin
+    [max_position, rotary_dim]: the first rotary_dim dims turn, pairs (i, i + rotary_dim / 2) or,
+    interleaved, (2i, 2i + 1); the others are copied.  inverse: the
     rotation back.  error_word (optional int32 device tensor) collects
     DORY_DEVERR_POSITION_OOB; such a token's outputs are zero."""
     code = _IO_DTYPES.get(q.dtype)
@@ -194,6 +231,14 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if out_heads != kv_heads:
             raise ValueError("k_out must have k's heads")
         _check_output("k_out", ko_rows, size, k_rows, size, tokens, dim, True)
+        qo_end, ko_end = _end(qo_rows, size, tokens, dim), _end(ko_rows, size, tokens, dim)
+        if ((qo_ptr < _end(k_rows, size, tokens, dim) and k_ptr < qo_end
+             and _meet(qo_rows, size, k_rows, size, tokens, dim))
+                or (ko_ptr < _end(q_rows, size, tokens, dim) and q_ptr < ko_end
+                    and _meet(ko_rows, size, q_rows, size, tokens, dim))
+                or (qo_ptr < ko_end and ko_ptr < qo_end
+                    and _meet(qo_rows, size, ko_rows, size, tokens, dim))):
+            raise ValueError("the outputs must lie apart, from each other and from the other's input")
     pos_ptr, table, rotary, max_position, table_code, pos32 = _table(cos_sin, positions, tokens, dim)
     flags = ((_native.ROTARY_INTERLEAVED if interleaved else 0) |
              (_native.ROTARY_INVERSE if inverse else 0))
@@ -216,8 +261,8 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     the root), and writes k and v [T, NKV, D] to the cache views [blocks, block_size, NKV, D]
     at slot_mapping[t] (int64, as vLLM's: block * block_size + row; negative: a padding token,
     nothing is written; no slot twice).  BF16 caches, or e4m3 (float8_e4m3fn or uint8) with the
-    layer's k_scale / v_scale.  q_out: BF16 [T, NH, D] (or [T, NH * D]); q and q_out None: k
-    and v alone.  q, k, v: one type, BF16, FP16 or FP32, e.g. slices of a fused projection.
+    layer's k_scale / v_scale.  q_out: BF16 [T, NH, D] (or [T, NH * D]), apart from the
+    inputs and the caches; q and q_out None: k and v alone.  q, k, v: one type, BF16, FP16 or FP32, e.g. slices of a fused projection.
     head_dim 64, 128 or 256.  error_word (optional int32 device tensor) collects
     DORY_DEVERR_SLOT_OOB (slot beyond the cache, skipped) and DORY_DEVERR_POSITION_OOB."""
     code = _IO_DTYPES.get(k.dtype)
@@ -233,8 +278,8 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     _native.check_device_index(device, q, v, positions, cos_sin, slot_mapping, key_cache,
                                value_cache, q_out, sqk, error_word)
     tokens, _, dim = k.shape
-    k_ptr, k_t, k_h, kv_heads = _heads("k", k, tokens, dim)
-    v_ptr, v_t, v_h, v_heads = _heads("v", v, tokens, dim)
+    k_ptr, k_t, k_h, kv_heads = k_rows = _heads("k", k, tokens, dim)
+    v_ptr, v_t, v_h, v_heads = v_rows = _heads("v", v, tokens, dim)
     if v_heads != kv_heads:
         raise ValueError("v must have k's heads")
     q_ptr = q_t = q_h = qo_ptr = qo_t = qo_h = heads = 0
@@ -249,7 +294,14 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         qo_ptr, qo_t, qo_h, out_heads = qo_rows = _heads("q_out", q_out, tokens, dim)
         if out_heads != heads:
             raise ValueError("q_out must have q's heads")
-        _check_output("q_out", qo_rows, 2, q_rows, q.element_size(), tokens, dim, False)
+        size = q.element_size()
+        _check_output("q_out", qo_rows, 2, q_rows, size, tokens, dim, False)
+        qo_end = _end(qo_rows, 2, tokens, dim)
+        if ((qo_ptr < _end(k_rows, size, tokens, dim) and k_ptr < qo_end
+             and _meet(qo_rows, 2, k_rows, size, tokens, dim))
+                or (qo_ptr < _end(v_rows, size, tokens, dim) and v_ptr < qo_end
+                    and _meet(qo_rows, 2, v_rows, size, tokens, dim))):
+            raise ValueError("q_out must lie apart from k and v")
     pos_ptr, table, rotary, max_position, table_code, pos32 = _table(cos_sin, positions, tokens, dim)
     shape, stride = key_cache.shape, key_cache.stride()
     if stride != value_cache.stride() or stride[-1] != 1 or shape != value_cache.shape:
@@ -265,6 +317,13 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         kv_code = _native.DTYPE_FP8_E4M3
     else:
         raise ValueError("caches must be bfloat16, or float8_e4m3fn / uint8 for FP8")
+    key, value = key_cache.data_ptr(), value_cache.data_ptr()
+    if q is not None and tokens and shape[0] and shape[1]:
+        reach = (shape[0] - 1) * stride[0] + (shape[1] - 1) * stride[1] \
+            + (kv_heads - 1) * stride[2] + dim
+        reach *= 2 if kv_code == _native.DTYPE_BF16 else 1
+        if (qo_ptr < key + reach and key < qo_end) or (qo_ptr < value + reach and value < qo_end):
+            raise ValueError("q_out must lie apart from the caches")
     if (slot_mapping.dtype is not torch.int64 or slot_mapping.numel() < tokens
             or not slot_mapping.is_contiguous()):
         raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
@@ -278,7 +337,7 @@ def rotary_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         flags |= _native.ROTARY_INTERLEAVED
     _launch("dory_rotary_append", device, _pack(
         q_ptr, k_ptr, v_ptr, pos_ptr, table, sqk_ptr, slot_mapping.data_ptr(), qo_ptr, 0,
-        key_cache.data_ptr(), value_cache.data_ptr(), _error_ptr(error_word),
+        key, value, _error_ptr(error_word),
         q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, 0, 0, stride[0], stride[1], stride[2], shape[0],
         max_position, float(sqk_factor), float(eps), float(k_scale), float(v_scale), tokens,
         heads, kv_heads, dim, rotary, shape[1], code, table_code, pos32, sqk_code, kv_code, flags))

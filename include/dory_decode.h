@@ -363,7 +363,8 @@ int32_t dory_residual_update(const DoryResidualParams* params, void* stream);
  * (DORY_DEVERR_POSITION_OOB in error_word; not for a padding token of the append).
  *
  * dory_rotary_embed writes q_out and, where k is given, k_out, in the inputs' type; an output
- * may be its input itself (same pointer and strides).
+ * may be its input itself (same pointer and strides).  Otherwise the outputs of both calls lie
+ * apart from every input, from each other and from the caches (not checked here).
  *
  * dory_rotary_append writes q_out (BF16; q and q_out may be NULL) and the cache rows of k and
  * v at slot_mapping[t] (negative: a padding token, no row is written; outside the cache:

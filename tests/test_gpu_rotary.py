@@ -459,3 +459,36 @@ def test_normalised_rows_off_the_16_byte_grid_give_the_same_bits(interleaved):
         outs.append((key, value, q_out))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_outputs_over_other_arguments_are_refused():
+    T, NH, NKV, D = 6, 4, 2, 64
+    fused = torch.randn(T, NH + 2 * NKV, D, device=DEV).to(torch.bfloat16)
+    kept = fused.clone()
+    q, k, v = fused.split([NH, NKV, NKV], dim=1)
+    table, pos = rotary_cos_sin(8, D, device=DEV), torch.arange(T, device=DEV)
+    other = torch.empty(T, NH, D, dtype=torch.bfloat16, device=DEV)
+    cache = torch.zeros(3, 16, NKV, D, dtype=torch.bfloat16, device=DEV)
+    value = torch.zeros_like(cache)
+    for args in ((q, k, pos, table, fused[:, NH - 1:2 * NH - 1], torch.empty_like(k)),
+                 (q, k, pos, table, other, fused[:, 1:1 + NKV]),
+                 (q, k, pos, table, other, other[:, 1:1 + NKV])):
+        with pytest.raises(ValueError, match="apart"):
+            rotary_embed(*args)
+    over = cache.view(-1)[:T * NH * D].view(T, NH, D)
+    for out in (fused[:, NH:2 * NH], over, over.flatten(1)):
+        with pytest.raises(ValueError, match="apart"):
+            rotary_append(q, k, v, pos, table, pos, cache, value, out)
+    with pytest.raises(ValueError, match="apart"):
+        rotary_append(other, k, v, pos, table, pos, cache, value, fused[:, 2 * NKV:])
+    pool = torch.zeros(8, 16, NKV, D, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="apart"):  # over the end of a cache
+        rotary_append(q, k, v, pos, table, pos, pool[:3], value, pool[2:].view(-1)[16 * D:][:over.numel()]
+                      .view_as(over))
+    assert not pool.any()
+    assert torch.equal(fused, kept) and not cache.any() and not value.any()
+    rotary_append(q, k, v, pos, table, pos, pool[:3], value, pool[3:].view(-1)[:over.numel()]
+                  .view_as(over))  # right behind it
+    rotary_append(other, k, v, pos, table, pos, cache, value, q)  # beside k and v, token by token
+    assert torch.equal(fused[:, NH:], kept[:, NH:])
+    assert torch.equal(value.view(-1, NKV, D)[:T], v)

@@ -169,3 +169,50 @@ def test_host_validation(lib, append, kw, status, message):
     assert fn(ctypes.byref(p), None) == status
     assert message in lib.dory_decode_last_error().decode()
     assert fn(None, None) == _native.ERR_INVALID_ARGUMENT
+
+
+def _rows(x):
+    return _heads("x", x, x.shape[0], x.shape[2])
+
+
+def test_rows_that_share_memory_are_told_from_rows_side_by_side():
+    from dory_rotary_steps import _meet
+    T, D = 5, 8
+    fused = torch.zeros(T, 7, D)
+    q, k, v = fused.split([4, 2, 1], dim=1)
+
+    def meet(a, b):
+        got = _meet(_rows(a), a.element_size(), _rows(b), b.element_size(), T, D)
+        assert got == _meet(_rows(b), b.element_size(), _rows(a), a.element_size(), T, D)
+        return got
+    for a, b in ((q, k), (k, v), (q, v), (q, torch.zeros(T, 2, D)), (q, fused[:, 4:])):
+        assert not meet(a, b)
+    for a, b in ((q, q), (q, fused[:, 3:5]), (fused, v)):
+        assert meet(a, b)
+    # heads between heads, as one projection a head leaves them
+    each = torch.zeros(T, 4, 3, D)
+    assert not meet(each[:, :, 0], each[:, :, 1]) and not meet(each[:, :, 2], each[:, 1:, 0])
+    assert meet(each[:, :, 0], each[:, 2:, 0])
+    # tokens between tokens, and another type over the same memory
+    two = torch.zeros(2 * T, 3, D)
+    assert not meet(two[::2], two[1::2]) and meet(two[::2], two[:T])
+    wide = torch.zeros(T, 3, 2 * D)
+    half = wide.view(torch.float16)
+    assert meet(wide[..., :D], half[..., :D]) and not meet(wide[..., :D], half[..., 2 * D:3 * D])
+    assert not meet(q, fused.view(torch.bfloat16)[:, 4:, :D])
+    assert not _meet((64, 8, 8, 0), 4, _rows(k), 4, T, D)  # no heads
+    # every pair of slices of a small buffer, against the bytes themselves
+    memory = torch.zeros(64, dtype=torch.int16)
+    g = torch.Generator().manual_seed(1)
+    for _ in range(300):
+        views = []
+        for _ in range(2):
+            token, head, start = (int(torch.randint(0, n, (), generator=g)) for n in (14, 7, 20))
+            views.append(memory.as_strided((3, 2, 2), (token, head, 1), start))
+        marks = []
+        for x in views:
+            memory.zero_()
+            x.fill_(1)
+            marks.append(memory.clone().bool())
+        got = _meet(_rows(views[0]), 2, _rows(views[1]), 2, 3, 2)
+        assert got == bool((marks[0] & marks[1]).any()), [x.stride() for x in views]
