@@ -14,7 +14,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 LIBRARY = HERE / "libdory_decode.so"
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # DoryStatus
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA = range(5)
@@ -164,6 +164,8 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib = ctypes.CDLL(str(path))
     lib.dory_decode_abi_version.restype = _i32
     lib.dory_decode_abi_version.argtypes = []
+    if lib.dory_decode_abi_version() != ABI_VERSION:
+        raise RuntimeError(f"{path}: ABI version {lib.dory_decode_abi_version()} != {ABI_VERSION}")
     lib.dory_decode_params_bytes.restype = _i64
     lib.dory_decode_params_bytes.argtypes = []
     lib.dory_decode_scratch_bytes.restype = _i64
@@ -203,8 +205,6 @@ def load(path: os.PathLike | None = None) -> ctypes.CDLL:
     lib.dory_chunk_scratch_bytes.argtypes = [_i32, _i32, _i32]
     lib.dory_chunk_attention.restype = _i32
     lib.dory_chunk_attention.argtypes = [_vp, _vp]
-    if lib.dory_decode_abi_version() != ABI_VERSION:
-        raise RuntimeError(f"{path}: ABI version {lib.dory_decode_abi_version()} != {ABI_VERSION}")
     if lib.dory_decode_params_bytes() != ctypes.sizeof(DoryDecodeParams):
         raise RuntimeError(f"{path}: DoryDecodeParams is {lib.dory_decode_params_bytes()} bytes, "
                            f"the binding's is {ctypes.sizeof(DoryDecodeParams)}")

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define DORY_DECODE_ABI_VERSION 8
+#define DORY_DECODE_ABI_VERSION 9
 
 /* Status codes returned by every entry point. */
 typedef enum DoryStatus {

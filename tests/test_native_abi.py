@@ -199,3 +199,15 @@ def test_zero_token_calls_need_no_tensors(lib):
     p = _native.DoryResidualParams()
     p.num_tokens, p.hidden, p.split_k = 0, 64, 1
     assert lib.dory_residual_update(ctypes.byref(p), None) == _native.OK
+
+
+def test_an_older_library_is_refused_by_its_version(tmp_path, monkeypatch):
+    """Not by the first symbol that it lacks."""
+    import subprocess
+    (tmp_path / "old.c").write_text("int dory_decode_abi_version(void) { return 8; }\n")
+    old = tmp_path / "old.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(old), str(tmp_path / "old.c")], check=True)
+    monkeypatch.setattr(_native, "_lib", None)
+    with pytest.raises(RuntimeError, match=f"ABI version 8 != {_native.ABI_VERSION}"):
+        _native.load(old)
+    assert _native._lib is None
