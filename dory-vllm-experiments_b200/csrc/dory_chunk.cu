@@ -1911,6 +1911,8 @@ int32_t dory_chunk_attention(const DoryChunkParams* P, void* stream) {
     return fail(DORY_ERR_ALIGNMENT, "key/value caches need 16-byte aligned bases and strides");
   if (p.gate && (!aligned16(p.gate) || (gate_t & 7)))
     return fail(DORY_ERR_ALIGNMENT, "gate needs a 16-byte aligned base and rows");
+  if (!aligned16(p.scratch))
+    return fail(DORY_ERR_ALIGNMENT, "scratch needs a 16-byte aligned base");
   const int64_t need = dory_chunk_scratch_bytes(p.num_heads, p.num_kv_heads, p.head_dim);
   if (p.scratch_bytes < need)
     return fail(DORY_ERR_INVALID_ARGUMENT, "scratch too small (%lld < %lld bytes)",

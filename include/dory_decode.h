@@ -458,7 +458,7 @@ typedef struct DoryChunkParams {
   const void* gate;               /* optional [T, NH * HD] of gate_dtype                     */
   void* out;                      /* BF16 [T, NH * HD], 16-byte aligned rows; apart from q and
                                    * gate                                                    */
-  void* scratch;                  /* dory_chunk_scratch_bytes(), zeroed once by
+  void* scratch;                  /* dory_chunk_scratch_bytes(), 16-byte aligned, zeroed once by
                                    * dory_decode_scratch_init(); word 0 is the error word
                                    * (dory_decode_fetch_errors); calls that can overlap on the
                                    * GPU need a scratch each                                  */

@@ -118,3 +118,10 @@ def test_oracle_against_a_dense_softmax():
             want = torch.softmax(s.masked_fill(hide, -torch.inf), -1) @ flat_v[:, h // G]
             torch.testing.assert_close(out[:n, h * D:(h + 1) * D], want)
         assert (out[n] == 0).all() and out[n + 1].isnan().all() and (size[:n] > 0).all()
+
+
+def test_a_scratch_off_the_16_byte_grid_is_refused(lib):
+    """The join reads it 16 bytes at a time."""
+    for at in (0x1004, 0x1008):
+        assert lib.dory_chunk_attention(ctypes.byref(params(scratch=at)), None) == _native.ERR_ALIGNMENT
+        assert "scratch" in lib.dory_decode_last_error().decode()
