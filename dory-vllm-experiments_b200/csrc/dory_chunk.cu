@@ -63,6 +63,7 @@ namespace {
 
 using namespace sm100;
 using dory::aligned16;
+using dory::device_sms;
 using dory::fail;
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1768,17 +1769,6 @@ ScratchLayout scratch_layout(int ctas, int head_dim) {
   s.o = s.ml + 2 * ctas * rows * 8;
   s.total = s.o + 2 * ctas * rows * head_dim * 4;
   return s;
-}
-
-int device_sms(int* device) {  // 0 on failure
-  static int counts[64] = {0};
-  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= 64) return 0;
-  if (!counts[*device]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) == cudaSuccess)
-      counts[*device] = n;
-  }
-  return counts[*device];
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {

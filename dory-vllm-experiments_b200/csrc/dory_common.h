@@ -26,6 +26,18 @@ __attribute__((format(printf, 2, 3))) inline int32_t fail(int32_t status, const 
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// SMs of the current device, whose number goes to *device; 0 on failure.
+inline int device_sms(int* device) {
+  static int counts[64] = {0};
+  if (cudaGetDevice(device) != cudaSuccess || *device < 0 || *device >= 64) return 0;
+  if (!counts[*device]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *device) == cudaSuccess)
+      counts[*device] = n;
+  }
+  return counts[*device];
+}
+
 // The status of a kernel launch just made.
 inline int32_t launched(cudaError_t e) {
   if (e == cudaSuccess) e = cudaGetLastError();

@@ -34,7 +34,6 @@ using dory::fail;
 using namespace sm100;  // packed FP32 arithmetic
 
 constexpr int kVecThreads = 384;  // of rotary_vec, in a block at most; two blocks an SM
-constexpr int kSms = 148;
 constexpr int kMaxShared = 227 * 1024;
 
 struct Rows {  // one of q, k, v or an output
@@ -494,23 +493,23 @@ int32_t run(RotaryArgs& a, bool pieces, cudaStream_t stream) {
     return dory::launched(cudaLaunchKernelEx(&cfg, rotary_any<T, APPEND, KV8>, a));
   }
   // A block takes `group` heads of one token after the other: as many blocks as tokens while
-  // that leaves SMs idle, then about kVecThreads threads an SM, which prefetch a token ahead.
+  // that leaves SMs idle, then about 2 kVecThreads threads an SM, each with kAhead tokens in flight.
+  int device = 0;
+  const int sms = dory::device_sms(&device);
+  if (sms <= 0) return fail(DORY_ERR_CUDA, "no current CUDA device");
   const int lanes = a.D / 16;
   a.group = kVecThreads / lanes < a.heads ? kVecThreads / lanes : a.heads;
   const int parts = (a.heads + a.group - 1) / a.group;
   a.group = (a.heads + parts - 1) / parts;
   const int threads = (a.group * lanes + 31) / 32 * 32;
-  const int64_t resident = int64_t(kSms) * (2 * kVecThreads / threads);
+  const int64_t resident = int64_t(sms) * (2 * kVecThreads / threads);
   const int64_t blocks = (resident + parts - 1) / parts;
   a.run = int((a.T + blocks - 1) / blocks);
   cfg.gridDim = dim3(unsigned((a.T + a.run - 1) / a.run), unsigned(parts));
   cfg.blockDim = dim3(unsigned(threads));
   const int angles = a.R * (a.cs_dtype == DORY_DTYPE_F32 ? 4 : 2);
   cfg.dynamicSmemBytes = unsigned(kAhead * (threads * kElementBytes<T> + threads / 32 * angles));
-  int device = 0;
   static bool ready[64] = {false};
-  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64)
-    return fail(DORY_ERR_CUDA, "no current CUDA device");
   if (!ready[device]) {
     const cudaError_t e =
         cudaFuncSetAttribute(rotary_vec<T, APPEND, KV8>,

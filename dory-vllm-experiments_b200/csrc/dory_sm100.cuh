@@ -251,7 +251,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-__device__ __forceinline__ float max2(float a, float b) {
+__device__ __forceinline__ float max2(float a, float b) {  // NaN if either is
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
@@ -280,11 +280,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max2_nan(float a, float b) {  // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // 2^x for two x below 2^7 on the FP32 pipe, for when the special-function unit is the bottleneck:
 // x = n + f with n the nearest whole number, 2^f by a degree-4 polynomial (own minimax fit of
 // the relative error on [-1/2, 1/2] with p(0) = 1: 2.9e-6 in FP32), n added to the exponent.
@@ -294,7 +289,7 @@ __device__ __forceinline__ float max2_nan(float a, float b) {  // NaN if either 
 __device__ __forceinline__ void exp2_poly2(uint64_t x, float& y0, float& y1) {
   float x0, x1;
   split(x, x0, x1);
-  x = pair(max2_nan(x0, -127.0f), max2_nan(x1, -127.0f));
+  x = pair(max2(x0, -127.0f), max2(x1, -127.0f));
   const float magic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the whole number
   const uint64_t t = add2(x, pair(magic, magic));
   const uint64_t n = add2(t, pair(-magic, -magic));
