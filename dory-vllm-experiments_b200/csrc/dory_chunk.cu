@@ -35,12 +35,14 @@
 // from finite weights is looked at by the join kernel, which computes it again from its own
 // positions alone if it took part in a product with such a position without seeing it.
 //
-// What bounds it, measured (CUDA graph, 16-row pages, FP32 gate): long chunks the hand-over
-// between softmax and product warps, tile by tile (prompt of 8192, 32 query heads on 8, 128 dims:
-// 535 us, 1,025 TFLOP/s, 64% of the library GEMM's rate; no exponentials, or half of the
-// products, would save 5-13%); 256-dim heads the page copies as well (16 heads on 4: 674 us, 575
-// with 128-row pages); FP8 caches the conversion (589 us); short items their latency, 4-5 us
-// each, and a call of few tokens the chain from launch to join (4 tokens over 640: 16 us).
+// What bounds it, measured (CUDA graph, 16-row pages, FP32 gate): long chunks the length of a cache
+// tile's chain (scores, the row's maximum over all columns, the columns read again for the weights,
+// product), which two tiles in turn do not hide: no unit is full (prompt of 8192, 32 query heads on
+// 8, 128 dims: 543 us, 1,012 TFLOP/s, 63% of the library GEMM's rate; no exponentials, or half of
+// the products, would save 5-13%).  64-dim heads have the same chain for half of the products (476
+// us, 577 TFLOP/s); 256-dim heads the page copies as well (16 heads on 4: 669 us, 585 with 128-row
+// pages); FP8 caches the conversion (597 us); short items their latency, 4-5 us each, and a call of
+// few tokens the chain from launch to join (4 tokens over 640: 16.5 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

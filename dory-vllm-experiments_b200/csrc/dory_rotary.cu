@@ -4,8 +4,9 @@
 //
 // Both read every input once and write every output once, with a handful of operations per
 // element: HBM bounds a long rotation (8192 tokens of 32 + 8 heads of 128 bf16 dims: 30.9 us, 85%
-// of the measured copy rate), instruction issue and then HBM a long append (40.4 us, 78%), the
-// launch and two dependent loads (position, then table row) a single token (4.3 us).
+// of the measured copy rate), instruction issue and then HBM a long append (37.5 us; 46 with the
+// norm, whose sum is FP64, 69%), the launch and two dependent loads (position, then table row) a
+// single token (4.3 us).
 //
 // rotary_vec: a head's row belongs to head_dim / 16 neighbouring lanes.  Lane l holds two
 // 8-element pieces that contain both members of its pairs: dims 8l and rotary_dim / 2 + 8l of
@@ -14,7 +15,9 @@
 // block takes the heads of one token, then of the next: a lane keeps its head, so its share of
 // sqk stays in registers, the heads of a token share its angles in L1, and the loads of the next
 // two tokens are on their way while this one is worked on.
-// rotary_any: one warp per row, a pair per lane, for every size, stride and alignment.
+// rotary_any: one warp per row, a pair per lane, for every size, stride and alignment, with the
+// wide kernel's arithmetic to the last bit (the same rotation one element off the 16-byte grid: 142
+// us; the append 205, with the norm 329).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -213,7 +216,8 @@ __global__ void __launch_bounds__(kVecThreads, 2) rotary_vec(const RotaryArgs a)
   const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   const int angle_quads = a.R * (a.cs_dtype == DORY_DTYPE_F32 ? 4 : 2) / 16;
   // Everything that steps with the token or the place in the ring is kept and added to: address
-  // arithmetic was half of the instructions, which bound the append (8192 tokens: 40 us, 53 before).
+  // arithmetic was half of the instructions, which bound the append (8192 tokens with the norm, then in
+  // FP32: 40 us, 53 before).
   const uint32_t place_bytes = kQuads * blockDim.x * 16, angle_bytes = warps * angle_quads * 16;
   const uint32_t own = uint32_t(__cvta_generic_to_shared(ring + threadIdx.x));
   const uint32_t own_angles = uint32_t(__cvta_generic_to_shared(ring)) + kAhead * place_bytes +
