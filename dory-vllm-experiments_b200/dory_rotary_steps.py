@@ -232,12 +232,11 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
             raise ValueError("k_out must have k's heads")
         _check_output("k_out", ko_rows, size, k_rows, size, tokens, dim, True)
         qo_end, ko_end = _end(qo_rows, size, tokens, dim), _end(ko_rows, size, tokens, dim)
-        if ((qo_ptr < _end(k_rows, size, tokens, dim) and k_ptr < qo_end
-             and _meet(qo_rows, size, k_rows, size, tokens, dim))
-                or (ko_ptr < _end(q_rows, size, tokens, dim) and q_ptr < ko_end
-                    and _meet(ko_rows, size, q_rows, size, tokens, dim))
-                or (qo_ptr < ko_end and ko_ptr < qo_end
-                    and _meet(qo_rows, size, ko_rows, size, tokens, dim))):
+        if ((qo_ptr < ko_end and ko_ptr < qo_end and _meet(qo_rows, size, ko_rows, size, tokens, dim))
+                or (ko_rows != k_rows and qo_ptr < _end(k_rows, size, tokens, dim) and k_ptr < qo_end
+                    and _meet(qo_rows, size, k_rows, size, tokens, dim))
+                or (qo_rows != q_rows and ko_ptr < _end(q_rows, size, tokens, dim) and q_ptr < ko_end
+                    and _meet(ko_rows, size, q_rows, size, tokens, dim))):
             raise ValueError("the outputs must lie apart, from each other and from the other's input")
     pos_ptr, table, rotary, max_position, table_code, pos32 = _table(cos_sin, positions, tokens, dim)
     flags = ((_native.ROTARY_INTERLEAVED if interleaved else 0) |
