@@ -523,3 +523,41 @@ def test_scattered_bad_values(D, fp8, window, seed):
         v = b.value.float().nan_to_num(0, 0, 0).abs().max().item() * b.scales[1]
         tol = tol + 2.0 ** -32 * 2500 * v
     assert ((out.double() - want).abs() <= tol)[clean].all()
+
+
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, False), (256, False), (128, True), (256, True)])
+def test_bad_values_among_many_sequences_and_in_a_replay(D, fp8):
+    """More sequences than a warp looks at once, several whole items an SM, and values that turn bad
+    between the capture of a graph and its replay."""
+    g = torch.Generator().manual_seed(70)
+    lens = [(int(n), int(n + x)) for n, x in zip(torch.randint(1, 40, (150,), generator=g),
+                                                 torch.randint(0, 200, (150,), generator=g))]
+    b = Batch(lens, NH=4, NKV=2, D=D, fp8=fp8, seed=71)
+    attn = b.attention()
+    first = b.run(attn=attn, gate=b.gate).clone()
+    b.check(first, gate=b.gate)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attn(b.q, b.key, b.value, b.tables, b.query_start, b.seq_lens, 0, b.scale, b.out, gate=b.gate,
+             k_scale=b.scales[0], v_scale=b.scales[1])
+    spoilt = torch.zeros(b.T, b.NH, D, dtype=torch.bool)
+    for i in range(0, 150, 3):  # every third sequence: a position of its chunk, one column
+        n, length = lens[i]
+        at = length - 1 - int(torch.randint(0, n, (), generator=g))
+        column, head = int(torch.randint(0, D, (), generator=g)), i // 3 % 2
+        b.value[b.tables[i, at // 16].long(), at % 16, head, column] = float("nan")
+        start = int(b.query_start[i])
+        spoilt[start + at - (length - n):start + n, 2 * head:2 * head + 2, column] = True
+    spoilt = spoilt.view(b.T, -1).to(DEV)
+    b.out.fill_(5.0)
+    graph.replay()
+    replayed = b.out.clone()
+    assert torch.equal(replayed.isnan(), spoilt)
+    # the others as before, but for the rounding of rows that were computed again
+    off = (replayed.float() - first.float()).abs()[~spoilt]
+    assert (off <= 2.0 ** -6 * (first.float().abs() + 1)[~spoilt]).all()
+    again = b.run(attn=attn, gate=b.gate)
+    assert torch.equal(again.isnan(), spoilt) and torch.equal(again[~spoilt], replayed[~spoilt])
+    whole = torch.tensor([i % 3 != 0 for i in range(150)]).repeat_interleave(
+        torch.tensor([n for n, _ in lens])).to(DEV)
+    assert torch.equal(replayed[whole], first[whole])
